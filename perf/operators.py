@@ -1,0 +1,674 @@
+"""The serving operators on a paged 8-bit KV cache: what is measured of them.
+
+Four operators, each as a serving loop calls it, on the attention geometry that
+the framework serves (32 query heads of 128, groups of 1 to 8 per kv head):
+
+  pages    block tables and slot maps of a step built on the GPU from the
+           requests' lengths, and the step rolled back again
+  rotary   rotary positions of q and k, each token at its own position
+  append   k and v of a step into pages of 64 tokens held in e4m3, one power
+           of two scale per page and kv head for k and for v; q and k rotated
+           on the way
+  attend   attention of a step's query tokens over that cache
+
+With ``own`` false they are computed by elementary torch operations in 32 bits
+(angles in 64); with ``own`` true by ``oi2.PagedKVCache`` and ``oi2.Rotary``.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+N_Q = 32
+HEAD = 128
+PAGE = 64
+E4M3_MAX = 448.0
+E_MIN, E_MAX = -40, 60
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+# ── the cases ────────────────────────────────────────────────────────────────
+
+def listed():
+    return [
+        # the smallest step of a serving loop: eight chats, a token each
+        {"name": "pages_step_8", "op": "pages", "seqs": 8, "past_lo": 100, "past_hi": 3000, "new_lo": 1, "new_hi": 1,
+         "idle": 0, "tight": False},
+        # a large server's admission step: prompts of many lengths beside running requests and idle rows
+        {"name": "pages_admit_700", "op": "pages", "seqs": 700, "past_lo": 1, "past_hi": 8000, "new_lo": 1, "new_hi": 1500,
+         "idle": 5, "tight": False},
+        # the tokens of 16 sequences decoding together, a context extended fourfold
+        {"name": "rotary_step_16", "op": "rotary", "tokens": 16, "far": 32000, "n_kv": 8, "dtype": "fp16",
+         "layout": "half", "part": 128, "scaling": "wavelength"},
+        # a long prompt of a model with interleaved pairs that rotates half of each head
+        {"name": "rotary_prompt_12001", "op": "rotary", "tokens": 12001, "far": 131000, "n_kv": 8, "dtype": "bf16",
+         "layout": "interleaved", "part": 64, "scaling": "yarn"},
+        # one decoding step of 16 sequences: a token each into pages partly filled
+        {"name": "append_step_16", "op": "append", "seqs": 16, "past_lo": 30, "past_hi": 900, "new_lo": 1, "new_hi": 1,
+         "idle": 0, "n_kv": 8, "dtype": "fp16", "layout": "half", "part": 128, "scaling": "none"},
+        # prompts of several requests, odd lengths, behind short cached prefixes
+        {"name": "append_prompts_7", "op": "append", "seqs": 7, "past_lo": 1, "past_hi": 200, "new_lo": 300, "new_hi": 2500,
+         "idle": 0, "n_kv": 8, "dtype": "bf16", "layout": "half", "part": 128, "scaling": "linear"},
+        # drafts of four tokens of a model with a kv head for each query head, part of the head rotated in pairs
+        {"name": "append_drafts_40", "op": "append", "seqs": 40, "past_lo": 5, "past_hi": 300, "new_lo": 4, "new_hi": 4,
+         "idle": 0, "n_kv": 32, "dtype": "fp16", "layout": "interleaved", "part": 96, "scaling": "ntk"},
+        # the smallest: one chat's next token
+        {"name": "attend_step_1", "op": "attend", "seqs": 1, "past_lo": 700, "past_hi": 700, "new_lo": 1, "new_hi": 1,
+         "idle": 0, "n_kv": 8, "dtype": "fp16"},
+        # a server's decoding step: ragged contexts, a padded batch with idle rows
+        {"name": "attend_step_56", "op": "attend", "seqs": 56, "past_lo": 300, "past_hi": 14000, "new_lo": 1, "new_hi": 1,
+         "idle": 7, "n_kv": 8, "dtype": "fp16"},
+        # few sequences over very long contexts, eight query heads a kv head
+        {"name": "attend_long_3", "op": "attend", "seqs": 3, "past_lo": 40000, "past_hi": 110000, "new_lo": 1, "new_hi": 1,
+         "idle": 0, "n_kv": 4, "dtype": "bf16"},
+        # a whole prompt at once, no cache before it
+        {"name": "attend_prompt_5000", "op": "attend", "seqs": 1, "past_lo": 0, "past_hi": 0, "new_lo": 5000, "new_hi": 5000,
+         "idle": 0, "n_kv": 8, "dtype": "fp16"},
+        # chunks of prompts on their caches beside single decoding tokens
+        {"name": "attend_mixed_9", "op": "attend", "seqs": 9, "past_lo": 500, "past_hi": 9000, "new_lo": 1, "new_hi": 900,
+         "idle": 0, "n_kv": 8, "dtype": "bf16"},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def _range(rng, lo, hi):
+    a, b = sorted((_log_int(rng, lo, hi), _log_int(rng, lo, hi)))
+    return a, b
+
+
+def draw(rng):
+    op = rng.choice(["pages", "rotary", "append", "append", "attend", "attend", "attend", "attend"])
+    dtype = rng.choice(["fp16", "bf16"])
+    rope = {"layout": rng.choice(["half", "interleaved"]), "part": rng.choice([32, 64, 96, 128, 128]),
+            "scaling": rng.choice(["none", "linear", "ntk", "wavelength", "yarn"])}
+    n_kv = rng.choice([4, 8, 8, 16, 32])
+    if op == "rotary":
+        return {"op": op, "tokens": _log_int(rng, 1, 12000), "far": _log_int(rng, 1000, 131000), "n_kv": n_kv,
+                "dtype": dtype, **rope}
+    if op == "pages":
+        a, b = _range(rng, 1, 8000)
+        lo, hi = rng.choice([(1, 1), (1, 8), _range(rng, 1, 1000)])
+        return {"op": op, "seqs": _log_int(rng, 1, 700), "past_lo": a, "past_hi": b, "new_lo": lo, "new_hi": hi,
+                "idle": rng.choice([0, 3, 6]), "tight": rng.random() < 0.3}
+    if op == "append":
+        a, b = _range(rng, 1, 600)
+        lo, hi = rng.choice([(1, 1), (2, 6), _range(rng, 10, 2000)])
+        seqs = _log_int(rng, 1, max(1, min(64, 10000 // hi)))
+        return {"op": op, "seqs": seqs, "past_lo": a, "past_hi": b, "new_lo": lo, "new_hi": hi, "idle": rng.choice([0, 4]),
+                "n_kv": n_kv, "dtype": dtype, **rope}
+    kind = rng.choice(["step", "step", "drafts", "prompt", "mixed"])
+    if kind in ("step", "drafts"):
+        a, b = _range(rng, 50, 30000)
+        lo, hi = (1, 1) if kind == "step" else (2, rng.choice([3, 5, 8]))
+        seqs = _log_int(rng, 1, max(1, min(56, 1800000 // (b * n_kv))))
+    elif kind == "prompt":
+        a, b = 0, 0
+        lo, hi = _range(rng, 20, 3500)
+        seqs = _log_int(rng, 1, max(1, min(8, (3500 // hi) ** 2)))
+    else:
+        a, b = _range(rng, 100, 8000)
+        lo, hi = 1, _log_int(rng, 30, 800)
+        seqs = rng.randint(2, 8)
+    return {"op": op, "seqs": seqs, "past_lo": a, "past_hi": b, "new_lo": lo, "new_hi": hi, "idle": rng.choice([0, 3]),
+            "n_kv": n_kv, "dtype": dtype}
+
+
+# ── inputs ───────────────────────────────────────────────────────────────────
+
+def _spread(lo, hi, n, turn):
+    """n lengths from lo to hi, spread over their logarithm, in no order."""
+    if n == 1 or lo == hi:
+        return [hi] * n
+    return [int(round(max(lo, 1) * (hi / max(lo, 1)) ** ((turn + i * 0.6180339887) % 1.0))) for i in range(n)]
+
+
+def _lengths(case):
+    """(past, new) of every row; with ``idle`` = k every k-th row has no token in the step."""
+    n, idle = case["seqs"], case["idle"]
+    past = _spread(case["past_lo"], case["past_hi"], n, 0.999)
+    new = _spread(case["new_lo"], case["new_hi"], n, 0.2)
+    if idle and n > 1:
+        new = [0 if i % idle == idle - 1 else t for i, t in enumerate(new)]
+    return past, new
+
+
+def _pages(n):
+    return (n + PAGE - 1) // PAGE
+
+
+def _generator(seed):
+    return torch.Generator(device="cuda").manual_seed(int(seed))
+
+
+def _values(g, tokens, heads, dtype):
+    """Keys and values as projections leave them: each head and channel its own spread, a few channels large."""
+    spread = torch.exp(0.7 * torch.randn((heads, HEAD), generator=g, device="cuda"))
+    return (torch.randn((tokens, heads, HEAD), generator=g, device="cuda") * spread).to(dtype)
+
+
+def _fused_qkv(g, tokens, n_kv, dtype):
+    """q, k, v as slices of one projection's output."""
+    x = torch.cat([torch.randn((tokens, N_Q, HEAD), generator=g, device="cuda").to(dtype),
+                   _values(g, tokens, 2 * n_kv, dtype)], dim=1)
+    return x[:, :N_Q], x[:, N_Q:N_Q + n_kv], x[:, N_Q + n_kv:]
+
+
+SCALING = {
+    "none": None,
+    "linear": {"type": "linear", "factor": 4.0},
+    "ntk": {"type": "ntk", "factor": 8.0},
+    "wavelength": {"type": "wavelength", "factor": 8.0, "original_len": 8192, "low_factor": 1.0, "high_factor": 4.0},
+    "yarn": {"type": "yarn", "factor": 16.0, "original_len": 8192, "beta_fast": 32.0, "beta_slow": 1.0},
+}
+THETA = 500000.0
+
+
+def _frequencies(case):
+    """(angles per position in float64, magnitude) of the plain form."""
+    rot, s = case["part"], SCALING[case["scaling"]]
+    theta, kind = THETA, s and s["type"]
+    if kind == "ntk":
+        theta = theta * s["factor"] ** (rot / (rot - 2))
+    f = theta ** (-torch.arange(rot // 2, dtype=torch.float64, device="cuda") * 2 / rot)
+    if kind == "linear":
+        f = f / s["factor"]
+    elif kind == "wavelength":
+        turns = s["original_len"] * f / (2 * math.pi)
+        keep = ((turns - s["low_factor"]) / (s["high_factor"] - s["low_factor"])).clamp(0, 1)
+        f = f * keep + f / s["factor"] * (1 - keep)
+    elif kind == "yarn":
+        at = [rot * math.log(s["original_len"] / (b * 2 * math.pi)) / (2 * math.log(theta))
+              for b in (s["beta_fast"], s["beta_slow"])]
+        lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rot - 1)
+        keep = 1 - ((torch.arange(rot // 2, dtype=torch.float64, device="cuda") - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+        f = f * keep + f / s["factor"] * (1 - keep)
+    return f, (0.1 * math.log(s["factor"]) + 1.0) if kind == "yarn" else 1.0
+
+
+def _inputs(case, seed):
+    """What both sides and the 64-bit results start from."""
+    g = _generator(seed)
+    if case["op"] == "rotary":
+        q, k, _ = _fused_qkv(g, case["tokens"], case["n_kv"], DTYPES[case["dtype"]])
+        pos = torch.randint(0, case["far"], (case["tokens"],), generator=g, device="cuda", dtype=torch.int32)
+        return {"q": q, "k": k, "pos": pos}
+    past, new = _lengths(case)
+    total = [_pages(a + b) for a, b in zip(past, new)]
+    d = {"past": past, "new": new, "width": max(_pages(max(past) + max(new)), 1)}
+    if case["op"] == "pages":
+        held = sum(_pages(a) for a in past)
+        spare = sum(total) - held
+        d["n_pages"] = held + (spare * 2 // 3 if case["tight"] else spare + 5)
+    else:
+        d["n_pages"] = sum(total) + 3
+        dtype = DTYPES[case["dtype"]]
+        d["past_k"] = _values(g, sum(past), case["n_kv"], dtype)
+        d["past_v"] = _values(g, sum(past), case["n_kv"], dtype)
+        d["q"], d["k"], d["v"] = _fused_qkv(g, sum(new), case["n_kv"], dtype)
+    # a pool that has run for a while hands its pages out in no order
+    d["free"] = torch.randperm(d["n_pages"], generator=g, device="cuda").to(torch.int32)
+    return d
+
+
+# ── states ───────────────────────────────────────────────────────────────────
+
+def _ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def prepare(case, seed):
+    d = _inputs(case, seed)
+    if case["op"] == "rotary":
+        return {"case": case, **d, **({"rotary": _own_rotary(case)} if own else {})}
+    return _own_state(case, d) if own else _plain_state(case, d)
+
+
+def _plain_state(case, d):
+    n, width = case["seqs"], d["width"]
+    s = {"case": case, "n": n, "width": width, "n_tokens": sum(d["new"]), "max_new": max(max(d["new"]), 1),
+         "past": _ints(d["past"]), "new": _ints(d["new"]), "free": d["free"].clone(),
+         "n_free": torch.tensor([d["n_pages"]], dtype=torch.int32, device="cuda"),
+         "table": torch.full((n, width), -1, dtype=torch.int32, device="cuda"),
+         "lens": torch.zeros(n, dtype=torch.int32, device="cuda"), "max_len": width * PAGE}
+    s["step"] = _plain_extend(s, s["past"], sum(d["past"]))
+    if case["op"] == "pages":
+        return s
+    n_kv = case["n_kv"]
+    s["k_codes"], s["v_codes"] = (torch.zeros((d["n_pages"], n_kv, PAGE, HEAD), device="cuda").to(torch.float8_e4m3fn)
+                                  for _ in range(2))
+    s["k_scale"], s["v_scale"] = (torch.full((d["n_pages"], n_kv), 2.0 ** E_MIN, device="cuda") for _ in range(2))
+    _plain_store(s, d["past_k"], d["past_v"])
+    s["step"] = _plain_extend(s, s["new"], sum(d["new"]))
+    s["q"], s["k"], s["v"] = d["q"], d["k"], d["v"]
+    if case["op"] == "attend":
+        _plain_store(s, d["k"], d["v"])
+    return s
+
+
+def _oi2():
+    at = os.path.join(os.getcwd(), "hot-cold-neural-split-openinfer2_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    import oi2
+    return oi2
+
+
+def _own_rotary(case):
+    return _oi2().Rotary(HEAD, THETA, rotary_dim=case["part"], layout=case["layout"], scaling=SCALING[case["scaling"]],
+                         device="cuda")
+
+
+def _own_state(case, d):
+    # a table without room for pages of k and v serves for the page operator's own case
+    n_kv = case.get("n_kv", 1)
+    cache = _oi2().PagedKVCache(1 if case["op"] != "pages" else 0, N_Q, n_kv, case["seqs"], d["width"] * PAGE, d["n_pages"],
+                                device="cuda")
+    cache.free.copy_(d["free"])
+    first = cache.new_plan(max(sum(d["past"]), 1))
+    cache.extend(_ints(d["past"]), first)
+    s = {"case": case, "cache": cache, "past": _ints(d["past"]), "new": _ints(d["new"]),
+         "plan": cache.new_plan(max(sum(d["new"]), 1), max_new=max(max(d["new"]), 1))}
+    if case["op"] == "pages":
+        return s
+    if sum(d["past"]):
+        cache.append(0, d["past_k"], d["past_v"], first)
+    cache.extend(s["new"], s["plan"])
+    s["q"], s["k"], s["v"] = d["q"], d["k"], d["v"]
+    if case["op"] == "attend":
+        cache.append(0, d["k"], d["v"], s["plan"])
+    else:
+        s["rotary"] = _own_rotary(case)
+    return s
+
+
+# ── one pass ─────────────────────────────────────────────────────────────────
+
+def run(s):
+    op = s["case"]["op"]
+    if own:
+        return {"pages": _own_pages, "rotary": _own_rotate, "append": _own_append, "attend": _own_attend}[op](s)
+    return {"pages": _plain_pages, "rotary": _plain_rotate, "append": _plain_append, "attend": _plain_attend}[op](s)
+
+
+def _own_pages(s):
+    cache, plan = s["cache"], s["plan"]
+    cache.extend(s["new"], plan)
+    cache.rewind(s["past"])
+    return {"cu": plan.cu, "positions": plan.positions, "slots": plan.slots, "seen": plan.kv_len, "rejected": plan.rejected,
+            "lens": cache.lens, "table": cache.block_table, "free": cache.free, "n_free": cache.n_free}
+
+
+def _own_rotate(s):
+    q, k = s["rotary"](s["q"], s["k"], s["pos"])
+    return {"q": q, "k": k}
+
+
+def _own_append(s):
+    cache = s["cache"]
+    q = cache.append(0, s["k"], s["v"], s["plan"], q=s["q"], rotary=s["rotary"])
+    (k, v), (ks, vs) = cache.codes(0), cache.scales(0)
+    return {"q": q, "k": k, "v": v, "k_scale": ks, "v_scale": vs}
+
+
+def _own_attend(s):
+    return {"out": s["cache"].attend(0, s["q"], s["plan"])}
+
+
+# ── the plain forms ──────────────────────────────────────────────────────────
+
+def _pages_of(n):
+    return (n + PAGE - 1).div(PAGE, rounding_mode="floor")
+
+
+def _plain_extend(s, new, n_tokens):
+    """Rows grow by ``new`` tokens: pages from the free stack's top in row order, and where every token goes."""
+    past, width, lens = s["lens"].long(), s["width"], s["lens"]
+    new = new.long()
+    end = new.cumsum(0)
+    fits = (past + new <= s["max_len"]) & (end <= n_tokens)
+    need = torch.where(fits, _pages_of(past + new) - _pages_of(past), 0)
+    upto = need.cumsum(0)
+    n_free = s["n_free"].long()
+    taken = fits & ((need == 0) | (upto <= n_free))
+    seen = torch.where(taken, past + new, 0)
+    # table entry j of row i: the row's (j - pages held)-th new page
+    j = torch.arange(width, device="cuda")[None, :]
+    at = j - _pages_of(past)[:, None]
+    fresh = taken[:, None] & (at >= 0) & (at < need[:, None])
+    place = (n_free - 1 - (upto - need)[:, None] - at).clamp(0, s["free"].numel() - 1)
+    s["table"] = torch.where(fresh, s["free"][place], s["table"])
+    s["n_free"] = (n_free - torch.where(taken, need, 0).sum()).int()
+    s["lens"] = torch.where(taken, past + new, past).int()
+    t = torch.arange(max(n_tokens, 1), device="cuda")
+    row = torch.searchsorted(end, t, right=True).clamp(max=lens.numel() - 1)
+    pos = past[row] + t - (end - new)[row]
+    real = (t < end[-1]) & taken[row]
+    page = s["table"][row, torch.where(real, pos, 0).div(PAGE, rounding_mode="floor")]
+    return {"cu": torch.cat([torch.zeros_like(end[:1]), end]).int(), "row": row, "past": past,
+            "positions": torch.where(real, pos, -1).int(), "slots": torch.where(real, page * PAGE + pos % PAGE, -1).int(),
+            "seen": seen.int(), "rejected": (~taken).int()}
+
+
+def _plain_pages(s):
+    held = {k: s[k] for k in ("table", "n_free", "lens", "free")}
+    p = _plain_extend(s, s["new"], max(s["n_tokens"], 1))
+    # rolled back to the former lengths: the pages return to the stack in the order that undoes the step
+    lens, back = s["lens"].long(), torch.minimum(s["past"], s["lens"]).long()
+    freed = _pages_of(lens) - _pages_of(back)
+    before = freed.cumsum(0) - freed
+    j = torch.arange(s["width"], device="cuda")[None, :]
+    at = j - _pages_of(back)[:, None]
+    gone = (at >= 0) & (at < freed[:, None])
+    top = s["n_free"].long() + freed.sum()
+    place = torch.where(gone, top - 1 - before[:, None] - at, s["free"].numel())
+    free = torch.cat([s["free"], s["free"][:1]]).scatter(0, place.reshape(-1), s["table"].reshape(-1))[:-1]
+    out = {"cu": p["cu"], "positions": p["positions"], "slots": p["slots"], "seen": p["seen"], "rejected": p["rejected"],
+           "lens": back.int(), "table": torch.where(gone, -1, s["table"]), "free": free, "n_free": top.int()}
+    s.update(held)
+    return out
+
+
+def _turned(x, cos, sin, layout, part):
+    """x (tokens, heads, 128) rotated: cos, sin (tokens, 1, part / 2) in 32 bits."""
+    x = x.float()
+    a, b = (x[..., :part // 2], x[..., part // 2:part]) if layout == "half" else (x[..., 0:part:2], x[..., 1:part:2])
+    c, d = a * cos - b * sin, a * sin + b * cos
+    y = torch.cat([c, d], -1) if layout == "half" else torch.stack([c, d], -1).flatten(-2)
+    return torch.cat([y, x[..., part:]], -1)
+
+
+def _plain_tables(case, pos):
+    f, magnitude = _frequencies(case)
+    angle = pos.double()[:, None, None] * f
+    return (angle.cos() * magnitude).float(), (angle.sin() * magnitude).float()
+
+
+def _plain_rotate(s):
+    case = s["case"]
+    cos, sin = _plain_tables(case, s["pos"])
+    return {k: _turned(s[k], cos, sin, case["layout"], case["part"]).to(s[k].dtype) for k in ("q", "k")}
+
+
+def _exponent(amax):
+    """The smallest e in [E_MIN, E_MAX] with amax <= 448 2^e."""
+    m, x = torch.frexp(amax)                       # amax = m 2^x, 0.5 <= m < 1; 448 = 0.875 2^9
+    e = x - 9 + (m > 0.875)
+    return torch.where(amax > 0, e, E_MIN).clamp(E_MIN, E_MAX)
+
+
+def _plain_store(s, k, v):
+    """New tokens into their pages: a page's scale grows with its largest value, what it holds is coded again."""
+    if k.shape[0] == 0:
+        return
+    p, n = s["step"], s["n"]
+    width = s["width"]
+    # every page of the tables that the step touches, as (rows, width)
+    j = torch.arange(width, device="cuda")[None, :] * PAGE
+    lo = p["past"][:, None] - j                    # positions of the page that were held before
+    hi = p["seen"].long()[:, None] - j
+    row, page = torch.nonzero((hi > 0) & (lo < PAGE) & (p["past"] < p["seen"])[:, None], as_tuple=True)
+    at = torch.arange(PAGE, device="cuda")
+    held, upto = lo[row, page].clamp(min=0), hi[row, page]
+    old = at < held[:, None]
+    fresh = ~old & (at < upto[:, None])
+    token = p["cu"].long()[row][:, None] + page[:, None] * PAGE + at - p["past"][row][:, None]
+    token = torch.where(fresh, token, 0)
+    ids = s["table"][row, page].long()
+    for name, x in (("k", k), ("v", v)):
+        codes, scale = s[name + "_codes"], s[name + "_scale"]
+        new = x.float()[token].transpose(1, 2)     # (pages, heads, 64, 128)
+        new = torch.where(fresh[:, None, :, None], new, 0.0)
+        e = _exponent(new.abs().nan_to_num(0.0, 0.0, 0.0).amax((2, 3)))
+        before = torch.frexp(scale[ids])[1] - 1
+        e = torch.where(held[:, None] > 0, torch.maximum(e, before), e)
+        unit = torch.exp2(e.double())
+        kept = codes.view(torch.uint8)[ids].view(torch.float8_e4m3fn)
+        again = (kept.float() * torch.exp2((before - e).double()).float()[..., None, None]).to(torch.float8_e4m3fn)
+        coded = new / unit.float()[..., None, None]
+        coded = torch.where(coded.abs() <= E4M3_MAX, coded, float("nan")).to(torch.float8_e4m3fn)
+        out = torch.where(old[:, None, :, None], again.view(torch.uint8), kept.view(torch.uint8))
+        codes.view(torch.uint8)[ids] = torch.where(fresh[:, None, :, None], coded.view(torch.uint8), out)
+        scale[ids] = unit.float()
+
+
+def _plain_append(s):
+    case = s["case"]
+    cos, sin = _plain_tables(case, s["step"]["positions"])
+    q, k = (_turned(s[x], cos, sin, case["layout"], case["part"]).to(s[x].dtype) for x in ("q", "k"))
+    _plain_store(s, k, s["v"])
+    return {"q": q, "k": s["k_codes"], "v": s["v_codes"], "k_scale": s["k_scale"], "v_scale": s["v_scale"]}
+
+
+def _plain_attend(s):
+    case, p, n = s["case"], s["step"], s["n"]
+    n_kv, m, width = case["n_kv"], s["max_new"], s["width"]
+    ids = s["table"].clamp(min=0).long()
+
+    def rows(name):                                # (rows, heads, width * 64, 128)
+        x = s[name + "_codes"].view(torch.uint8)[ids].view(torch.float8_e4m3fn).float()
+        x = x * s[name + "_scale"][ids][..., None, None]
+        return x.transpose(1, 2).reshape(n, n_kv, width * PAGE, HEAD)
+
+    # the packed query tokens as (rows, most tokens of a row)
+    t = torch.arange(m, device="cuda")
+    cu = p["cu"].long()
+    real = t < (cu[1:] - cu[:-1])[:, None]
+    index = torch.where(real, cu[:-1, None] + t, 0)
+    q = s["q"].float()[index].reshape(n, m, n_kv, N_Q // n_kv, HEAD).permute(0, 2, 3, 1, 4).reshape(n, n_kv, -1, HEAD)
+    pos = torch.arange(width * PAGE, device="cuda")
+    seen = real[..., None] & (pos <= p["past"][:, None, None] + t[:, None]) & (pos < p["seen"][:, None, None])
+    score = torch.matmul(q * HEAD ** -0.5, rows("k").transpose(2, 3)).reshape(n, N_Q, m, -1)
+    score = torch.where(seen[:, None], score, float("-inf"))
+    top = score.amax(-1, keepdim=True)
+    weight = torch.exp(score - torch.where(top == float("-inf"), 0.0, top))
+    total = weight.sum(-1, keepdim=True)
+    out = torch.matmul(weight.reshape(n, n_kv, -1, width * PAGE), rows("v")).reshape(n, N_Q, m, HEAD)
+    out = torch.where(total > 0, out / total, 0.0).transpose(1, 2)
+    y = torch.empty(s["q"].shape, dtype=s["q"].dtype, device="cuda")
+    y[index[real]] = out[real].to(y.dtype)
+    return {"out": y}
+
+
+# ── least work ───────────────────────────────────────────────────────────────
+
+def work(case):
+    if case["op"] == "rotary":
+        values = case["tokens"] * (N_Q + case["n_kv"]) * HEAD
+        turned = case["tokens"] * (N_Q + case["n_kv"]) * case["part"]
+        return {"bytes": 4 * values + 4 * case["tokens"], "flops": 3 * turned}
+    past, new = _lengths(case)
+    if case["op"] == "pages":
+        # lengths in, table entries, sums, positions and slots out, and the rolled back state
+        fresh = sum(_pages(a + b) - _pages(a) for a, b in zip(past, new))
+        return {"bytes": 4 * (6 * len(past) + 4 * fresh + 2 * sum(new)), "flops": 4 * sum(new) + 8 * len(past)}
+    n_kv, tokens = case["n_kv"], sum(new)
+    if case["op"] == "append":
+        kv = 2 * tokens * n_kv * HEAD
+        return {"bytes": 3 * kv + 4 * tokens * N_Q * HEAD,
+                "flops": 3 * tokens * (N_Q + n_kv) * case["part"] + 2 * kv}
+    read = sum(a + b for a, b in zip(past, new) if b)
+    pairs = sum(b * a + b * (b + 1) // 2 for a, b in zip(past, new))
+    return {"bytes": 2 * read * n_kv * HEAD + 4 * tokens * N_Q * HEAD, "flops": 4 * pairs * N_Q * HEAD}
+
+
+# ── results in 64 bits, from the definitions ─────────────────────────────────
+
+def _angles64(case, positions):
+    rot, s = case["part"], SCALING[case["scaling"]] or {"type": "none"}
+    base = THETA if s["type"] != "ntk" else THETA * s["factor"] ** (rot / (rot - 2.0))
+    freqs = []
+    for i in range(rot // 2):
+        f = base ** (-2.0 * i / rot)
+        if s["type"] == "linear":
+            f /= s["factor"]
+        elif s["type"] == "wavelength":
+            wave, short = 2 * math.pi / f, s["original_len"] / s["high_factor"]
+            if wave > s["original_len"] / s["low_factor"]:
+                f /= s["factor"]
+            elif wave > short:
+                w = (s["original_len"] / wave - s["low_factor"]) / (s["high_factor"] - s["low_factor"])
+                f = (1 - w) * f / s["factor"] + w * f
+        elif s["type"] == "yarn":
+            def dim(turns):
+                return rot * math.log(s["original_len"] / (turns * 2 * math.pi)) / (2 * math.log(base))
+            lo, hi = max(math.floor(dim(s["beta_fast"])), 0), min(math.ceil(dim(s["beta_slow"])), rot - 1)
+            ramp = min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0)
+            f = f / s["factor"] * ramp + f * (1 - ramp)
+        freqs.append(f)
+    return positions.double()[:, None] * torch.tensor(freqs, dtype=torch.float64, device="cuda")
+
+
+def _turn64(x, angle, case):
+    mag = 0.1 * math.log(SCALING["yarn"]["factor"]) + 1.0 if case["scaling"] == "yarn" else 1.0
+    y, rot = x.double().clone(), case["part"]
+    for i in range(rot // 2):
+        a, b = (i, i + rot // 2) if case["layout"] == "half" else (2 * i, 2 * i + 1)
+        z = torch.complex(x[..., a].double(), x[..., b].double())
+        z = z * torch.polar(torch.full_like(angle[:, i], mag), angle[:, i])[:, None]
+        y[..., a], y[..., b] = z.real, z.imag
+    return y
+
+
+def _two64(e):
+    """2^e in float64 for whole e, to the bit (pow and exp2 may be off by one)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def _code64(x, e):
+    """The e4m3 number nearest to x / 2^e, ties to even, as float64."""
+    y = x / _two64(e)
+    step = _two64((torch.frexp(y.abs().clamp(min=2.0 ** -6))[1] - 1) - 3)
+    return torch.round(y / step) * step
+
+
+def _e64(block):
+    top = float(block.abs().max())
+    if top == 0:
+        return E_MIN
+    e = math.ceil(math.log2(top / E4M3_MAX)) - 1
+    while top > E4M3_MAX * 2.0 ** e:
+        e += 1
+    return min(max(e, E_MIN), E_MAX)
+
+
+def _block64(old, new):
+    """Codes and exponents per head of a page of ``old`` tokens (codes, exponents or None) and then ``new``
+    ones (tokens, heads, 128)."""
+    es, parts = [], []
+    for h in range(new.shape[1]):
+        e = _e64(new[:, h])
+        kept = []
+        if old is not None:
+            e = max(e, old[1][h])
+            kept = [_code64(old[0][:, h] * 2.0 ** old[1][h], torch.tensor(e, device="cuda"))]
+        parts.append(torch.cat(kept + [_code64(new[:, h], torch.tensor(e, device="cuda"))]))
+        es.append(e)
+    return torch.stack(parts, 1), es
+
+
+def _free_order(d):
+    """Pages as rows get them, in the order of the stack's top, for the past and then for the step."""
+    stack, table = d["free"].tolist(), [[] for _ in d["past"]]
+    for grow in (d["past"], [a + b for a, b in zip(d["past"], d["new"])]):
+        for i, n in enumerate(grow):
+            while len(table[i]) < _pages(n):
+                table[i].append(stack.pop())
+    return table
+
+
+def _exact_append(case, d):
+    n_kv = case["n_kv"]
+    pos = torch.tensor([a + t for a, b in zip(d["past"], d["new"]) for t in range(b)], device="cuda")
+    angle = _angles64(case, pos)
+    dtype = DTYPES[case["dtype"]]
+    q = _turn64(d["q"], angle, case)
+    k = _turn64(d["k"], angle, case).to(dtype).double()     # a key is rounded to its type before it is coded
+    if sum(_pages(a) + _pages(b) for a, b in zip(d["past"], d["new"])) * n_kv > 6000:
+        return {"q": q, "k": None, "v": None, "k_scale": None, "v_scale": None}
+    out = {"q": q}
+    for name, x, before in (("k", k, d["past_k"].double()), ("v", d["v"].double(), d["past_v"].double())):
+        codes = torch.zeros((d["n_pages"], n_kv, PAGE, HEAD), dtype=torch.float64, device="cuda")
+        scale = torch.full((d["n_pages"], n_kv), 2.0 ** E_MIN, dtype=torch.float64, device="cuda")
+        t0 = t1 = 0
+        for i, pages in enumerate(_free_order(d)):
+            a, b = d["past"][i], d["new"][i]
+            for j, page in enumerate(pages):
+                first = before[t0 + j * PAGE:t0 + min(a, (j + 1) * PAGE)] if a > j * PAGE else None
+                block = None if first is None else _block64(None, first)
+                lo, hi = max(a, j * PAGE), min(a + b, (j + 1) * PAGE)
+                if hi > lo:
+                    block = _block64(block, x[t1 + lo - a:t1 + hi - a])
+                codes[page, :, :block[0].shape[0]] = block[0].transpose(0, 1)
+                scale[page] = _two64(torch.tensor(block[1], device="cuda"))
+            t0, t1 = t0 + a, t1 + b
+        out[name], out[name + "_scale"] = codes, scale
+    return out
+
+
+def _held64(x, y):
+    """What a row's cache stands for after x (past, heads, 128) and then y (new, heads, 128) were stored."""
+    a, parts = x.shape[0], []
+
+    def coded(z, least=None):                      # z (pages, 64, heads, 128), zeros behind a row's end
+        e = torch.full((z.shape[0], 1, z.shape[2], 1), float(E_MIN), dtype=torch.float64, device=z.device)
+        top = z.abs().amax((1, 3), keepdim=True)
+        e = torch.where(top > 0, torch.ceil(torch.log2(top.clamp(min=1e-300) / E4M3_MAX)), e).clamp(E_MIN, E_MAX)
+        e = e + (top > E4M3_MAX * _two64(e))
+        return e if least is None else torch.maximum(e, least)
+
+    whole = a // PAGE * PAGE
+    for z in (x[:whole],):
+        if z.shape[0]:
+            z = z.reshape(-1, PAGE, *z.shape[1:])
+            e = coded(z)
+            parts.append((_code64(z, e) * _two64(e)).flatten(0, 1))
+    rest = x[whole:]
+    if rest.shape[0]:
+        e = coded(rest[None])
+        old = (_code64(rest[None], e) * _two64(e))
+        room = y[:PAGE - rest.shape[0]]
+        y = y[room.shape[0]:]
+        if room.shape[0]:
+            e = coded(room[None], e)
+        parts.append((_code64(torch.cat([old[0], room])[None], e) * _two64(e))[0])
+    if y.shape[0]:
+        full = torch.zeros((_pages(y.shape[0]) * PAGE, *y.shape[1:]), dtype=torch.float64, device=y.device)
+        full[:y.shape[0]] = y
+        z = full.reshape(-1, PAGE, *y.shape[1:])
+        e = coded(z)
+        parts.append((_code64(z, e) * _two64(e)).flatten(0, 1)[:y.shape[0]])
+    return torch.cat(parts)
+
+
+def _exact_attend(case, d):
+    n_kv, group = case["n_kv"], N_Q // case["n_kv"]
+    out, t0, t1 = [], 0, 0
+    for a, b in zip(d["past"], d["new"]):
+        x = [_held64(d["past_" + c][t0:t0 + a].double(), d[c][t1:t1 + b].double()) if b else None for c in "kv"]
+        q = d["q"][t1:t1 + b].double()
+        t0, t1 = t0 + a, t1 + b
+        if not b:
+            continue
+        heads = []
+        for h in range(N_Q):
+            s = q[:, h] @ x[0][:, h // group].T / math.sqrt(HEAD)
+            s = s.masked_fill(torch.arange(a + b, device="cuda") > a + torch.arange(b, device="cuda")[:, None], -math.inf)
+            heads.append(torch.softmax(s, -1) @ x[1][:, h // group])
+        out.append(torch.stack(heads, 1))
+    return {"out": torch.cat(out)}
+
+
+def exact(case, seed):
+    if case["op"] == "pages":
+        return None                                # whole numbers
+    d = _inputs(case, seed)
+    if case["op"] == "rotary":
+        angle = _angles64(case, d["pos"])
+        return {k: _turn64(d[k], angle, case) for k in ("q", "k")}
+    return _exact_append(case, d) if case["op"] == "append" else _exact_attend(case, d)
