@@ -442,7 +442,10 @@ def _plain_append(s):
     cos, sin = _plain_tables(case, s["step"]["positions"])
     q, k = (_turned(s[x], cos, sin, case["layout"], case["part"]).to(s[x].dtype) for x in ("q", "k"))
     _plain_store(s, k, s["v"])
-    return {"q": q, "k": s["k_codes"], "v": s["v_codes"], "k_scale": s["k_scale"], "v_scale": s["v_scale"]}
+    # positions and dims split as the cache's own views of its codes have them
+    pages, heads = s["k_scale"].shape
+    return {"q": q, "k": s["k_codes"].view(pages, heads, 4, 4, 4, 8, 16), "v": s["v_codes"].view(pages, heads, 4, 16, 8, 16),
+            "k_scale": s["k_scale"], "v_scale": s["v_scale"]}
 
 
 def _plain_attend(s):
