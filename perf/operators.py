@@ -266,7 +266,7 @@ def _own_rotary(case):
 
 def _own_state(case, d):
     # a table without room for pages of k and v serves for the page operator's own case
-    n_kv = case.get("n_kv", 1)
+    n_kv = case.get("n_kv", 8)
     cache = _oi2().PagedKVCache(1 if case["op"] != "pages" else 0, N_Q, n_kv, case["seqs"], d["width"] * PAGE, d["n_pages"],
                                 device="cuda")
     cache.free.copy_(d["free"])
