@@ -10,7 +10,9 @@ from .decode_step import DecoderStep
 from .format import (ALIGN_BYTES, HIDDEN_DIM, NEURON_RECORD_BYTES, PAGE_ALIGN, quantize_int4)
 from .hot import HotWeights
 from .layer import ColdNeurons, SparseFFNLayer, sparse_ffn
+from .paged import PagedKVCache, PagePlan
 from .predictor import NeuronPredictor, PredictorRegistry
+from .rotary import Rotary, rotary_frequencies
 from .stack import DecodeStack, StackLayer
 from .store import ColdSection, ColdWeightStore
 
@@ -19,4 +21,5 @@ __all__ = [
     "PAGE_ALIGN", "quantize_int4", "HotWeights", "ColdNeurons", "SparseFFNLayer", "sparse_ffn",
     "NeuronPredictor", "PredictorRegistry", "DecodeStack", "StackLayer", "ColdSection",
     "ColdWeightStore", "GroupedQueryAttention", "rope_tables", "DecoderStep",
+    "PagedKVCache", "PagePlan", "Rotary", "rotary_frequencies",
 ]

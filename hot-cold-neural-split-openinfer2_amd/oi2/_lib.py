@@ -8,7 +8,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
-from ctypes import POINTER, Structure, c_float, c_int32, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_float, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
 
@@ -50,6 +50,29 @@ class Predictor(Structure):
 class Attn(Structure):
     _fields_ = [("n_q", c_int32), ("n_kv", c_int32), ("wq", c_void_p), ("wk", c_void_p),
                 ("wv", c_void_p), ("wo", c_void_p), ("norm_w", c_void_p)]
+
+
+class Paged(Structure):
+    _fields_ = [("n_q", c_int32), ("n_kv", c_int32), ("n_seqs", c_int32), ("max_len", c_int32),
+                ("n_pages", c_int32), ("n_layers", c_int32), ("block_table", c_void_p),
+                ("lens", c_void_p), ("free_pages", c_void_p), ("n_free", c_void_p),
+                ("pages", c_void_p), ("scales", c_void_p)]
+
+
+class PagePlan(Structure):
+    _fields_ = [("max_tokens", c_int32), ("max_new", c_int32), ("cu", c_void_p),
+                ("positions", c_void_p), ("slots", c_void_p), ("kv_len", c_void_p),
+                ("rejected", c_void_p), ("work", c_void_p)]
+
+
+class Rotary(Structure):
+    _fields_ = [("head_dim", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32),
+                ("magnitude", c_float), ("freq", c_void_p)]
+
+
+class Heads(Structure):
+    _fields_ = [("data", c_void_p), ("heads", c_int32), ("token_stride", c_int64),
+                ("head_stride", c_int64)]
 
 
 class Layer(Structure):
@@ -121,6 +144,17 @@ _SIGS = {
     "oi2_attn_forward": (c_int32, [c_void_p, c_int32, c_int32, POINTER(Attn), c_float, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p,
                                    c_void_p, c_void_p, c_size_t, c_void_p]),
+    "oi2_page_plan_bytes": (c_size_t, [POINTER(Paged), c_int32, c_int32]),
+    "oi2_page_extend": (c_int32, [POINTER(Paged), POINTER(PagePlan), c_void_p, c_void_p]),
+    "oi2_page_rewind": (c_int32, [POINTER(Paged), c_void_p, c_void_p]),
+    "oi2_rotary_apply": (c_int32, [POINTER(Rotary), c_int32, c_int32, c_void_p, POINTER(Heads), c_void_p,
+                                   POINTER(Heads), c_void_p, c_void_p]),
+    "oi2_kv_append": (c_int32, [POINTER(Paged), POINTER(PagePlan), c_int32, c_int32, c_int32,
+                                POINTER(Heads), POINTER(Heads), POINTER(Rotary), POINTER(Heads), c_void_p,
+                                c_void_p]),
+    "oi2_kv_attend_workspace_bytes": (c_size_t, [POINTER(Paged), c_int32, c_int32]),
+    "oi2_kv_attend": (c_int32, [POINTER(Paged), POINTER(PagePlan), c_int32, c_int32, c_int32,
+                                POINTER(Heads), c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "oi2_section_bytes": (c_size_t, [c_int32]),
     "oi2_quantize_section": (c_int32, [c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
@@ -194,6 +228,38 @@ def stream_handle(device=None) -> int | None:
     else:
         torch.cuda.init()
     return torch._C._cuda_getCurrentRawStream(index) or None
+
+
+def gpu(device) -> torch.device:
+    """A GPU device with its index (the current one's, where it has none)."""
+    d = torch.device(device)
+    if d.type != "cuda":
+        raise ValueError(f"expected a GPU device, got {d}")
+    return d if d.index is not None else torch.device("cuda", torch.cuda.current_device())
+
+
+class on_device:
+    """``with on_device(d)``: d is the current device, which the kernels are
+    launched on.  Costs a comparison where it is already."""
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def heads(x: torch.Tensor) -> Heads:
+    """(tokens, heads, dim) as the C ABI takes it; the last dimension dense."""
+    st = x.stride()
+    return Heads(x.data_ptr(), x.shape[1], st[0], st[1])
 
 
 def logit_threshold(p: float) -> float:

@@ -433,6 +433,135 @@ int oi2_attn_forward(const uint16_t* x, int32_t batch, int32_t seq, const oi2_at
                      int32_t cache_cap, int32_t past, int32_t causal, uint16_t* out, uint16_t* x_out,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- paged 8-bit KV cache ------------------------------------------------ */
+/* No counterpart in the reference, whose cache is one fp16 tensor per layer
+ * and batch, grown by torch.cat (engine.py:105-109): a cache for requests of
+ * different lengths.  Row i of the cache is one sequence.  Memory is handed
+ * out in pages of 64 positions from one pool, the same pages in every layer;
+ * k and v are held in fp8 e4m3fn, with one scale per (page, kv head) for k
+ * and one for v.
+ *
+ * A scale is 2^e, e the smallest integer in [-40, 60] for which the largest
+ * finite value of the page and head is at most 448 2^e, 2^-40 where there is
+ * none.  A power of two, so that a page that grows rescales what it holds
+ * without a new rounding (but for values that become subnormal), and codes
+ * times scale are exact in fp32.  Infinities, NaN and values past 448 2^60
+ * are stored as NaN, which a row's attention returns where it sees them.
+ *
+ * pages: (layer, page, kv head) blocks of 16384 bytes, k then v, each 8192
+ * bytes of codes in the order in which the attention loads them:
+ *   k[p][d] at 2048 (p / 4 % 4) + 256 (d / 16) + 16 (4 (p / 16) + p % 4) + d % 16
+ *   v[p][d] at 1024 (d / 16) + 256 (p / 16) + 16 (d % 16) + p % 16
+ * scales: (layer, page, kv head, 2) fp32, of k and of v; v's is negative
+ * where the page holds a NaN in v. */
+enum { OI2_PAGE = 64, OI2_MAX_SEQS = 2048 };
+typedef struct oi2_paged {
+  int32_t n_q;                /* query heads of 128 */
+  int32_t n_kv;               /* kv heads; n_q / n_kv in {1, 2, 4, 8} */
+  int32_t n_seqs;             /* rows, 1 .. 2048 */
+  int32_t max_len;            /* most positions of a row */
+  int32_t n_pages;            /* pages of the pool, fewer than 2^25 */
+  int32_t n_layers;
+  int32_t* block_table;       /* (n_seqs, ceil(max_len / 64)): pages of a row, -1 none */
+  int32_t* lens;              /* (n_seqs) positions held */
+  int32_t* free_pages;        /* (n_pages) a stack of the free pages */
+  int32_t* n_free;            /* (1) its height */
+  uint8_t* pages;             /* (n_layers, n_pages, n_kv, 16384), 16-byte aligned */
+  float* scales;              /* (n_layers, n_pages, n_kv, 2), 8-byte aligned */
+} oi2_paged;
+
+/* One step over the cache as oi2_page_extend lays it out: the step's tokens
+ * are packed row after row. */
+typedef struct oi2_page_plan {
+  int32_t max_tokens;         /* most tokens of a step */
+  int32_t max_new;            /* most tokens of one row */
+  int32_t* cu;                /* (n_seqs + 1) first token of each row */
+  int32_t* positions;         /* (max_tokens) position of each token, -1 none */
+  int32_t* slots;             /* (max_tokens) page * 64 + place in it, -1 none */
+  int32_t* kv_len;            /* (n_seqs) positions of the row with the step's; 0: rejected */
+  int32_t* rejected;          /* (n_seqs) 1 where the row could not grow */
+  int32_t* work;              /* oi2_page_plan_bytes bytes, 16-byte aligned: work lists */
+} oi2_page_plan;
+
+/* Bytes of a plan's work lists; 0 for sizes that are not supported. */
+size_t oi2_page_plan_bytes(const oi2_paged* c, int32_t max_tokens, int32_t max_new);
+
+/* Row i of the cache grows by new_lens[i] positions (device memory, n_seqs
+ * values, negative ones as 0), and the plan of that step is written.  Pages
+ * come off the stack's top in row order.  A row is rejected, and neither it
+ * nor its table changes, when it would pass max_len, has more than max_new
+ * new tokens, ends past max_tokens in the packed order, or needs pages and
+ * the pool does not hold what it and the rows before it (but those rejected
+ * for one of the former reasons) need.  A rejected row keeps its tokens in
+ * the packed order; their positions and slots are -1.  Entries of positions
+ * and slots past the last token are -1. */
+int oi2_page_extend(const oi2_paged* c, const oi2_page_plan* p, const int32_t* new_lens, void* stream);
+
+/* Row i is cut back to lens[i] positions (device memory, n_seqs values) where
+ * it holds more; a negative value leaves it.  The pages it no longer needs go
+ * back on the stack, in the order that undoes an oi2_page_extend.  The paged
+ * form of a rolled-back draft; 0 ends a sequence.  A page that stays keeps
+ * its scales. */
+int oi2_page_rewind(const oi2_paged* c, const int32_t* lens, void* stream);
+
+/* Rotary positions.  A token at position t turns pair j of its heads by
+ * t * freq[j] / 2^64 of a whole turn, computed in 64-bit fixed point, so that
+ * far positions lose nothing:
+ *   (a, b) -> magnitude (a cos - b sin, a sin + b cos)
+ * with (a, b) dims (j, j + rotary_dim / 2), or (2 j, 2 j + 1) if interleaved;
+ * dims from rotary_dim on are copied.  fp64, rounded to fp32 and then to the type. */
+typedef struct oi2_rotary {
+  int32_t head_dim;           /* even, at most 256 */
+  int32_t rotary_dim;         /* even, at most head_dim */
+  int32_t interleaved;
+  float magnitude;
+  const uint64_t* freq;       /* (rotary_dim / 2), device memory */
+} oi2_rotary;
+
+/* Rows of (tokens, heads, head_dim) values of OI2_DTYPE_F16 or _BF16, the last
+ * dimension dense; strides in elements. */
+typedef struct oi2_heads {
+  const void* data;
+  int32_t heads;
+  int64_t token_stride;
+  int64_t head_stride;
+} oi2_heads;
+
+/* The rotary positions of q and k (either may have no heads) of n_tokens
+ * tokens at positions (device memory): the arithmetic of engine.py:140-157
+ * with each token at its own position, in fp64.  q_out and k_out are dense
+ * (n_tokens, heads, head_dim) and may be the inputs themselves where those
+ * are dense.  A token at a negative position is left out: its rows in the
+ * outputs are not written. */
+int oi2_rotary_apply(const oi2_rotary* r, int32_t dtype, int32_t n_tokens, const int32_t* positions,
+                     const oi2_heads* q, void* q_out, const oi2_heads* k, void* k_out, void* stream);
+
+/* k and v (n_tokens, n_kv, 128) of the plan's step into the pages of `layer`;
+ * with r not NULL, k is rotated first (rounded to its type, then coded: the
+ * codes of oi2_rotary_apply's k) and q, if given, is rotated into q_out
+ * (n_tokens, q heads, 128).  The plan's tokens past n_tokens are left out.
+ * A row's step is appended once per layer, in the order of the extends. */
+int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
+                  const oi2_heads* k, const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q, void* q_out,
+                  void* stream);
+
+/* Workspace bytes of oi2_kv_attend over a plan of these sizes: the partial
+ * sums of rows whose pages are cut into parts. */
+size_t oi2_kv_attend_workspace_bytes(const oi2_paged* c, int32_t max_tokens, int32_t max_new);
+
+/* Attention of the plan's tokens (engine.py:110-122, causal) over the pages of
+ * `layer`, after the step's own tokens were appended: the token at position t
+ * of row i sees positions [0, t] of the row.
+ *   out = softmax(scale q k^T) v,  k and v the codes times their scales
+ * q (n_tokens, n_q, 128) with strides, out (n_tokens, n_q, 128) dense, both of
+ * `dtype` (OI2_DTYPE_F16 or _BF16).  Scores, the softmax's sums and the output
+ * are fp32 until the one rounding of out; probabilities enter the products as
+ * two fp16 parts.  The tokens of a rejected row give zeros; rows of out past
+ * the step's last token are left as they were. */
+int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
+                  const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
 /* ---- split writer ------------------------------------------------------- */
 /* Bytes of one cold_weights.bin section with n_cold records: the 16-byte
  * <HHIq header, n_cold x 6400, zero padding to a 4096 multiple
