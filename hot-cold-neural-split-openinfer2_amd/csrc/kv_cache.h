@@ -59,7 +59,7 @@ inline PlanLayout plan_layout(const oi2_paged& c, int32_t n_tokens, int32_t max_
   l.parts_many = (kManyWgs + c.n_kv - 1) / c.n_kv;
   // a row's n tokens touch at most n, and at most n / 64 + 2, pages
   l.cap_append = (int32_t)min64(min64(n_tokens, n_tokens / kPage + 2 * rows), c.n_pages);
-  const int64_t few = rows + n_tokens / l.few_tokens, many = 0;
+  const int64_t few = rows + n_tokens / l.few_tokens, many = (int64_t)max_new * g > kFewRows ? rows + n_tokens / l.many_tokens : 0;
   // parts are at least total / parts pages long: tiles + parts of them, and
   // 2 parts where a tile has several
   const int64_t most_few = few * ((width + kFewMinPages - 1) / kFewMinPages);

@@ -329,7 +329,7 @@ ExtendArgs extend_args(const oi2_paged* c, const oi2_page_plan* p, const int32_t
   a.max_tokens = p->max_tokens;
   a.max_new = p->max_new;
   a.group = c->n_q / c->n_kv;
-  a.few_only = 1;
+  a.few_only = (int64_t)p->max_new * a.group <= kFewRows;
   a.fill = p->max_tokens <= kOneLaunchTokens;
   a.new_lens = new_lens;
   a.table = c->block_table;
