@@ -1,9 +1,11 @@
 // Attention of a step's query tokens over the paged 8-bit KV cache.
 //
-//   k_attend_few   up to 16 query rows (tokens times query heads of a kv head)
-//                  over a range of a row's pages
-//   k_attend_many  up to 128 query rows over a range of a row's pages
-//   k_attend_join  joins the ranges where a row's pages were cut into parts
+//   attend_few   up to 16 query rows (tokens times query heads of a kv head)
+//                over a range of a row's pages
+//   attend_many  up to 128 query rows over a range of a row's pages
+// in one launch.  Where a row's pages were cut into parts, a part leaves its
+// sums in the workspace, and the one that arrives last joins them, in the order
+// of the parts: the result does not depend on who that is.
 //
 // A page's k and v codes are widened exactly to fp16 (e4m3 has 4 significant
 // bits) and multiplied on the matrix cores; the page's scales, powers of two,
@@ -33,9 +35,17 @@ constexpr float kLift = 10.0f;
 // The running maximum follows the row's once that is 2^kSlack above it.
 constexpr float kSlack = 5.0f;
 
+struct PartArgs {             // of one of the two kernels
+  const AttendItem* items;
+  int groups;                 // workgroups of the launch
+  int32_t* count;             // (slot, kv head) arrivals, zero between calls
+  float* o;                   // (slot, kv head, rows, 128)
+  float* ml;                  // (slot, kv head, rows, 2)
+};
+
 struct AttendArgs {
   const int32_t* work;        // the plan's
-  int items_at, merge_at;     // its lists of this kernel, in ints
+  PartArgs few, many;
   const int32_t* table;
   const uint8_t* pages;       // of the layer
   const float* scales;
@@ -45,8 +55,6 @@ struct AttendArgs {
   int wide;                   // 16-byte loads of q
   float scale;                // of the scores, times log2 e
   uint16_t* out;
-  float* part_o;              // (slot, kv head, rows, 128)
-  float* part_ml;             // (slot, kv head, rows, 2)
 };
 
 __device__ __forceinline__ h8 widen8(uint32_t d0, uint32_t d1) {
@@ -86,21 +94,189 @@ __device__ __forceinline__ float ldexp2(float x, int e) { return __builtin_ldexp
 // A row of bf16 values over its largest one's power of two is exact in fp16 but
 // for what lies 2^-24 below that one.
 template <bool BF16>
-__device__ __forceinline__ h8 q_frag(const uint16_t (&v)[8], int e) {
+__device__ __forceinline__ h8 q_frag(const uint16_t (&v)[8], int e, bool negate) {
   h8 r;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     r[i] = BF16 ? (_Float16)ldexp2(bf16_bits_to_float(v[i]), -e) : __builtin_bit_cast(_Float16, v[i]);
-  return r;
+  return negate ? -r : r;
 }
+
+// Eight probabilities, times 2^kLift, as the operand of out^T = V^T P^T.  fp16
+// outputs take them in two fp16 parts (hi truncated, lo the rest: at least 21
+// bits), as one part's rounding would be as large as the output's own.  Of bf16
+// outputs, rounded to 8 bits, it is an eighth: one part, to nearest.
+template <bool BF16>
+struct Probs {
+  h8 hi, lo;
+};
+template <bool BF16>
+__device__ __forceinline__ Probs<BF16> to_probs(const float (&e)[8]) {
+  Probs<BF16> p;
+  if constexpr (BF16) {
+    typedef float f8 __attribute__((ext_vector_type(8)));
+    p.hi = __builtin_convertvector((f8{e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]}), h8);
+  } else {
+    u32x4 uh, ul;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(e[2 * k], e[2 * k + 1]));
+      uh[k] = hi;
+      ul[k] = __builtin_bit_cast(
+          uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(half_lo(hi), -1.0f, e[2 * k]), fmaf(half_hi(hi), -1.0f, e[2 * k + 1])));
+    }
+    p.hi = __builtin_bit_cast(h8, uh);
+    p.lo = __builtin_bit_cast(h8, ul);
+  }
+  return p;
+}
+
+// A page's scores are dot * score_scale + ev, with q negated where the scale of
+// the scores is negative, so that the largest dot is the largest score; a scale
+// of zero counts as 2^-120, because a masked dot is minus infinity.
+__device__ __forceinline__ float score_scale(float sc, float k_scale) { return fmaxf(fabsf(sc) * k_scale, 7.52316385e-37f); }
 
 __device__ __forceinline__ float quad_max(float v) {   // over the lanes l, l ^ 16, l ^ 32, l ^ 48
   v = fmaxf(v, __shfl_xor(v, 16));
   return fmaxf(v, __shfl_xor(v, 32));
 }
 
-constexpr int kFewWaves = 4, kFewThreads = 64 * kFewWaves;
+constexpr int kThreads = 256;
+
+// ── parts ────────────────────────────────────────────────────────────────────
+
+constexpr int kSc1 = 16;                   // cache-policy operand: agent-coherent access
+
+__device__ __forceinline__ void st_agent(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// A part's sums, row by row of n_rows, are stored (agent-coherent, by every
+// thread).  True in the workgroup that completes the set, which then joins it.
+__device__ __forceinline__ bool arrive(const PartArgs& pa, const ItemHead& it, int n_kv, int g) {
+  __shared__ int s_last;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // every store acknowledged
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int32_t* c = pa.count + (int64_t)it.slot0 * n_kv + g;
+    const int old = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_last = old + 1 == it.n_parts;
+    if (s_last) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+  }
+  __syncthreads();
+  return s_last;
+}
+
+// Joins the parts of a tile.  32 threads take a row's 128 dims; with fewer rows
+// than such groups, several groups a row, each every pg-th part.  The
+// tail of a call waits for this, and it waits for its loads, which go past the
+// caches: sums, maxima and exponential sums of U parts of RB rows go out
+// together, and are taken in with a running maximum.  smem: 16.1 bytes
+// a thread.
+template <bool BF16, int ROWS>
+__device__ __forceinline__ void join_parts(const AttendArgs& a, const PartArgs& pa, const ItemHead& it, int g, int n_rows,
+                                           float* smem) {
+  constexpr int kGroups = kThreads / 32, RB = ROWS == kFewRows ? 1 : 4, U = ROWS == kFewRows ? 8 : 4;
+  f32x4* s_y = reinterpret_cast<f32x4*>(smem);       // (kGroups, 32)
+  float* s_M = smem + 4 * kThreads;
+  float* s_L = s_M + kGroups;
+  const int tid = threadIdx.x, grp = tid >> 5, lane = tid & 31, lg = a.group_log, n_parts = it.n_parts;
+  const float ninf = -__builtin_inff();
+  const int64_t base = ((int64_t)it.slot0 * a.n_kv + g) * ROWS;
+  const int stride = a.n_kv * ROWS;                  // rows from a part to the next
+  const uint32_t rows = (uint32_t)((n_parts - 1) * stride + ROWS);
+  const rsrc_t ro = rsrc(pa.o + base * kHeadD, rows * (kHeadD * 4)), rml = rsrc(pa.ml + 2 * base, rows * 8);
+  const int pg = n_rows < kGroups ? kGroups / n_rows : 1, per = n_rows < kGroups ? n_rows : kGroups;
+  const int first = grp / per;
+  for (int r0 = 0; r0 < n_rows; r0 += kGroups * RB) {
+    f32x4 y[RB];
+    float M[RB], L[RB];
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      M[i] = ninf;
+      L[i] = 0.0f;
+    }
+    const int row0 = r0 + grp % per;                 // rows row0, row0 + kGroups, ..
+    for (int k = first; k < n_parts && first < pg; k += U * pg) {
+      u32x4 x[U][RB];
+      u32x2v ml[U][RB];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+          const int row = row0 + kGroups * i;
+          const bool is = k + u * pg < n_parts && row < n_rows;
+          const uint32_t at = (uint32_t)((k + u * pg) * stride + row);
+          ml[u][i] = __builtin_amdgcn_raw_buffer_load_b64(rml, is ? 8 * at : kNoOff, 0, kSc1);
+          x[u][i] = __builtin_amdgcn_raw_buffer_load_b128(ro, is ? at * (kHeadD * 4) + 16 * lane : kNoOff, 0, kSc1);
+        }
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        float top = M[i], m[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          m[u] = k + u * pg < n_parts ? as_f32(ml[u][i].x) : ninf;
+          top = fmaxf(top, m[u]);
+        }
+        const float f0 = M[i] == ninf ? 0.0f : __builtin_amdgcn_exp2f(M[i] - top);
+        M[i] = top;
+        L[i] *= f0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[i][e] *= f0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          // 0 times a NaN sum, of a part whose every score is NaN, stays NaN
+          const float f = m[u] == ninf ? 0.0f : __builtin_amdgcn_exp2f(m[u] - top);
+          L[i] = fmaf(f, as_f32(ml[u][i].y), L[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[i][e] = fmaf(f, as_f32(x[u][i][e]), y[i][e]);
+        }
+      }
+    }
+    if (pg > 1) {                                    // one row a group: a row's groups meet in its first one
+      __syncthreads();
+      s_y[tid] = y[0];
+      if (lane == 0) {
+        s_M[grp] = M[0];
+        s_L[grp] = L[0];
+      }
+      __syncthreads();
+      if (first == 0) {
+        float top = M[0];
+        for (int k = 1; k < pg; ++k) top = fmaxf(top, s_M[grp + k * per]);
+        const float f0 = M[0] == ninf ? 0.0f : __builtin_amdgcn_exp2f(M[0] - top);
+        L[0] *= f0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[0][e] *= f0;
+        for (int k = 1; k < pg; ++k) {
+          const float m = s_M[grp + k * per], f = m == ninf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+          L[0] = fmaf(f, s_L[grp + k * per], L[0]);
+          const f32x4 x = s_y[tid + 32 * k * per];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[0][e] = fmaf(f, x[e], y[0][e]);
+        }
+      }
+    }
+    if (first > 0) continue;
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      const int row = row0 + kGroups * i;
+      if (row >= n_rows) continue;
+      const float inv = 1.0f / L[i];
+      uint16_t z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = narrow<BF16>(y[i][e] * inv);
+      const int64_t to =
+          ((int64_t)(it.token0 + (row >> lg)) * a.n_q + (g << lg) + (row & ((1 << lg) - 1))) * kHeadD + 4 * lane;
+      *reinterpret_cast<u32x2v*>(a.out + to) = *reinterpret_cast<u32x2v*>(z);
+    }
+  }
+}
+
+// ── few rows ─────────────────────────────────────────────────────────────────
+
 constexpr int kORow = kHeadD + 4;          // floats of an output row in LDS, padded
+constexpr int kFewLds = (kFewWaves * kFewRows * (kORow + 2) + kHeadD) * 4;
 
 // Lane (r = lane % 16, grp = lane / 16).  K's 16-row tile t of a page: row
 // r = 4 a + i is position 16 a + 4 t + i; D's element i of lane (r, grp) is
@@ -108,15 +284,20 @@ constexpr int kORow = kHeadD + 4;          // floats of an output row in LDS, pa
 // positions 16 grp .. 16 grp + 15 of its query row, which are the positions of
 // the 16 bytes of V^T that it loads for each dim.
 template <bool BF16>
-__global__ __launch_bounds__(kFewThreads) void k_attend_few(AttendArgs a) {
-  __shared__ __align__(16) float s_o[kFewWaves][kFewRows][kORow];
-  __shared__ float s_m[kFewWaves][kFewRows], s_l[kFewWaves][kFewRows];
-  __shared__ int s_nan[kHeadD];
-  const int item = blockIdx.x / a.n_kv, g = blockIdx.x - item * a.n_kv;
+__device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* smem) {
+  const int item = b / a.n_kv, g = b - item * a.n_kv;
+  const AttendItem& full = a.few.items[item];
+  const ItemHead it = full;
   if (item >= a.work[kNFew]) return;
-  const AttendItem it = reinterpret_cast<const AttendItem*>(a.work + a.items_at)[item];
+  typedef float Rows[kFewRows];
+  float (*s_o)[kFewRows][kORow] = reinterpret_cast<float (*)[kFewRows][kORow]>(smem);
+  Rows* s_m = reinterpret_cast<Rows*>(smem + kFewWaves * kFewRows * kORow * 4);
+  Rows* s_l = s_m + kFewWaves;
+  int* s_nan = reinterpret_cast<int*>(s_l + kFewWaves);
   const int n_tok = min(it.n_tokens, a.n_tokens - it.token0);
-  if (n_tok <= 0) return;
+  // a tile whose last part is not in the launch (fewer tokens than the plan's)
+  // is left out whole: its arrivals would not be complete
+  if (n_tok <= 0 || item - it.part + it.n_parts > a.few.groups / a.n_kv) return;
   const int tid = threadIdx.x, lane = lane_id(), r = lane & 15, grp = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lg = a.group_log, n_rows = n_tok << lg;
@@ -152,7 +333,7 @@ __global__ __launch_bounds__(kFewThreads) void k_attend_few(AttendArgs a) {
   }
   h8 qf[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) qf[i] = q_frag<BF16>(qv[i], qe);
+  for (int i = 0; i < 4; ++i) qf[i] = q_frag<BF16>(qv[i], qe, a.scale < 0.0f);
   const float sc = BF16 ? ldexp2(a.scale, qe) : a.scale;
   const int lim = r < n_rows ? min(it.pos0 + tok + 1, it.kv_len) : 0;   // positions that this row sees
   const int all_see = min(it.pos0 + 1, it.kv_len);                      // ... and every row does
@@ -163,23 +344,42 @@ __global__ __launch_bounds__(kFewThreads) void k_attend_few(AttendArgs a) {
   for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = ninf, l = 0.0f;
 
+  // A page's k, then its v: each is loaded as soon as the products of the page
+  // before have taken theirs, so a wave always has 8 KB in flight.  Past the
+  // last page the descriptor's range is empty: nothing is read.
   const int32_t* table = a.table + (int64_t)it.row * a.width;
-  for (int page = it.page0 + w; page < it.page1; page += kFewWaves) {
-    int id = table[page];
+  auto block_of = [&](int page) {
+    int id = table[min(page, it.page1 - 1)];
     id = (unsigned)id < (unsigned)a.n_pages ? id : 0;
-    id = __builtin_amdgcn_readfirstlane(id);
-    const int64_t block = (int64_t)id * a.n_kv + g;
-    const uint8_t* kb = a.pages + block * kBlock;
-    u32x4 kr[8], vr[8];
+    return (int64_t)__builtin_amdgcn_readfirstlane(id) * a.n_kv + g;
+  };
+  auto page_rsrc = [&](int64_t block, int page) { return rsrc(a.pages + block * kBlock, page < it.page1 ? kBlock : 0); };
+  auto scale_of = [&](int64_t block) { return *reinterpret_cast<const float2*>(a.scales + 2 * block); };
+  u32x4 kr[8], vr[8];
+  auto load8 = [&](u32x4 (&x)[8], rsrc_t r, int at) {
 #pragma unroll
-    for (int n = 0; n < 8; ++n) kr[n] = load16_nt(kb + 1024 * n + 16 * lane);
-#pragma unroll
-    for (int n = 0; n < 8; ++n) vr[n] = load16_nt(kb + kHalfBlock + 1024 * n + 16 * lane);
-    const float ks = a.scales[2 * block], vs = a.scales[2 * block + 1];
+    for (int n = 0; n < 8; ++n) x[n] = wld16(r, at + 1024 * n + 16 * lane);
+  };
+  const int first = it.page0 + w;
+  int64_t next = 0;
+  float2 scale = {1.0f, 1.0f};
+  if (first < it.page1) {
+    const int64_t block = (int64_t)__builtin_amdgcn_readfirstlane(full.ids[w]) * a.n_kv + g;
+    const rsrc_t r0 = page_rsrc(block, first);
+    load8(kr, r0, 0);
+    load8(vr, r0, kHalfBlock);
+    scale = scale_of(block);
+    next = block_of(first + kFewWaves);
+  }
+  for (int page = first; page < it.page1; page += kFewWaves) {
+    const rsrc_t rn = page_rsrc(next, page + kFewWaves);
+    const float ks = scale.x, vs = scale.y;
+    scale = scale_of(next);
+    next = block_of(page + 2 * kFewWaves);
     const float ev = (float)((int)((as_u32(vs) >> 23) & 0xFF) - 127);
 
     float s[16];
-    const float ksc = sc * ks;
+    const float ksc = score_scale(sc, ks);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -187,8 +387,11 @@ __global__ __launch_bounds__(kFewThreads) void k_attend_few(AttendArgs a) {
       for (int i = 0; i < 4; ++i)
         acc = mfma16(widen8(kr[2 * t + (i >> 1)][2 * (i & 1)], kr[2 * t + (i >> 1)][2 * (i & 1) + 1]), qf[i], acc);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * t + i] = fmaf(acc[i], ksc, ev);
+      for (int i = 0; i < 4; ++i) s[4 * t + i] = acc[i];
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load8(kr, rn, 0);
+    __builtin_amdgcn_sched_barrier(0);
     const int p0 = page * kPage + 16 * grp;
     if (page * kPage + kPage > all_see) {
 #pragma unroll
@@ -197,7 +400,7 @@ __global__ __launch_bounds__(kFewThreads) void k_attend_few(AttendArgs a) {
     float cm = s[0];
 #pragma unroll
     for (int j = 1; j < 16; ++j) cm = fmaxf(cm, s[j]);
-    cm = quad_max(cm);
+    cm = fmaf(quad_max(cm), ksc, ev);
     const bool up = cm > m + kSlack;
     if (__any(up)) {
       const float mn = up ? cm : m;
@@ -207,28 +410,20 @@ __global__ __launch_bounds__(kFewThreads) void k_attend_few(AttendArgs a) {
       for (int d = 0; d < 8; ++d) o[d] *= alpha;
       m = mn;
     }
-    const float ref = (m == ninf ? 0.0f : m) - kLift;
-    float p[16], sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(s[j] - ref);
-      sum += p[j];
-    }
-    l = fmaf(sum, ldexp2(1.0f, -(int)ev), l);
-    h8 ph[2], pl[2];
+    const float rel = ev - ((m == ninf ? 0.0f : m) - kLift);
+    float sum[2] = {0.0f, 0.0f};
+    Probs<BF16> p[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      u32x4 uh, ul;
+      float e[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float e0 = p[8 * h + 2 * k], e1 = p[8 * h + 2 * k + 1];
-        const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(e0, e1));
-        uh[k] = hi;
-        ul[k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(e0 - half_lo(hi), e1 - half_hi(hi)));
+      for (int j = 0; j < 8; ++j) {
+        e[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + j], ksc, rel));
+        sum[h] += e[j];
       }
-      ph[h] = __builtin_bit_cast(h8, uh);
-      pl[h] = __builtin_bit_cast(h8, ul);
+      p[h] = to_probs<BF16>(e);
     }
+    l = fmaf(sum[0] + sum[1], ldexp2(1.0f, -(int)ev), l);
     // places behind the row's end hold whatever their page held before
     const int tail = it.kv_len - p0;
     if (page * kPage + kPage > it.kv_len) {
@@ -246,9 +441,12 @@ __global__ __launch_bounds__(kFewThreads) void k_attend_few(AttendArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const h8 vf = widen8(vr[d][2 * h], vr[d][2 * h + 1]);
-        o[d] = mfma16(vf, ph[h], o[d]);
-        o[d] = mfma16(vf, pl[h], o[d]);
+        o[d] = mfma16(vf, p[h].hi, o[d]);
+        if (!BF16) o[d] = mfma16(vf, p[h].lo, o[d]);
       }
+    __builtin_amdgcn_sched_barrier(0);
+    load8(vr, rn, kHalfBlock);
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   l += __shfl_xor(l, 16);
@@ -260,52 +458,58 @@ __global__ __launch_bounds__(kFewThreads) void k_attend_few(AttendArgs a) {
     s_l[w][r] = l;
   }
   __syncthreads();
-  // thread: query row tid / 16, dims 8 (tid % 16) ..
-  const int row = tid >> 4, d0 = 8 * (tid & 15);
-  if (row >= n_rows) return;
-  float M = ninf, L = 0.0f;
+  // thread: E dims from d0 of a query row
+  constexpr int E = kFewRows * kHeadD / kThreads;
+  const int row = tid * E / kHeadD, d0 = tid * E % kHeadD;
+  float M = ninf, L = 0.0f, y[E];
 #pragma unroll
   for (int k = 0; k < kFewWaves; ++k) M = fmaxf(M, s_m[k][row]);
-  float y[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+  for (int e = 0; e < E; ++e) y[e] = 0.0f;
 #pragma unroll
   for (int k = 0; k < kFewWaves; ++k) {
     const float mk = s_m[k][row], f = mk == ninf ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
     L = fmaf(f, s_l[k][row], L);
     // 0 times a NaN sum, of a wave whose every score is NaN, stays NaN
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = fmaf(f, s_o[k][row][d0 + e], y[e]);
+    for (int e = 0; e < E; ++e) y[e] = fmaf(f, s_o[k][row][d0 + e], y[e]);
   }
   const int tk = row >> lg, head = (g << lg) + (row & ((1 << lg) - 1));
   const int sees = min(it.pos0 + tk + 1, it.kv_len);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = s_nan[d0 + e] < sees ? __builtin_nanf("") : y[e];
-  if (it.part >= 0) {
-    const int64_t at = ((int64_t)it.part * a.n_kv + g) * kFewRows + row;
-    f32x4* po = reinterpret_cast<f32x4*>(a.part_o + at * kHeadD + d0);
-    po[0] = f32x4{y[0], y[1], y[2], y[3]};
-    po[1] = f32x4{y[4], y[5], y[6], y[7]};
-    if (d0 == 0) {
-      a.part_ml[2 * at] = M;
-      a.part_ml[2 * at + 1] = L;
+  for (int e = 0; e < E; ++e) y[e] = s_nan[d0 + e] < sees ? __builtin_nanf("") : y[e];
+  if (it.n_parts > 1) {
+    const int64_t base = ((int64_t)(it.slot0 + it.part) * a.n_kv + g) * kFewRows;
+    if (row < n_rows) {
+      const rsrc_t ro = rsrc(a.few.o + base * kHeadD, kFewRows * kHeadD * 4);
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2v{as_u32(y[e]), as_u32(y[e + 1])}, ro, (row * kHeadD + d0 + e) * 4, 0, kSc1);
+      if (d0 == 0) {
+        st_agent(a.few.ml + 2 * (base + row), M);
+        st_agent(a.few.ml + 2 * (base + row) + 1, L);
+      }
     }
+    if (arrive(a.few, it, a.n_kv, g)) join_parts<BF16, kFewRows>(a, a.few, it, g, n_rows, reinterpret_cast<float*>(smem));
     return;
   }
+  if (row >= n_rows) return;
   const float inv = it.kv_len > 0 ? 1.0f / L : 0.0f;     // a rejected row: zeros
-  uint16_t z[8];
+  uint16_t z[E];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) z[e] = it.kv_len > 0 ? narrow<BF16>(y[e] * inv) : 0;
-  *reinterpret_cast<u32x4*>(a.out + ((int64_t)(it.token0 + tk) * a.n_q + head) * kHeadD + d0) = *reinterpret_cast<u32x4*>(z);
+  for (int e = 0; e < E; ++e) z[e] = it.kv_len > 0 ? narrow<BF16>(y[e] * inv) : 0;
+  uint16_t* to = a.out + ((int64_t)(it.token0 + tk) * a.n_q + head) * kHeadD + d0;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(to + e) = z[e] | (uint32_t)z[e + 1] << 16;
 }
+
+// ── many rows ────────────────────────────────────────────────────────────────
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ f32x16 mfma32(h8 a, h8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-
-constexpr int kManyThreads = 256;
 
 // A page in LDS, fp16: k's rows of one position (256 bytes, 16 chunks of 8
 // dims), then v's rows of one dim (128 bytes, 8 chunks of 8 positions).  Chunks
@@ -326,15 +530,17 @@ __device__ __forceinline__ int v_lds(int d, int c) { return kVLds + d * 128 + 16
 // because row 8 b + 4 h + i (+ 16 s) of the product is given position
 // 8 h + 4 b + i (+ 16 s); eight consecutive ones are a fragment of P^T and a
 // 16-byte chunk of a dim's row of V^T.
+constexpr int kManyLds = 2 * kPageLds + kHeadD * 4;
+
 template <bool BF16>
-__global__ __launch_bounds__(kManyThreads, 2) void k_attend_many(AttendArgs a) {
-  __shared__ __align__(1024) uint8_t s_page[2 * kPageLds];
-  __shared__ int s_nan[kHeadD];
-  const int item = blockIdx.x / a.n_kv, g = blockIdx.x - item * a.n_kv;
+__device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t* s_page) {
+  int* s_nan = reinterpret_cast<int*>(s_page + 2 * kPageLds);
+  const int item = b / a.n_kv, g = b - item * a.n_kv;
+  const AttendItem& full = a.many.items[item];
+  const ItemHead it = full;
   if (item >= a.work[kNMany]) return;
-  const AttendItem it = reinterpret_cast<const AttendItem*>(a.work + a.items_at)[item];
   const int n_tok = min(it.n_tokens, a.n_tokens - it.token0);
-  if (n_tok <= 0) return;
+  if (n_tok <= 0 || item - it.part + it.n_parts > a.many.groups / a.n_kv) return;
   const int tid = threadIdx.x, lane = lane_id(), r = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lg = a.group_log, n_rows = n_tok << lg;
@@ -368,7 +574,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_attend_many(AttendArgs a) {
       qe = min(max((int)(as_u32(top) >> 23) - 127, -126), 126);
     }
 #pragma unroll
-    for (int st = 0; st < 8; ++st) qf[st] = q_frag<BF16>(qv[st], qe);
+    for (int st = 0; st < 8; ++st) qf[st] = q_frag<BF16>(qv[st], qe, a.scale < 0.0f);
   }
   const float sc = BF16 ? ldexp2(a.scale, qe) : a.scale;
   const int lim = row < n_rows ? min(it.pos0 + tok + 1, it.kv_len) : 0;   // positions that this row sees
@@ -427,18 +633,30 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_attend_many(AttendArgs a) {
   auto compute = [&](int page, int at, float2 scale) {
     int ka = at + k_rd, va = at + v_rd;
     asm volatile("" : "+v"(ka), "+v"(va));
-    const float ev = (float)((int)((as_u32(scale.y) >> 23) & 0xFF) - 127), ksc = sc * scale.x;
+    const float ev = (float)((int)((as_u32(scale.y) >> 23) & 0xFF) - 127), ksc = score_scale(sc, scale.x);
+    // k's fragments two steps ahead of their products, v's a step of
+    // probabilities ahead: an LDS read takes longer than two products
     f32x16 s[2] = {};
+    h8 kf[3][2], vf[2][4];
+    auto read_k = [&](int st) {
 #pragma unroll
-    for (int st = 0; st < 8; ++st)
+      for (int T = 0; T < 2; ++T)   // a 2 further: the swizzle's bit 3
+        kf[st % 3][T] = *reinterpret_cast<const h8*>(s_page + (ka ^ (32 * st) ^ (128 * T)) + 8192 * T);
+    };
+    auto read_v = [&](int f) {
 #pragma unroll
-      for (int T = 0; T < 2; ++T)
-        s[T] = mfma32(*reinterpret_cast<const h8*>(s_page + (ka ^ (32 * st) ^ (128 * T)) + 8192 * T), qf[st], s[T]);   // a 2 further: bit 3
-    __builtin_amdgcn_sched_barrier(0);
+      for (int d = 0; d < 4; ++d) vf[f & 1][d] = *reinterpret_cast<const h8*>(s_page + (va ^ (32 * f)) + 4096 * d);
+    };
+    read_k(0);
+    read_k(1);
 #pragma unroll
-    for (int T = 0; T < 2; ++T)
+    for (int st = 0; st < 8; ++st) {
+      if (st < 6) read_k(st + 2);
+      if (st == 6) read_v(0);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s[T][j] = fmaf(s[T][j], ksc, ev);
+      for (int T = 0; T < 2; ++T) s[T] = mfma32(kf[st % 3][T], qf[st], s[T]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     const int p0 = page * kPage + 8 * h;
     if (page * kPage + kPage > all_see) {
 #pragma unroll
@@ -451,7 +669,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_attend_many(AttendArgs a) {
     for (int T = 0; T < 2; ++T)
 #pragma unroll
       for (int j = 0; j < 16; ++j) cm = fmaxf(cm, s[T][j]);
-    cm = fmaxf(cm, __shfl_xor(cm, 32));
+    cm = fmaf(fmaxf(cm, __shfl_xor(cm, 32)), ksc, ev);
     const bool up = cm > m + kSlack;
     if (__any(up)) {
       const float mn = up ? cm : m;
@@ -461,41 +679,32 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_attend_many(AttendArgs a) {
       for (int d = 0; d < 4; ++d) o[d] *= alpha;
       m = mn;
     }
-    const float ref = (m == ninf ? 0.0f : m) - kLift;
-    float sum = 0.0f;
-    h8 ph, pl;
-    // fragment f of the probabilities: positions 16 f + 8 h ..
-    auto probabilities = [&](int f) {
-      u32x4 uh, ul;
+    const float rel = ev - ((m == ninf ? 0.0f : m) - kLift);
+    float sum[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int j = 8 * (f & 1) + 2 * k;
-        const float e0 = __builtin_amdgcn_exp2f(s[f >> 1][j] - ref), e1 = __builtin_amdgcn_exp2f(s[f >> 1][j + 1] - ref);
-        sum += e0;
-        sum += e1;
-        const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(e0, e1));
-        uh[k] = hi;
-        ul[k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(half_lo(hi), -1.0f, e0), fmaf(half_hi(hi), -1.0f, e1)));
+    for (int f = 0; f < 4; ++f) {          // positions 16 f + 8 h ..
+      float e[8];
+      sum[f] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = __builtin_amdgcn_exp2f(fmaf(s[f >> 1][8 * (f & 1) + j], ksc, rel));
+        sum[f] += e[j];
       }
-      ph = __builtin_bit_cast(h8, uh);
-      pl = __builtin_bit_cast(h8, ul);
-    };
-#pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      probabilities(f);
+      const Probs<BF16> p = to_probs<BF16>(e);
+      if (f < 3) read_v(f + 1);
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        const h8 vf = *reinterpret_cast<const h8*>(s_page + (va ^ (32 * f)) + 4096 * d);
-        o[d] = mfma32(vf, ph, o[d]);
-        o[d] = mfma32(vf, pl, o[d]);
+        o[d] = mfma32(vf[f & 1][d], p.hi, o[d]);
+        if (!BF16) o[d] = mfma32(vf[f & 1][d], p.lo, o[d]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    l = fmaf(sum, ldexp2(1.0f, -(int)ev), l);
+    l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ldexp2(1.0f, -(int)ev), l);
   };
 
   if (it.page0 < it.page1) {
-    int64_t b0 = block_of(it.page0), b1 = block_of(it.page0 + 1);
+    const int64_t b0 = (int64_t)__builtin_amdgcn_readfirstlane(full.ids[0]) * a.n_kv + g;
+    const int64_t b1 = (int64_t)__builtin_amdgcn_readfirstlane(full.ids[1]) * a.n_kv + g;
     load(b0);
     float2 sc0 = scale_of(b0), sc1 = scale_of(b1);
     store(it.page0, 0, sc0.y);
@@ -514,26 +723,34 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_attend_many(AttendArgs a) {
   }
 
   l += __shfl_xor(l, 32);
-  if (row >= n_rows) return;
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
     for (int j = 0; j < 16; ++j)
       o[d][j] = s_nan[32 * d + 8 * (j >> 2) + 4 * h + (j & 3)] < lim ? __builtin_nanf("") : o[d][j];
-  if (it.part >= 0) {
-    const int64_t at = ((int64_t)it.part * a.n_kv + g) * kManyRows + row;
+  if (it.n_parts > 1) {
+    // through LDS (chunks of a row swizzled by it), so that rows leave whole
+    __syncthreads();
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4*>(a.part_o + at * kHeadD + 32 * d + 8 * q + 4 * h) =
+        *reinterpret_cast<f32x4*>(s_page + row * 512 + 16 * ((8 * d + 2 * q + h) ^ r)) =
             f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
-    if (h == 0) {
-      a.part_ml[2 * at] = m;
-      a.part_ml[2 * at + 1] = l;
+    const int64_t base = ((int64_t)(it.slot0 + it.part) * a.n_kv + g) * kManyRows;
+    const rsrc_t ro = rsrc(a.many.o + base * kHeadD, kManyRows * kHeadD * 4);
+    __syncthreads();
+    for (int i = tid; i < n_rows * 32; i += kThreads)
+      __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4*>(s_page + (i >> 5) * 512 + 16 * ((i ^ (i >> 5)) & 31)),
+                                             ro, 16 * i, 0, kSc1);
+    if (h == 0 && row < n_rows) {
+      st_agent(a.many.ml + 2 * (base + row), m);
+      st_agent(a.many.ml + 2 * (base + row) + 1, l);
     }
+    if (arrive(a.many, it, a.n_kv, g)) join_parts<BF16, kManyRows>(a, a.many, it, g, n_rows, reinterpret_cast<float*>(s_page));
     return;
   }
+  if (row >= n_rows) return;
   const float inv = it.kv_len > 0 ? 1.0f / l : 0.0f;   // a rejected row: zeros
   uint16_t* po = a.out + ((int64_t)(it.token0 + tok) * a.n_q + (g << lg) + (row & ((1 << lg) - 1))) * kHeadD + 4 * h;
 #pragma unroll
@@ -547,38 +764,21 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_attend_many(AttendArgs a) {
     }
 }
 
-// Joins the parts of one tile of query tokens and kv head: a row of 128 dims by
-// 32 threads.
-template <bool BF16, int ROWS>
-__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, int count) {
-  const int item = blockIdx.x / a.n_kv, g = blockIdx.x - item * a.n_kv;
-  if (item >= a.work[count]) return;
-  const MergeItem it = reinterpret_cast<const MergeItem*>(a.work + a.merge_at)[item];
-  const int n_tok = min(it.n_tokens, a.n_tokens - it.token0), lg = a.group_log;
-  const int n_rows = max(n_tok, 0) << lg;
-  const float ninf = -__builtin_inff();
-  const int64_t stride = (int64_t)a.n_kv * ROWS;
-  for (int row = threadIdx.x >> 5; row < n_rows; row += 8) {
-    const int d0 = 4 * (threadIdx.x & 31);
-    const int64_t at = ((int64_t)it.part0 * a.n_kv + g) * ROWS + row;
-    float M = ninf;
-    for (int k = 0; k < it.n_parts; ++k) M = fmaxf(M, a.part_ml[2 * (at + k * stride)]);
-    float L = 0.0f;
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < it.n_parts; ++k) {
-      const float mk = a.part_ml[2 * (at + k * stride)], f = mk == ninf ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
-      L = fmaf(f, a.part_ml[2 * (at + k * stride) + 1], L);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (at + k * stride) * kHeadD + d0);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = fmaf(f, x[e], y[e]);
-    }
-    const float inv = 1.0f / L;
-    uint16_t z[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) z[e] = narrow<BF16>(y[e] * inv);
-    const int64_t to = ((int64_t)(it.token0 + (row >> lg)) * a.n_q + (g << lg) + (row & ((1 << lg) - 1))) * kHeadD + d0;
-    *reinterpret_cast<u32x2v*>(a.out + to) = *reinterpret_cast<u32x2v*>(z);
-  }
+// Steps whose rows all have few query rows, and steps with rows of either kind:
+// the long tiles first, the others fill the chip behind and beside them.
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void k_attend_few(AttendArgs a) {
+  __shared__ __align__(16) uint8_t smem[kFewLds];
+  attend_few<BF16>(a, blockIdx.x, smem);
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void k_attend(AttendArgs a) {
+  static_assert(kManyLds >= kFewLds && kThreads == 64 * kFewWaves, "one workgroup for either");
+  __shared__ __align__(1024) uint8_t smem[kManyLds];
+  const int b = blockIdx.x;
+  if (b < a.many.groups) attend_many<BF16>(a, b, smem);
+  else attend_few<BF16>(a, b - a.many.groups, smem);
 }
 
 // The workspace: the partial sums of either kernel's parts, out and then m, l.
@@ -637,34 +837,23 @@ int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int
   hipStream_t st = (hipStream_t)stream;
   const bool bf = dtype == OI2_DTYPE_BF16;
   const int64_t few = (int64_t)now.cap_few * c->n_kv, many = (int64_t)now.cap_many * c->n_kv;
-  OI2_CHECK_ARG(few < 1 << 23 && many < 1 << 23, "%d tokens are too many for one call", n_tokens);
-  AttendArgs b = a;
-  b.items_at = (int)l.many;
-  b.merge_at = (int)l.merge_many;
-  b.part_o = (float*)workspace + few_floats(l, c->n_kv);
-  b.part_ml = b.part_o + (size_t)l.cap_parts_many * c->n_kv * kManyRows * kHeadD;
-  a.items_at = (int)l.few;
-  a.merge_at = (int)l.merge_few;
-  a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + (size_t)l.cap_parts_few * c->n_kv * kFewRows * kHeadD;
-  if (many) {
-    if (bf) hipLaunchKernelGGL(k_attend_many<true>, dim3((uint32_t)many), dim3(kManyThreads), 0, st, b);
-    else hipLaunchKernelGGL(k_attend_many<false>, dim3((uint32_t)many), dim3(kManyThreads), 0, st, b);
-    OI2_CHECK_LAUNCH();
-  }
-  if (bf) hipLaunchKernelGGL(k_attend_few<true>, dim3((uint32_t)few), dim3(kFewThreads), 0, st, a);
-  else hipLaunchKernelGGL(k_attend_few<false>, dim3((uint32_t)few), dim3(kFewThreads), 0, st, a);
+  OI2_CHECK_ARG(few + many < 1 << 23, "%d tokens are too many for one call", n_tokens);
+  a.few.items = reinterpret_cast<const AttendItem*>(p->work + l.few);
+  a.few.groups = (int)few;
+  a.few.count = p->work + l.count_few;
+  a.few.o = (float*)workspace;
+  a.few.ml = a.few.o + (size_t)l.cap_parts_few * c->n_kv * kFewRows * kHeadD;
+  a.many.items = reinterpret_cast<const AttendItem*>(p->work + l.many);
+  a.many.groups = (int)many;
+  a.many.count = p->work + l.count_many;
+  a.many.o = a.few.o + few_floats(l, c->n_kv);
+  a.many.ml = a.many.o + (size_t)l.cap_parts_many * c->n_kv * kManyRows * kHeadD;
+  const dim3 grid((uint32_t)(few + many)), block(kThreads);
+  if (many && bf) hipLaunchKernelGGL(k_attend<true>, grid, block, 0, st, a);
+  else if (many) hipLaunchKernelGGL(k_attend<false>, grid, block, 0, st, a);
+  else if (bf) hipLaunchKernelGGL(k_attend_few<true>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(k_attend_few<false>, grid, block, 0, st, a);
   OI2_CHECK_LAUNCH();
-  if (const uint32_t n = (uint32_t)now.cap_merge_few * c->n_kv) {
-    if (bf) hipLaunchKernelGGL((k_attend_join<true, kFewRows>), dim3(n), dim3(256), 0, st, a, kNMergeFew);
-    else hipLaunchKernelGGL((k_attend_join<false, kFewRows>), dim3(n), dim3(256), 0, st, a, kNMergeFew);
-    OI2_CHECK_LAUNCH();
-  }
-  if (const uint32_t n = (uint32_t)now.cap_merge_many * c->n_kv) {
-    if (bf) hipLaunchKernelGGL((k_attend_join<true, kManyRows>), dim3(n), dim3(256), 0, st, b, kNMergeMany);
-    else hipLaunchKernelGGL((k_attend_join<false, kManyRows>), dim3(n), dim3(256), 0, st, b, kNMergeMany);
-    OI2_CHECK_LAUNCH();
-  }
   return OI2_OK;
 }
 

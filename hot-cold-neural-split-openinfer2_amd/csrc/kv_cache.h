@@ -18,32 +18,39 @@ constexpr int kExpMin = -40, kExpMax = 60;
 // Query rows (tokens times query heads per kv head) of a workgroup of the
 // attention: up to 16 in the kernel for few rows, 128 in the one for many.
 constexpr int kFewRows = 16, kManyRows = 128;
-// Parts that the attention's work is cut into per kv head (over all rows),
-// and the fewest pages of a part.
-constexpr int kFewWgs = 1024, kManyWgs = 512;
-constexpr int kFewMinPages = 4, kManyMinPages = 16;
+// Waves of a workgroup for few rows, each every fourth page.
+constexpr int kFewWaves = 4;
+// Workgroups that the attention's work is cut for, over all rows and kv heads.
+constexpr int kFewWgs = 512, kManyWgs = 512;
+// Tiles of up to so many pages are never cut: a round of four pages costs about
+// 1.1 us, joining parts 3.5.
+constexpr int kFewWhole = 16, kManyWhole = 16;
 
 // Work lists of a plan.
 struct AppendItem {           // one page that the step writes to
   int32_t page, token0;       // its first new token, in the packed order
   int32_t held, upto;         // places [held, upto) of the page are new
 };
-struct AttendItem {           // query tokens of one row over a range of its pages
+struct ItemHead {             // query tokens of one row over a range of its pages
   int32_t row, token0, n_tokens, pos0;    // pos0: position of token0
-  int32_t page0, page1, kv_len, part;     // part: slot of its partial sums, -1: writes the output
+  int32_t page0, page1, kv_len;
+  int32_t part, n_parts;                  // of the tokens' pages: which part, of how many
+  int32_t slot0;                          // the parts' partial sums are at slot0 + part
+  int32_t pad[2];
 };
-struct MergeItem {            // query tokens whose pages were cut into parts
-  int32_t token0, n_tokens, part0, n_parts;
+struct AttendItem : ItemHead {
+  int32_t ids[4];                         // the first pages, so that they need no look-up
 };
+constexpr int kItemInts = sizeof(AttendItem) / 4;
 
 struct PlanLayout {           // offsets in ints into oi2_page_plan.work
-  int32_t cap_append, cap_few, cap_many, cap_merge_few, cap_merge_many, cap_parts_few, cap_parts_many;
+  int32_t cap_append, cap_few, cap_many, cap_parts_few, cap_parts_many;
   int32_t few_tokens, many_tokens;        // tokens of a workgroup
   int32_t parts_few, parts_many;          // parts per kv head that the work is cut for
-  int64_t append, few, many, merge_few, merge_many, ints;
+  int64_t append, few, many, count_few, count_many, ints;   // count: arrivals of the parts of (slot0, kv head)
 };
 // counts at the head of the work lists
-enum { kNAppend = 0, kNFew, kNMany, kNMergeFew, kNMergeMany, kHeadInts = 16 };
+enum { kNAppend = 0, kNFew, kNMany, kHeadInts = 16 };
 
 inline int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
 
@@ -55,27 +62,27 @@ inline PlanLayout plan_layout(const oi2_paged& c, int32_t n_tokens, int32_t max_
   const int64_t rows = min64(c.n_seqs, n_tokens);
   l.few_tokens = kFewRows / g;
   l.many_tokens = kManyRows / g;
-  l.parts_few = (kFewWgs + c.n_kv - 1) / c.n_kv;
   l.parts_many = (kManyWgs + c.n_kv - 1) / c.n_kv;
   // a row's n tokens touch at most n, and at most n / 64 + 2, pages
   l.cap_append = (int32_t)min64(min64(n_tokens, n_tokens / kPage + 2 * rows), c.n_pages);
-  const int64_t few = rows + n_tokens / l.few_tokens, many = (int64_t)max_new * g > kFewRows ? rows + n_tokens / l.many_tokens : 0;
-  // parts are at least total / parts pages long: tiles + parts of them, and
-  // 2 parts where a tile has several
-  const int64_t most_few = few * ((width + kFewMinPages - 1) / kFewMinPages);
-  const int64_t most_many = many * ((width + kManyMinPages - 1) / kManyMinPages);
-  l.cap_few = (int32_t)min64(few + l.parts_few, most_few > few ? most_few : few);
-  l.cap_many = (int32_t)min64(many + (many ? l.parts_many : 0), most_many > many ? most_many : many);
-  l.cap_parts_few = width > kFewMinPages ? 2 * l.parts_few : 0;
-  l.cap_parts_many = width > kManyMinPages && many ? 2 * l.parts_many : 0;
-  l.cap_merge_few = (int32_t)min64(few, l.cap_parts_few / 2);
-  l.cap_merge_many = (int32_t)min64(many, l.cap_parts_many / 2);
+  // where no row may have more than kFewRows, a rejected one still gets its zeros
+  // from the kernel for few rows, in several tiles
+  const bool few_only = (int64_t)max_new * g <= kFewRows;
+  l.parts_few = (kFewWgs + c.n_kv - 1) / c.n_kv;
+  const int64_t few = rows + (few_only ? n_tokens / l.few_tokens : 0), many = few_only ? 0 : rows + n_tokens / l.many_tokens;
+  // parts are at least total / parts pages long, so there are tiles + parts of
+  // them, and twice as many where only tiles with several count
+  const bool cut_few = width > kFewWhole, cut_many = width > kManyWhole && many > 0;
+  l.cap_few = (int32_t)(few + (cut_few ? l.parts_few : 0));
+  l.cap_many = (int32_t)(many + (cut_many ? l.parts_many : 0));
+  l.cap_parts_few = cut_few ? 2 * l.parts_few : 0;
+  l.cap_parts_many = cut_many ? 2 * l.parts_many : 0;
   l.append = kHeadInts;
   l.few = l.append + 4 * (int64_t)l.cap_append;
-  l.many = l.few + 8 * (int64_t)l.cap_few;
-  l.merge_few = l.many + 8 * (int64_t)l.cap_many;
-  l.merge_many = l.merge_few + 4 * (int64_t)l.cap_merge_few;
-  l.ints = l.merge_many + 4 * (int64_t)l.cap_merge_many;
+  l.many = l.few + kItemInts * (int64_t)l.cap_few;
+  l.count_few = l.many + kItemInts * (int64_t)l.cap_many;
+  l.count_many = l.count_few + (int64_t)l.cap_parts_few * c.n_kv;
+  l.ints = l.count_many + (int64_t)l.cap_parts_many * c.n_kv;
   return l;
 }
 

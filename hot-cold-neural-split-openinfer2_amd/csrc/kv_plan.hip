@@ -156,13 +156,12 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
     bl += l;
   }
   const int n_touch = (int)(both >> 32), n_tile = (int)(both & 0xFFFFFFFF);
-  // pages of a part: an equal share of all of them, in whole rounds of the
-  // workgroup's waves
-  auto share = [](int64_t all, int parts, int least) {
-    const int64_t c = (all + parts - 1) / parts;
-    return (int)min(max((c + 3) / 4 * 4, (int64_t)least), (int64_t)1 << 26);
+  // pages of a part: an equal share of all of them, in whole rounds of a
+  // workgroup's four waves
+  auto share = [](int64_t all, int parts) {
+    return (int)min(max(((all + parts - 1) / parts + 3) / 4 * 4, (int64_t)4), (int64_t)1 << 26);
   };
-  const int c_few = share(all_few, a.l.parts_few, kFewMinPages), c_many = share(all_many, a.l.parts_many, kManyMinPages);
+  const int c_few = share(all_few, a.l.parts_few), c_many = share(all_many, a.l.parts_many);
   __syncthreads();
 
   // table entries.  The rows that are served are those whose need ends within
@@ -198,9 +197,7 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
   // attention tiles, cut into parts
   AttendItem* few_list = reinterpret_cast<AttendItem*>(a.work + a.l.few);
   AttendItem* many_list = reinterpret_cast<AttendItem*>(a.work + a.l.many);
-  MergeItem* mf = reinterpret_cast<MergeItem*>(a.work + a.l.merge_few);
-  MergeItem* mm = reinterpret_cast<MergeItem*>(a.work + a.l.merge_many);
-  int64_t base_items = 0, base_slots = 0, base_merge = 0;
+  int64_t base_items = 0, base_slots = 0;
   for (int i0 = 0; i0 < n_tile; i0 += nt) {
     const int i = i0 + tid;
     bool few = false;
@@ -216,33 +213,33 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
       tok0 = s_tok[r] + first;
       pages = s_kv[r] ? pages_of(min(s_past[r] + first + count, s_kv[r])) : 0;
       const int c = few ? c_few : c_many;
-      parts = max((pages + c - 1) / c, 1);
+      parts = pages <= (few ? kFewWhole : kManyWhole) ? 1 : (pages + c - 1) / c;
     }
     const int slots = parts > 1 ? parts : 0;
-    int64_t t_items, t_slots, t_merge;
+    int64_t t_items, t_slots;
     const int64_t x_items = scan_excl(few ? pair(0, parts) : pair(parts, 0), s_scan, t_items) + base_items;
     const int64_t x_slots = scan_excl(few ? pair(0, slots) : pair(slots, 0), s_scan, t_slots) + base_slots;
-    const int64_t x_merge = scan_excl(parts > 1 ? (few ? pair(0, 1) : pair(1, 0)) : 0, s_scan, t_merge) + base_merge;
     base_items += t_items;
     base_slots += t_slots;
-    base_merge += t_merge;
     if (i < n_tile) {
       const int item = (int)(few ? x_items & 0xFFFFFFFF : x_items >> 32);
       const int slot = (int)(few ? x_slots & 0xFFFFFFFF : x_slots >> 32);
-      const int merge = (int)(few ? x_merge & 0xFFFFFFFF : x_merge >> 32);
-      const int c = few ? c_few : c_many;
       AttendItem* list = few ? few_list : many_list;
-      for (int k = 0; k < parts; ++k)
-        list[item + k] = AttendItem{r, tok0, count, s_past[r] + first, min(k * c, pages), min((k + 1) * c, pages),
-                                    s_kv[r], parts > 1 ? slot + k : -1};
-      if (parts > 1) (few ? mf : mm)[merge] = MergeItem{tok0, count, slot, parts};
+      const int each = parts > 1 ? ((pages + parts - 1) / parts + 3) / 4 * 4 : pages;   // at most c: as many parts, alike
+      const int32_t* ids = a.table + (int64_t)r * a.width;
+      for (int k = 0; k < parts; ++k) {
+        AttendItem x{{r, tok0, count, s_past[r] + first, min(k * each, pages), min((k + 1) * each, pages),
+                      s_kv[r], k, parts, slot, {0, 0}}, {}};
+#pragma unroll
+        for (int e = 0; e < kFewWaves; ++e)
+          if (few || e < 2) x.ids[e] = x.page0 + e < x.page1 ? page_id(a, ids[x.page0 + e]) : 0;
+        list[item + k] = x;
+      }
     }
   }
   if (tid == 0) {
     a.work[kNFew] = (int)(base_items & 0xFFFFFFFF);
     a.work[kNMany] = (int)(base_items >> 32);
-    a.work[kNMergeFew] = (int)(base_merge & 0xFFFFFFFF);
-    a.work[kNMergeMany] = (int)(base_merge >> 32);
   }
   if (a.fill)
     for (int t = tid; t < a.max_tokens; t += nt) {

@@ -131,7 +131,7 @@ class Cache:
         return [np.concatenate([c[p] * 2.0 ** e[p].astype(np.float64)[:, None, None] for p in ids], 1)[:, :n]
                 for c, e in zip(self.codes, self.exps)]
 
-    def attend(self, q, plan, scale):
+    def attend(self, q, plan, scale, one_part=False):
         """(out, bound): out (tokens, n_q, 128) float64, zeros for rejected rows;
         bound is what sum p |v| and the scores' error give: per output, the
         absolute error of fp32 sums (see attend_bound)."""
@@ -159,16 +159,17 @@ class Cache:
                     y = p @ np.where(nan, 0.0, vv)
                     y[((~hide).astype(float) @ nan.astype(float)) > 0] = np.nan
                 out[t0:t0 + n, h] = y
-                bound[t0:t0 + n, h] = attend_bound(mag.max(1), np.abs(np.where(hide, 0, s)).max(1), now)[:, None] * (p @ np.abs(np.where(nan, 0.0, vv)))
+                bound[t0:t0 + n, h] = attend_bound(mag.max(1), np.abs(np.where(hide, 0, s)).max(1), now, one_part)[:, None] * (p @ np.abs(np.where(nan, 0.0, vv)))
         return out, bound
 
 
-def attend_bound(mag, top, n):
+def attend_bound(mag, top, n, one_part):
     """Relative to sum p |v|: each score's fp32 sum of 128 exact products is off
     by at most 128 2^-24 mag (mag = scale sum |q k|), its product with the scale,
     the sum with v's exponent (up to 60) and the difference to the maximum by
     2^-24 of values up to 1.45 (top + 60) each; a probability is off by that and
     2^-22 of the exponential, in numerator and denominator; two fp16 parts cut
-    2^-20; sums over n positions are off by n 2^-24 each at most."""
+    2^-20, one part, to nearest, half a step of fp16, 2^-11 (the numerator's
+    alone); sums over n positions are off by n 2^-24 each at most."""
     score = 128 * 2.0 ** -24 * mag + 4 * 2.0 ** -24 * 1.45 * (2 * top + 60)
-    return 2 * (score + 2.0 ** -22 + n * 2.0 ** -24) + 2.0 ** -20
+    return 2 * (score + 2.0 ** -22 + n * 2.0 ** -24) + 2.0 ** (-11 if one_part else -20)

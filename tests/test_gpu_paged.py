@@ -4,7 +4,8 @@ slot maps, rotary positions, the quantising append, the attention.
 Tables, codes and scales are compared bit for bit.  Rotary outputs may be off
 by half a step of their type and of fp32, and the pair times 2^-40 (fp64 on both sides) and
 times what half a step of a 64-bit frequency makes at the token's position; attention outputs by half a step of their type
-and the oracle's bound on fp32 sums.
+and the oracle's bound on fp32 sums and on the probabilities' fp16 parts (two
+for fp16 outputs, one for bf16).
 """
 import math
 import random
@@ -342,7 +343,7 @@ def test_attend(dev, dtype, past, new):
         n_q = 8 if n_kv == 1 else 32
         print(f"[attend] {dtype} {past} {new} q {n_q} kv {n_kv}", flush=True)
         c, o, plan, ref, q = _filled(dev, n_q, n_kv, past, new, dtype, 7)
-        want, bound = o.attend(_np(q), ref, D ** -0.5)
+        want, bound = o.attend(_np(q), ref, D ** -0.5, q.dtype == torch.bfloat16)
         _check_attend(c.attend(0, q, plan), want, bound, dtype)
 
 
@@ -351,7 +352,7 @@ def test_attend_head_layouts(dev, n_q, n_kv):
     print(f"[attend] heads {n_q} {n_kv}", flush=True)
     for past, new in (([70, 900], [1, 1]), ([70, 300], [5, 150])):
         c, o, plan, ref, q = _filled(dev, n_q, n_kv, past, new, torch.float16, 3)
-        want, bound = o.attend(_np(q), ref, D ** -0.5)
+        want, bound = o.attend(_np(q), ref, D ** -0.5, q.dtype == torch.bfloat16)
         _check_attend(c.attend(0, q, plan), want, bound, torch.float16)
 
 
@@ -378,7 +379,7 @@ def test_attend_pages_of_different_scales(dev, dtype, new):
         c.append(0, k, v, p)
         o.append(_np(k), _np(v), ref)
     q = torch.randn((sum(new), n_q, D), generator=g, device=dev).to(dtype)
-    want, bound = o.attend(_np(q), ref, 0.02)
+    want, bound = o.attend(_np(q), ref, 0.02, q.dtype == torch.bfloat16)
     y = c.attend(0, q, plan, scale=0.02)
     if dtype == torch.float16:
         assert np.abs(want).max() < 6.5e4
@@ -413,7 +414,7 @@ def test_attend_nan_where_it_is_seen(dev, new):
         c.append(0, k, v, p)
         o.append(_np(k), _np(v), ref)
     q = torch.randn((sum(new), n_q, D), generator=g, device=dev).half()
-    want, bound = o.attend(_np(q), ref, D ** -0.5)
+    want, bound = o.attend(_np(q), ref, D ** -0.5, q.dtype == torch.bfloat16)
     y = c.attend(0, q, plan)
     nan = np.isnan(want)
     assert nan.any() and not nan.all()
@@ -458,9 +459,9 @@ def test_attend_strides_and_repeats(dev):
     odd.copy_(q)
     for x in (odd, q.transpose(0, 1).contiguous().transpose(0, 1), q):
         assert torch.equal(c.attend(0, x, plan), y)
-    want, bound = o.attend(_np(q), ref, 0.0)
+    want, bound = o.attend(_np(q), ref, 0.0, q.dtype == torch.bfloat16)
     _check_attend(c.attend(0, q, plan, scale=0.0), want, bound, torch.bfloat16)
-    want, bound = o.attend(_np(q), ref, -0.3)
+    want, bound = o.attend(_np(q), ref, -0.3, q.dtype == torch.bfloat16)
     _check_attend(c.attend(0, q, plan, scale=-0.3), want, bound, torch.bfloat16)
 
 
