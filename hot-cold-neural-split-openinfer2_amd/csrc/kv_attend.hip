@@ -511,30 +511,38 @@ __device__ __forceinline__ f32x16 mfma32(h8 a, h8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// A page in LDS, fp16: k's rows of one position (256 bytes, 16 chunks of 8
-// dims), then v's rows of one dim (128 bytes, 8 chunks of 8 positions).  Chunks
-// are swizzled within their rows so that staging stores and fragment reads
-// touch all banks: k's by position p = 16 a + 4 t + i with i | (a ^ t) << 2,
+// In LDS, fp16: two pages of k, rows of one position (256 bytes, 16 chunks of 8
+// dims), and two of v, rows of one dim (128 bytes, 8 chunks of 8 positions).
+// Chunks are swizzled within their rows so that staging stores and fragment
+// reads touch all banks: k's by position p = 16 a + 4 t + i with i | (a ^ t) << 2,
 // distinct for the 16 rows of a store (one t) and of a read (one a); v's by
 // d / 2.  Every address is a lane's base with constant bits flipped and a
 // constant added, which costs an instruction where a register each would spill.
-constexpr int kPageLds = kPage * 256 + kHeadD * 128, kVLds = kPage * 256;
+constexpr int kHalfLds = kPage * 256, kVLds = 2 * kHalfLds;
+static_assert(kHalfLds == kHeadD * 128, "a page of k and one of v");
 __device__ __forceinline__ int k_swz(int p) { return (p & 3) | ((((p >> 4) ^ (p >> 2)) & 3) << 2); }
 __device__ __forceinline__ int k_lds(int p, int c) { return p * 256 + 16 * (c ^ k_swz(p)); }
 __device__ __forceinline__ int v_lds(int d, int c) { return kVLds + d * 128 + 16 * (c ^ ((d >> 1) & 7)); }
 
 // Four waves of 32 query rows.  A page is widened to fp16 once for all of them
-// on its way into LDS (two buffers, one barrier a page; its codes come two pages
-// ahead into registers).  Lane (r = lane % 32, h = lane / 32) has the scores of
-// query row r: element j of tile T is position 32 T + 16 (j / 8) + 8 h + j % 8,
-// because row 8 b + 4 h + i (+ 16 s) of the product is given position
-// 8 h + 4 b + i (+ 16 s); eight consecutive ones are a fragment of P^T and a
-// 16-byte chunk of a dim's row of V^T.
-constexpr int kManyLds = 2 * kPageLds + kHeadD * 4;
+// on its way into LDS (one barrier a page; its codes come a page ahead into
+// registers).  Lane (r = lane % 32, h = lane / 32) has the scores of query row
+// r: element j of tile T is position 32 T + 16 (j / 8) + 8 h + j % 8, because
+// row 8 b + 4 h + i (+ 16 s) of the product is given position 8 h + 4 b + i
+// (+ 16 s); eight consecutive ones are a fragment of P^T and a 16-byte chunk of
+// a dim's row of V^T.
+//
+// Two waves a SIMD are too few to fill the gaps where products wait for the
+// vector unit: one after the other they kept the matrix cores 43 % and the
+// vector unit 60 % busy (5000 tokens, bf16: 257 us).  So the next page's staging
+// stands between the products of the scores, and a fragment's exponentials
+// between the products of the fragment before.  (The next page's scores beside
+// this one's exponentials take 32 registers more: they spilled, 272 us.)
+constexpr int kManyLds = 4 * kHalfLds + kHeadD * 4;
 
 template <bool BF16>
 __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t* s_page) {
-  int* s_nan = reinterpret_cast<int*>(s_page + 2 * kPageLds);
+  int* s_nan = reinterpret_cast<int*>(s_page + 4 * kHalfLds);
   const int item = b / a.n_kv, g = b - item * a.n_kv;
   const AttendItem& full = a.many.items[item];
   const ItemHead it = full;
@@ -594,77 +602,85 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
     id = (unsigned)id < (unsigned)a.n_pages ? id : 0;
     return (int64_t)__builtin_amdgcn_readfirstlane(id) * a.n_kv + g;
   };
-  u32x4 kr[2], vr[2];
-  auto load = [&](int64_t block) {
-    const uint8_t* b = a.pages + block * kBlock;
+  u32x4 kr[2], vr[2];                  // codes on their way into LDS: vectors tid and tid + 256
+  auto load = [&](u32x4 (&x)[2], int64_t block, int half) {
+    const uint8_t* b = a.pages + block * kBlock + half;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      kr[n] = load16(b + 16 * tid + 4096 * n);
-      vr[n] = load16(b + kHalfBlock + 16 * tid + 4096 * n);
-    }
+    for (int n = 0; n < 2; ++n) x[n] = load16(b + 16 * tid + 4096 * n);
   };
-  // lane bases: stores of vectors tid (and tid + 256), reads
+  // lane bases of the stores and reads
   const int st_p = 16 * ((tid & 15) >> 2) + 4 * (tid >> 7) + (tid & 3), st_d = 16 * (tid >> 6) + (tid & 15);
   const int k_st = k_lds(st_p, 2 * ((tid >> 4) & 7)), v_st = v_lds(st_d, 2 * ((tid >> 4) & 3));
   const int k_rd = k_lds((r & 19) | ((r >> 3) & 1) << 2 | ((r >> 2) & 1) << 3, h), v_rd = v_lds(r, h);
-  auto store = [&](int page, int at, float v_scale) {
-    int ka = at + k_st, va = at + v_st;
-    asm volatile("" : "+v"(ka), "+v"(va));
+  // part q of 4 of the staged vectors, widened into LDS
+  auto put_k = [&](int ka, int q) {    // 8 positions (2 t) further: the swizzle's bit 3 flips
+    const int n = q >> 1, e = q & 1;
+    *reinterpret_cast<h8*>(s_page + (ka ^ (128 * n) ^ (16 * e)) + 2048 * n) = widen8(kr[n][2 * e], kr[n][2 * e + 1]);
+  };
+  auto put_v = [&](int va, int q) {    // 64 dims further
+    const int n = q >> 1, e = q & 1;
+    *reinterpret_cast<h8*>(s_page + (va ^ (16 * e)) + 8192 * n) = widen8(vr[n][2 * e], vr[n][2 * e + 1]);
+  };
+  auto fix_v = [&](int page, float v_scale) {
+    const int tail = it.kv_len - page * kPage - 16 * ((tid >> 4) & 3);
+    if (page * kPage + kPage > it.kv_len) {   // behind the row's end: whatever the page held before
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      // 8 positions (2 t) further: the swizzle's bit 3 flips
-      uint8_t* k0 = s_page + (ka ^ (128 * n)) + 2048 * n;
-      uint8_t* k1 = s_page + (ka ^ (128 * n) ^ 16) + 2048 * n;
-      *reinterpret_cast<h8*>(k0) = widen8(kr[n][0], kr[n][1]);
-      *reinterpret_cast<h8*>(k1) = widen8(kr[n][2], kr[n][3]);
-      u32x4 x = vr[n];
-      if (page * kPage + kPage > it.kv_len) {   // behind the row's end: whatever the page held before
-        const int tail = it.kv_len - page * kPage - 16 * ((tid >> 4) & 3);
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = first_bytes(x[k], tail - 4 * k);
-      }
-      if (v_scale < 0.0f) take_nans(x, page * kPage + 16 * ((tid >> 4) & 3), &s_nan[st_d + 64 * n]);
-      *reinterpret_cast<h8*>(s_page + va + 8192 * n) = widen8(x[0], x[1]);           // 64 dims further
-      *reinterpret_cast<h8*>(s_page + (va ^ 16) + 8192 * n) = widen8(x[2], x[3]);
+        for (int k = 0; k < 4; ++k) vr[n][k] = first_bytes(vr[n][k], tail - 4 * k);
+    }
+    if (v_scale < 0.0f) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) take_nans(vr[n], page * kPage + 16 * ((tid >> 4) & 3), &s_nan[st_d + 64 * n]);
     }
   };
   auto scale_of = [&](int64_t block) { return *reinterpret_cast<const float2*>(a.scales + 2 * block); };
 
-  auto compute = [&](int page, int at, float2 scale) {
+  h8 kf[2][2], vf[4];
+  auto read_k = [&](int ka, int st) {
+#pragma unroll
+    for (int T = 0; T < 2; ++T)        // a 2 further: the swizzle's bit 3
+      kf[st & 1][T] = *reinterpret_cast<const h8*>(s_page + (ka ^ (32 * st) ^ (128 * T)) + 8192 * T);
+  };
+  auto read_v = [&](int va, int i) {   // fragment f = i / 4, dims 32 (i % 4) ..
+    vf[i & 3] = *reinterpret_cast<const h8*>(s_page + (va ^ (32 * (i >> 2))) + 4096 * (i & 3));
+  };
+  // `page` is in buffers i % 2; the next one goes from kr and vr to the others.
+  auto round = [&](int page, int i, float2 scale, float2 next_scale) {
+    const int at = (i & 1) * kHalfLds, other = kHalfLds - at;
+    fix_v(page + 1, next_scale.y);
+    int k_to = other + k_st, v_to = other + v_st;
+    if (page * kPage >= some_see) {    // the wave sees nothing here: it only stages
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        put_k(k_to, q);
+        put_v(v_to, q);
+      }
+      return;
+    }
     int ka = at + k_rd, va = at + v_rd;
-    asm volatile("" : "+v"(ka), "+v"(va));
-    const float ev = (float)((int)((as_u32(scale.y) >> 23) & 0xFF) - 127), ksc = score_scale(sc, scale.x);
-    // k's fragments two steps ahead of their products, v's a step of
-    // probabilities ahead: an LDS read takes longer than two products
+    asm volatile("" : "+v"(ka), "+v"(va), "+v"(k_to), "+v"(v_to));
+    read_k(ka, 0);
     f32x16 s[2] = {};
-    h8 kf[3][2], vf[2][4];
-    auto read_k = [&](int st) {
-#pragma unroll
-      for (int T = 0; T < 2; ++T)   // a 2 further: the swizzle's bit 3
-        kf[st % 3][T] = *reinterpret_cast<const h8*>(s_page + (ka ^ (32 * st) ^ (128 * T)) + 8192 * T);
-    };
-    auto read_v = [&](int f) {
-#pragma unroll
-      for (int d = 0; d < 4; ++d) vf[f & 1][d] = *reinterpret_cast<const h8*>(s_page + (va ^ (32 * f)) + 4096 * d);
-    };
-    read_k(0);
-    read_k(1);
 #pragma unroll
     for (int st = 0; st < 8; ++st) {
-      if (st < 6) read_k(st + 2);
-      if (st == 6) read_v(0);
+      if (st < 7) read_k(ka, st + 1);
+      if (st >= 5) read_v(va, st - 5);
 #pragma unroll
-      for (int T = 0; T < 2; ++T) s[T] = mfma32(kf[st % 3][T], qf[st], s[T]);
+      for (int T = 0; T < 2; ++T) s[T] = mfma32(kf[st & 1][T], qf[st], s[T]);
+      if (st & 1) put_v(v_to, st >> 1);
+      else put_k(k_to, st >> 1);
       __builtin_amdgcn_sched_barrier(0);
     }
-    const int p0 = page * kPage + 8 * h;
+    const float ev = (float)((int)((as_u32(scale.y) >> 23) & 0xFF) - 127), ksc = score_scale(sc, scale.x);
     if (page * kPage + kPage > all_see) {
+      const int p0 = page * kPage + 8 * h;
 #pragma unroll
       for (int T = 0; T < 2; ++T)
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[T][j] = p0 + 32 * T + 16 * (j >> 3) + (j & 7) < lim ? s[T][j] : ninf;
     }
-    float cm = s[0][0];
+    float cm = ninf;
 #pragma unroll
     for (int T = 0; T < 2; ++T)
 #pragma unroll
@@ -680,24 +696,30 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
       m = mn;
     }
     const float rel = ev - ((m == ninf ? 0.0f : m) - kLift);
-    float sum[4];
+    // fragment f of the probabilities: positions 16 f + 8 h ..
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, e[8];
+    auto exps = [&](int f, int j0, int j1) {
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {          // positions 16 f + 8 h ..
-      float e[8];
-      sum[f] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = j0; j < j1; ++j) {
         e[j] = __builtin_amdgcn_exp2f(fmaf(s[f >> 1][8 * (f & 1) + j], ksc, rel));
         sum[f] += e[j];
       }
-      const Probs<BF16> p = to_probs<BF16>(e);
-      if (f < 3) read_v(f + 1);
+    };
+    Probs<BF16> p;
+    exps(0, 0, 8);
+    p = to_probs<BF16>(e);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        o[d] = mfma32(vf[f & 1][d], p.hi, o[d]);
-        if (!BF16) o[d] = mfma32(vf[f & 1][d], p.lo, o[d]);
+        if (4 * f + d < 13) read_v(va, 4 * f + d + 3);
+        o[d] = mfma32(vf[d], p.hi, o[d]);
+        if (!BF16) o[d] = mfma32(vf[d], p.lo, o[d]);
+        if (f < 3) exps(f + 1, 2 * d, 2 * d + 2);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if (f < 3) p = to_probs<BF16>(e);
     }
     l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ldexp2(1.0f, -(int)ev), l);
   };
@@ -705,18 +727,26 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
   if (it.page0 < it.page1) {
     const int64_t b0 = (int64_t)__builtin_amdgcn_readfirstlane(full.ids[0]) * a.n_kv + g;
     const int64_t b1 = (int64_t)__builtin_amdgcn_readfirstlane(full.ids[1]) * a.n_kv + g;
-    load(b0);
+    int64_t b2 = block_of(it.page0 + 2);
+    load(kr, b0, 0);
+    load(vr, b0, kHalfBlock);
     float2 sc0 = scale_of(b0), sc1 = scale_of(b1);
-    store(it.page0, 0, sc0.y);
-    load(b1);
+    fix_v(it.page0, sc0.y);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      put_k(k_st, q);
+      put_v(v_st, q);
+    }
+    load(kr, b1, 0);
+    load(vr, b1, kHalfBlock);
     for (int page = it.page0; page < it.page1; ++page) {
-      const int cur = (page - it.page0) & 1;
-      const int64_t b2 = block_of(page + 2);
-      __syncthreads();                 // the page is in LDS; its other buffer is read
-      if (page + 1 < it.page1) store(page + 1, (cur ^ 1) * kPageLds, sc1.y);
-      load(b2);
+      __syncthreads();                 // the page is in LDS, the last one is read
       const float2 sc2 = scale_of(b2);
-      if (page * kPage < some_see) compute(page, cur * kPageLds, sc0);
+      const int64_t b3 = block_of(page + 3);
+      round(page, page - it.page0, sc0, sc1);
+      load(kr, b2, 0);                 // past the last page: that one again, not used
+      load(vr, b2, kHalfBlock);
+      b2 = b3;
       sc0 = sc1;
       sc1 = sc2;
     }
@@ -730,6 +760,7 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
       o[d][j] = s_nan[32 * d + 8 * (j >> 2) + 4 * h + (j & 3)] < lim ? __builtin_nanf("") : o[d][j];
   if (it.n_parts > 1) {
     // through LDS (chunks of a row swizzled by it), so that rows leave whole
+    static_assert(kManyRows * 512 <= 4 * kHalfLds, "a tile's sums");
     __syncthreads();
 #pragma unroll
     for (int d = 0; d < 4; ++d)
