@@ -645,8 +645,9 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
   auto read_v = [&](int va, int i) {   // fragment f = i / 4, dims 32 (i % 4) ..
     vf[i & 3] = *reinterpret_cast<const h8*>(s_page + (va ^ (32 * (i >> 2))) + 4096 * (i & 3));
   };
-  // `page` is in buffers i % 2; the next one goes from kr and vr to the others.
-  auto round = [&](int page, int i, float2 scale, float2 next_scale) {
+  // `page` is in buffers i % 2; the next one goes from kr and vr to the others,
+  // the one after it is loaded.
+  auto round = [&](int page, int i, float2 scale, float2 next_scale, int64_t after) {
     const int at = (i & 1) * kHalfLds, other = kHalfLds - at;
     fix_v(page + 1, next_scale.y);
     int k_to = other + k_st, v_to = other + v_st;
@@ -656,6 +657,8 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
         put_k(k_to, q);
         put_v(v_to, q);
       }
+      load(kr, after, 0);
+      load(vr, after, kHalfBlock);
       return;
     }
     int ka = at + k_rd, va = at + v_rd;
@@ -672,6 +675,9 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
       else put_k(k_to, st >> 1);
       __builtin_amdgcn_sched_barrier(0);
     }
+    load(kr, after, 0);
+    load(vr, after, kHalfBlock);
+    __builtin_amdgcn_sched_barrier(0);
     const float ev = (float)((int)((as_u32(scale.y) >> 23) & 0xFF) - 127), ksc = score_scale(sc, scale.x);
     if (page * kPage + kPage > all_see) {
       const int p0 = page * kPage + 8 * h;
@@ -743,9 +749,7 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
       __syncthreads();                 // the page is in LDS, the last one is read
       const float2 sc2 = scale_of(b2);
       const int64_t b3 = block_of(page + 3);
-      round(page, page - it.page0, sc0, sc1);
-      load(kr, b2, 0);                 // past the last page: that one again, not used
-      load(vr, b2, kHalfBlock);
+      round(page, page - it.page0, sc0, sc1, b2);   // past the last page: that one again, not used
       b2 = b3;
       sc0 = sc1;
       sc1 = sc2;
