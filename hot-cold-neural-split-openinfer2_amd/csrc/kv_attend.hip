@@ -30,10 +30,10 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896341f;
-// p comes out times 2^kLift: its low fp16 part stays out of the subnormals.
-constexpr float kLift = 10.0f;
-// The running maximum follows the row's once that is 2^kSlack above it.
-constexpr float kSlack = 5.0f;
+// p comes out times 2^kLift, and the running maximum follows the row's once that
+// is 2^kSlack above it: p stays below fp16's 2^16, few pages rescale the sums,
+// and a low part's subnormals are off by 2^-25, 2^-27 of the largest p at most.
+constexpr float kLift = 2.0f, kSlack = 13.0f;
 
 struct PartArgs {             // of one of the two kernels
   const AttendItem* items;
@@ -65,6 +65,23 @@ __device__ __forceinline__ h8 widen8(uint32_t d0, uint32_t d1) {
 
 __device__ __forceinline__ f32x4 mfma16(h8 a, h8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Loads at uniform addresses of what no kernel writes meanwhile (tables, scales,
+// items), through the constant address space: scalar loads.  As vector loads
+// they return in order behind the codes on their way, and waiting for a page's
+// number then waits for those.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+  static_assert(sizeof(T) % 4 == 0, "dwords");
+  typedef const int32_t __attribute__((address_space(4))) cint;
+  cint* c = (cint*)(uintptr_t)p;
+  int32_t w[sizeof(T) / 4];
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(T) / 4; ++i) w[i] = c[i];
+  T v;
+  __builtin_memcpy(&v, w, sizeof(T));
+  return v;
 }
 
 // Bytes [0, n) of a dword's four kept, the rest zero.
@@ -287,8 +304,8 @@ template <bool BF16>
 __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* smem) {
   const int item = b / a.n_kv, g = b - item * a.n_kv;
   const AttendItem& full = a.few.items[item];
-  const ItemHead it = full;
-  if (item >= a.work[kNFew]) return;
+  const ItemHead it = scalar_load(static_cast<const ItemHead*>(&full));
+  if (item >= scalar_load(a.work + kNFew)) return;
   typedef float Rows[kFewRows];
   float (*s_o)[kFewRows][kORow] = reinterpret_cast<float (*)[kFewRows][kORow]>(smem);
   Rows* s_m = reinterpret_cast<Rows*>(smem + kFewWaves * kFewRows * kORow * 4);
@@ -349,12 +366,12 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
   // last page the descriptor's range is empty: nothing is read.
   const int32_t* table = a.table + (int64_t)it.row * a.width;
   auto block_of = [&](int page) {
-    int id = table[min(page, it.page1 - 1)];
+    int id = scalar_load(table + min(page, it.page1 - 1));
     id = (unsigned)id < (unsigned)a.n_pages ? id : 0;
-    return (int64_t)__builtin_amdgcn_readfirstlane(id) * a.n_kv + g;
+    return (int64_t)id * a.n_kv + g;
   };
   auto page_rsrc = [&](int64_t block, int page) { return rsrc(a.pages + block * kBlock, page < it.page1 ? kBlock : 0); };
-  auto scale_of = [&](int64_t block) { return *reinterpret_cast<const float2*>(a.scales + 2 * block); };
+  auto scale_of = [&](int64_t block) { return scalar_load(reinterpret_cast<const float2*>(a.scales) + block); };
   u32x4 kr[8], vr[8];
   auto load8 = [&](u32x4 (&x)[8], rsrc_t r, int at) {
 #pragma unroll
@@ -364,7 +381,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
   int64_t next = 0;
   float2 scale = {1.0f, 1.0f};
   if (first < it.page1) {
-    const int64_t block = (int64_t)__builtin_amdgcn_readfirstlane(full.ids[w]) * a.n_kv + g;
+    const int64_t block = (int64_t)scalar_load(full.ids + w) * a.n_kv + g;
     const rsrc_t r0 = page_rsrc(block, first);
     load8(kr, r0, 0);
     load8(vr, r0, kHalfBlock);
@@ -532,12 +549,15 @@ __device__ __forceinline__ int v_lds(int d, int c) { return kVLds + d * 128 + 16
 // (+ 16 s); eight consecutive ones are a fragment of P^T and a 16-byte chunk of
 // a dim's row of V^T.
 //
-// Two waves a SIMD are too few to fill the gaps where products wait for the
-// vector unit: one after the other they kept the matrix cores 43 % and the
-// vector unit 60 % busy (5000 tokens, bf16: 257 us).  So the next page's staging
-// stands between the products of the scores, and a fragment's exponentials
-// between the products of the fragment before.  (The next page's scores beside
-// this one's exponentials take 32 registers more: they spilled, 272 us.)
+// The next page's staging stands between the products of the scores, and a
+// fragment's exponentials between the products of the fragment before.  What
+// bounds it: matrix cores and vector unit are busy about half the time each, and
+// two waves a SIMD (206 registers) overlap little more than that by chance: 5000
+// tokens 325 us in fp16 (630 TFLOP/s), 240 in bf16 (853).  Tried without gain:
+// fragments read three steps ahead; raised priority around the products; one
+// wave a SIMD with 64 rows and the next page's scores between this one's
+// exponentials, whose accumulators in AGPRs cost more copies than the shared
+// fragments save (326 us in bf16); the same with 32 rows, which spilled (272).
 constexpr int kManyLds = 4 * kHalfLds + kHeadD * 4;
 
 template <bool BF16>
@@ -545,8 +565,8 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
   int* s_nan = reinterpret_cast<int*>(s_page + 4 * kHalfLds);
   const int item = b / a.n_kv, g = b - item * a.n_kv;
   const AttendItem& full = a.many.items[item];
-  const ItemHead it = full;
-  if (item >= a.work[kNMany]) return;
+  const ItemHead it = scalar_load(static_cast<const ItemHead*>(&full));
+  if (item >= scalar_load(a.work + kNMany)) return;
   const int n_tok = min(it.n_tokens, a.n_tokens - it.token0);
   if (n_tok <= 0 || item - it.part + it.n_parts > a.many.groups / a.n_kv) return;
   const int tid = threadIdx.x, lane = lane_id(), r = lane & 31, h = lane >> 5;
@@ -586,9 +606,8 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
   }
   const float sc = BF16 ? ldexp2(a.scale, qe) : a.scale;
   const int lim = row < n_rows ? min(it.pos0 + tok + 1, it.kv_len) : 0;   // positions that this row sees
-  // ... that every row of the wave sees, and that some row of it does
+  // ... that every row of the wave sees
   const int all_see = min(it.pos0 + (32 * w >> lg) + 1, it.kv_len);
-  const int some_see = 32 * w < n_rows ? min(it.pos0 + (min(32 * w + 31, n_rows - 1) >> lg) + 1, it.kv_len) : 0;
 
   const float ninf = -__builtin_inff();
   f32x16 o[4];
@@ -598,9 +617,9 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
 
   const int32_t* table = a.table + (int64_t)it.row * a.width;
   auto block_of = [&](int page) {
-    int id = table[min(page, it.page1 - 1)];
+    int id = scalar_load(table + min(page, it.page1 - 1));
     id = (unsigned)id < (unsigned)a.n_pages ? id : 0;
-    return (int64_t)__builtin_amdgcn_readfirstlane(id) * a.n_kv + g;
+    return (int64_t)id * a.n_kv + g;
   };
   u32x4 kr[2], vr[2];                  // codes on their way into LDS: vectors tid and tid + 256
   auto load = [&](u32x4 (&x)[2], int64_t block, int half) {
@@ -634,7 +653,7 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
       for (int n = 0; n < 2; ++n) take_nans(vr[n], page * kPage + 16 * ((tid >> 4) & 3), &s_nan[st_d + 64 * n]);
     }
   };
-  auto scale_of = [&](int64_t block) { return *reinterpret_cast<const float2*>(a.scales + 2 * block); };
+  auto scale_of = [&](int64_t block) { return scalar_load(reinterpret_cast<const float2*>(a.scales) + block); };
 
   h8 kf[2][2], vf[4];
   auto read_k = [&](int ka, int st) {
@@ -651,16 +670,6 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
     const int at = (i & 1) * kHalfLds, other = kHalfLds - at;
     fix_v(page + 1, next_scale.y);
     int k_to = other + k_st, v_to = other + v_st;
-    if (page * kPage >= some_see) {    // the wave sees nothing here: it only stages
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        put_k(k_to, q);
-        put_v(v_to, q);
-      }
-      load(kr, after, 0);
-      load(vr, after, kHalfBlock);
-      return;
-    }
     int ka = at + k_rd, va = at + v_rd;
     asm volatile("" : "+v"(ka), "+v"(va), "+v"(k_to), "+v"(v_to));
     read_k(ka, 0);
@@ -731,8 +740,8 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
   };
 
   if (it.page0 < it.page1) {
-    const int64_t b0 = (int64_t)__builtin_amdgcn_readfirstlane(full.ids[0]) * a.n_kv + g;
-    const int64_t b1 = (int64_t)__builtin_amdgcn_readfirstlane(full.ids[1]) * a.n_kv + g;
+    const int64_t b0 = (int64_t)scalar_load(full.ids) * a.n_kv + g;
+    const int64_t b1 = (int64_t)scalar_load(full.ids + 1) * a.n_kv + g;
     int64_t b2 = block_of(it.page0 + 2);
     load(kr, b0, 0);
     load(vr, b0, kHalfBlock);
