@@ -32,16 +32,29 @@ struct ExtendArgs {
 
 __device__ __forceinline__ int pages_of(int n) { return (int)(((int64_t)n + kPage - 1) / kPage); }
 
+// Inclusive prefix sum over the lanes of a wave: by row_shr 1, 2, 4, 8 within
+// rows of 16, then row_bcast:15 and row_bcast:31 from row to row.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int64_t dpp_i64(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROW_MASK, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROW_MASK, 0xF, false);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {
+  v += dpp_i64<0x111, 0xF>(v);
+  v += dpp_i64<0x112, 0xF>(v);
+  v += dpp_i64<0x114, 0xF>(v);
+  v += dpp_i64<0x118, 0xF>(v);
+  v += dpp_i64<0x142, 0xA>(v);
+  v += dpp_i64<0x143, 0xC>(v);
+  return v;
+}
+
 // Exclusive prefix sum of one value per thread over the workgroup, and the
 // total.  s: 16 words that no one else uses until the next call's first barrier.
 __device__ __forceinline__ int64_t scan_excl(int64_t v, int64_t* s, int64_t& total) {
   const int lane = lane_id(), wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  int64_t x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+  const int64_t x = wave_scan(v);
   __syncthreads();
   if (lane == 63) s[wave] = x;
   __syncthreads();
@@ -72,13 +85,22 @@ __device__ __forceinline__ int page_id(const ExtendArgs& a, int id) {
   return (unsigned)id < (unsigned)a.n_pages ? id : 0;   // a damaged table reads page 0
 }
 
+// Page p of row r: a new one is still on the stack, whose top n_free is the
+// step's first; the others are in the table.
+__device__ __forceinline__ int row_page(const ExtendArgs& a, int r, int p, int past, int need, int n_free) {
+  const int fresh = p - pages_of(past);
+  return page_id(a, fresh >= 0 ? a.stack[max(n_free - 1 - need - fresh, 0)] : a.table[(int64_t)r * a.width + p]);
+}
+
 // Packed pairs of sums, high and low 32 bits, neither past 2^31.
 __device__ __forceinline__ int64_t pair(int64_t hi, int64_t lo) { return hi << 32 | lo; }
 
 __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
   extern __shared__ int32_t lds[];
   __shared__ int64_t s_scan[16];
+  __shared__ int s_taken;            // pages that rows take
   const int n = a.n_seqs, nt = blockDim.x, tid = threadIdx.x;
+  if (tid == 0) s_taken = 0;
   int32_t* s_tok = lds;              // exclusive sums over the rows: tokens (capped at max_tokens + 1),
   int32_t* s_need = s_tok + n;       // pages needed,
   int32_t* s_touch = s_need + n;     // pages touched,
@@ -116,8 +138,6 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
   }
   int64_t all_need;
   int64_t before = scan_excl(need, s_scan, all_need);
-  // the rows that the pool serves are a prefix of those that need pages
-  const int64_t served = min(all_need, (int64_t)n_free);
   int64_t touch = 0, tiles = 0, pages_few = 0, pages_many = 0;
   for (int r = r0; r < r1; ++r) {
     const int pages = s_need[r], past = s_past[r], t = s_new[r];
@@ -128,6 +148,8 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
     a.kv_len[r] = kv;
     a.rejected[r] = taken ? 0 : 1;
     if (taken) a.lens[r] = kv;
+    // the rows that the pool serves are the first ones that need pages
+    if (taken && pages > 0) atomicMax(&s_taken, (int)before);
     s_kv[r] = kv;
     const int in = max(0, min(t, a.max_tokens - s_tok[r]));
     s_new[r] = in;
@@ -164,34 +186,21 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
   const int c_few = share(all_few, a.l.parts_few), c_many = share(all_many, a.l.parts_many);
   __syncthreads();
 
-  // table entries.  The rows that are served are those whose need ends within
-  // the pool; entries past the last of them belong to rejected rows.
-  for (int64_t i = tid; i < served; i += nt) {
-    const int r = row_of(s_need, n, (int)i), j = (int)i - s_need[r];
-    if (s_kv[r] == 0) continue;
+  const int taken = s_taken;
+  for (int i = tid; i < taken; i += nt) {
+    const int r = row_of(s_need, n, i), j = i - s_need[r];
     a.table[(int64_t)r * a.width + pages_of(s_past[r]) + j] = page_id(a, a.stack[n_free - 1 - i]);
   }
   if (tid == 0) {
     a.work[kNAppend] = n_touch;
-  }
-  __syncthreads();                   // the table is read below; every row's kv_len is known
-  // the pages that rows took: the end of the last served row's need
-  {
-    int64_t taken = 0;
-    for (int r = r0; r < r1; ++r) {
-      const int k = s_kv[r];
-      if (k > 0) taken += pages_of(k) - pages_of(s_past[r]);
-    }
-    int64_t all;
-    scan_excl(taken, s_scan, all);
-    if (tid == 0) a.n_free[0] = n_free - (int)all;
+    a.n_free[0] = n_free - taken;
   }
 
   AppendItem* ap = reinterpret_cast<AppendItem*>(a.work + a.l.append);
   for (int i = tid; i < n_touch; i += nt) {
     const int r = row_of(s_touch, n, i), past = s_past[r], p = past / kPage + i - s_touch[r];
     const int held = max(past - p * kPage, 0), upto = min(s_kv[r] - p * kPage, kPage);
-    ap[i] = AppendItem{page_id(a, a.table[(int64_t)r * a.width + p]), s_tok[r] + p * kPage + held - past, held, upto};
+    ap[i] = AppendItem{row_page(a, r, p, past, s_need[r], n_free), s_tok[r] + p * kPage + held - past, held, upto};
   }
 
   // attention tiles, cut into parts
@@ -226,13 +235,12 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
       const int slot = (int)(few ? x_slots & 0xFFFFFFFF : x_slots >> 32);
       AttendItem* list = few ? few_list : many_list;
       const int each = parts > 1 ? ((pages + parts - 1) / parts + 3) / 4 * 4 : pages;   // at most c: as many parts, alike
-      const int32_t* ids = a.table + (int64_t)r * a.width;
       for (int k = 0; k < parts; ++k) {
         AttendItem x{{r, tok0, count, s_past[r] + first, min(k * each, pages), min((k + 1) * each, pages),
                       s_kv[r], k, parts, slot, {0, 0}}, {}};
 #pragma unroll
         for (int e = 0; e < kFewWaves; ++e)
-          if (few || e < 2) x.ids[e] = x.page0 + e < x.page1 ? page_id(a, ids[x.page0 + e]) : 0;
+          if (few || e < 2) x.ids[e] = x.page0 + e < x.page1 ? row_page(a, r, x.page0 + e, s_past[r], s_need[r], n_free) : 0;
         list[item + k] = x;
       }
     }
@@ -248,7 +256,7 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
         const int r = row_of(s_tok, n, t);
         if (s_kv[r]) {
           pos = s_past[r] + t - s_tok[r];
-          slot = page_id(a, a.table[(int64_t)r * a.width + pos / kPage]) * kPage + pos % kPage;
+          slot = row_page(a, r, pos / kPage, s_past[r], s_need[r], n_free) * kPage + pos % kPage;
         }
       }
       a.positions[t] = pos;
@@ -395,7 +403,7 @@ int oi2_page_extend(const oi2_paged* c, const oi2_page_plan* p, const int32_t* n
   const ExtendArgs a = extend_args(c, p, new_lens);
   hipStream_t st = (hipStream_t)stream;
   // short steps: fewer waves have less to wait for at each barrier
-  const int threads = a.n_seqs <= 256 && p->max_tokens <= 1024 ? 256 : 1024;
+  const int threads = a.n_seqs <= 64 && p->max_tokens <= 128 ? 64 : a.n_seqs <= 256 && p->max_tokens <= 1024 ? 256 : 1024;
   hipLaunchKernelGGL(k_page_extend, dim3(1), dim3(threads), (size_t)a.n_seqs * 7 * 4, st, a);
   OI2_CHECK_LAUNCH();
   if (!a.fill) {
@@ -419,7 +427,7 @@ int oi2_page_rewind(const oi2_paged* c, const int32_t* lens, void* stream) {
   a.lens = c->lens;
   a.stack = c->free_pages;
   a.n_free = c->n_free;
-  hipLaunchKernelGGL(k_page_rewind, dim3(1), dim3(a.n_seqs <= 256 ? 256 : 1024), (size_t)a.n_seqs * 2 * 4,
+  hipLaunchKernelGGL(k_page_rewind, dim3(1), dim3(a.n_seqs <= 64 ? 64 : a.n_seqs <= 256 ? 256 : 1024), (size_t)a.n_seqs * 2 * 4,
                      (hipStream_t)stream, a);
   OI2_CHECK_LAUNCH();
   return OI2_OK;

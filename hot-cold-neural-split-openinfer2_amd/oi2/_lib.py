@@ -247,7 +247,8 @@ class on_device:
         self.index = device.index
 
     def __enter__(self):
-        self.before = torch.cuda.current_device()
+        torch.cuda.init()
+        self.before = torch._C._cuda_getDevice()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
 

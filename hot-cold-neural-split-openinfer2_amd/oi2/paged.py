@@ -108,6 +108,7 @@ class PagedKVCache:
                                  device=dev)
         self._scales = torch.full((self.n_layers, self.n_pages, self.n_kv, 2), 2.0 ** -40, dtype=torch.float32,
                                   device=dev)
+        self._views = {}
         self._struct = _lib.Paged(self.n_q, self.n_kv, self.n_seqs, self.max_len, self.n_pages, self.n_layers,
                                   self.block_table.data_ptr(), self.lens.data_ptr(), self.free.data_ptr(),
                                   self.n_free.data_ptr(), self.pages.data_ptr() or None,
@@ -221,13 +222,13 @@ class PagedKVCache:
         q = self._rows(q, self.n_q, "q")
         n = self._tokens(q, plan)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor like q")
         L = _lib.lib()
         nbytes = plan._attend_bytes
         with _lib.on_device(self.device):
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            ws = q.new_empty((nbytes,), dtype=torch.uint8)
             _lib.check(L.oi2_kv_attend(
                 ctypes.byref(self._struct), ctypes.byref(plan._struct), layer, _lib.dtype_code(q.dtype), n,
                 ctypes.byref(_lib.heads(q)), HEAD_DIM ** -0.5 if scale is None else float(scale), out.data_ptr(),
@@ -241,16 +242,22 @@ class PagedKVCache:
         dimensions are the 128 dims and the ones before them the 64 positions of
         a page, in order; the memory holds them in the order of the attention's
         loads."""
-        x = self.pages[self._layer(layer)].view(torch.float8_e4m3fn)
-        k = x[:, :, 0].view(self.n_pages, self.n_kv, 4, 8, 4, 4, 16).permute(0, 1, 4, 2, 5, 3, 6)
-        v = x[:, :, 1].view(self.n_pages, self.n_kv, 8, 4, 16, 16).permute(0, 1, 3, 5, 2, 4)
-        return k, v
+        return self._layer_views(layer)[0]
 
     def scales(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The scales (n_pages, n_kv) of k and of v, as views: powers of two;
         v's is negative where the page holds a NaN in v."""
-        x = self._scales[self._layer(layer)]
-        return x[..., 0], x[..., 1]
+        return self._layer_views(layer)[1]
+
+    def _layer_views(self, layer: int):
+        layer = self._layer(layer)
+        if layer not in self._views:
+            x = self.pages[layer].view(torch.float8_e4m3fn)
+            k = x[:, :, 0].view(self.n_pages, self.n_kv, 4, 8, 4, 4, 16).permute(0, 1, 4, 2, 5, 3, 6)
+            v = x[:, :, 1].view(self.n_pages, self.n_kv, 8, 4, 16, 16).permute(0, 1, 3, 5, 2, 4)
+            s = self._scales[layer]
+            self._views[layer] = (k, v), (s[..., 0], s[..., 1])
+        return self._views[layer]
 
     def read(self, layer: int, row: int, dtype=torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
         """What a row's cache stands for: k and v (n_kv, length, 128), as the

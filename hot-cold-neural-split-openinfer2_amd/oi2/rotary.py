@@ -121,7 +121,7 @@ class Rotary:
 
     def _output(self, out, x: torch.Tensor, what: str) -> torch.Tensor:
         if out is None:
-            return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            return torch.empty_like(x, memory_format=torch.contiguous_format)
         if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
             raise ValueError(f"{what} must be a contiguous tensor like its input")
         return out
