@@ -28,6 +28,8 @@
 // Cache layout: k_cache, v_cache (batch, n_kv, cap, 128) fp16, the
 // reference's (B, n_kv, S, D) tensors with room for cap positions.
 #include "attn_kernels.h"
+#include "kv_cache.h"
+#include "rotary.h"
 #include "capi_util.h"
 #include "decode_util.h"
 #include "ffn_kernels.h"
@@ -61,7 +63,7 @@ struct GemvArgs {
   uint16_t* k_cache;
   uint16_t* v_cache;
   int n_kv, cap, past, seq;
-  const float* cos;           // (seq, 64)
+  const float* cos;           // (seq, 64); null: q and k are not rotated
   const float* sin;
   uint32_t* counters;         // cleared here (once per call) for k_attn_sdpa
   int n_counters;
@@ -69,6 +71,7 @@ struct GemvArgs {
   uint16_t* out;              // (rows, H)
   const uint16_t* residual;   // (rows, H) or null
   uint16_t* x_out;
+  const int32_t* positions;   // (rows) or null: a negative one's out is 0
 };
 
 struct SdpaArgs {
@@ -258,8 +261,9 @@ __global__ __launch_bounds__(kThreads) void k_attn_gemv(GemvArgs a) {
   }
   if (lane >= R) return;
   const int row = lane;
-  const float y0 = round_f16(t0), y1 = round_f16(t1);
+  float y0 = round_f16(t0), y1 = round_f16(t1);
   if (a.mode == 1) {
+    if (a.positions && a.positions[row] < 0) y0 = y1 = 0.0f;
     uint16_t* o = a.out + (size_t)row * kH + hb * kHd + j;
     o[0] = float_to_half_bits(y0);
     o[kHalf] = float_to_half_bits(y1);
@@ -273,7 +277,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_gemv(GemvArgs a) {
   }
   const int b = row / a.seq, t = row - b * a.seq;
   float o0 = y0, o1 = y1;
-  if (hb < a.blocks0 + a.blocks1) {
+  if (hb < a.blocks0 + a.blocks1 && a.cos) {
     const RopePair o = rope_f16((_Float16)y0, (_Float16)y1, (_Float16)a.cos[t * kHalf + j], (_Float16)a.sin[t * kHalf + j]);
     o0 = (float)o.a;
     o1 = (float)o.b;
@@ -827,6 +831,21 @@ struct WsLayout {
   size_t q, attn, counters, part, total;
 };
 
+// The workspace of a layer over the paged cache.
+struct PagedLayout {
+  size_t q, k, v, attn, attend, total;
+};
+PagedLayout paged_layout(int rows, int n_q, int n_kv, size_t attend_bytes) {
+  PagedLayout w;
+  w.q = 0;
+  w.k = w.q + align256((size_t)rows * n_q * kHd * 2);
+  w.v = w.k + align256((size_t)rows * n_kv * kHd * 2);
+  w.attn = w.v + align256((size_t)rows * n_kv * kHd * 2);
+  w.attend = w.attn + align256((size_t)rows * kH * 2);
+  w.total = w.attend + align256(attend_bytes);
+  return w;
+}
+
 // The split partial sums: none when the span (past + seq positions) fits one
 // workgroup per query head or the prompt attention runs, else the splits
 // choose_steps picks for that span (the looping kernel makes at most as many).
@@ -1023,6 +1042,118 @@ int oi2_attn_forward(const uint16_t* x, int32_t batch, int32_t seq, const oi2_at
     o.residual = x_out ? x : nullptr;
     o.x_out = x_out;
     launch_gemv(o, rows, kH / kHd, st);
+  }
+  OI2_CHECK_LAUNCH();
+  return OI2_OK;
+}
+
+size_t oi2_attn_paged_workspace_bytes(const oi2_paged* c, int32_t max_tokens, int32_t max_new, int32_t n_tokens) {
+  const size_t attend = oi2_kv_attend_workspace_bytes(c, max_tokens, max_new);
+  if (!attend || n_tokens < 1 || n_tokens > max_tokens) return 0;
+  return paged_layout(n_tokens, c->n_q, c->n_kv, attend).total;
+}
+
+int oi2_attn_forward_paged(const uint16_t* x, int32_t n_tokens, const oi2_attn* w, float eps, const oi2_rotary* rotary,
+                           const oi2_paged* c, const oi2_page_plan* p, int32_t layer, uint16_t* out, uint16_t* x_out,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  OI2_CHECK_ARG(w && rotary, "null attention weights or rotary frequencies");
+  if (int rc = check_paged(c, layer, true)) return rc;
+  if (int rc = check_plan(c, p)) return rc;
+  if (int rc = check_rotary(rotary)) return rc;
+  OI2_CHECK_ARG(rotary->head_dim == kHd, "rotary head_dim %d, expected %d", rotary->head_dim, kHd);
+  OI2_CHECK_ARG(w->n_q == c->n_q && w->n_kv == c->n_kv, "%d query and %d kv heads on a cache of %d and %d", w->n_q, w->n_kv,
+                c->n_q, c->n_kv);
+  OI2_CHECK_ARG((int64_t)w->n_q * kHd == kH, "n_q %d: head_dim = %d / n_q must be %d", w->n_q, kH, kHd);
+  OI2_CHECK_ARG(n_tokens >= 0 && n_tokens <= p->max_tokens, "%d tokens in a plan of %d", n_tokens, p->max_tokens);
+  if (n_tokens == 0) return OI2_OK;
+  OI2_CHECK_ARG(x && (uintptr_t)x % 16 == 0, "x must be non-null and 16-byte aligned");
+  OI2_CHECK_ARG(w->wq && w->wk && w->wv && w->wo, "null weight");
+  OI2_CHECK_ARG((uintptr_t)w->wq % 16 == 0 && (uintptr_t)w->wk % 16 == 0 && (uintptr_t)w->wv % 16 == 0 &&
+                    (uintptr_t)w->wo % 16 == 0,
+                "weights must be 16-byte aligned");
+  OI2_CHECK_ARG(w->norm_w && (uintptr_t)w->norm_w % 16 == 0,
+                "norm weight must be non-null (ones for nn.RMSNorm's default) and 16-byte aligned");
+  OI2_CHECK_ARG(out, "null output");
+  const size_t attend = oi2_kv_attend_workspace_bytes(c, p->max_tokens, p->max_new);
+  const PagedLayout L = paged_layout(n_tokens, w->n_q, w->n_kv, attend);
+  OI2_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= L.total,
+                "workspace of %zu bytes, %zu needed, 16-byte aligned", workspace_bytes, L.total);
+  hipStream_t st = (hipStream_t)stream;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  uint16_t* qb = reinterpret_cast<uint16_t*>(ws + L.q);
+  uint16_t* kb = reinterpret_cast<uint16_t*>(ws + L.k);
+  uint16_t* vb = reinterpret_cast<uint16_t*>(ws + L.v);
+  uint16_t* attn = reinterpret_cast<uint16_t*>(ws + L.attn);
+  const oi2_heads q{qb, w->n_q, (int64_t)w->n_q * kHd, kHd};
+  const oi2_heads k{kb, w->n_kv, kHd, (int64_t)n_tokens * kHd}, v{vb, w->n_kv, kHd, (int64_t)n_tokens * kHd};
+
+  // q, k, v of the normalised rows, not rotated; k and v as a cache of one
+  // sequence of n_tokens positions
+  const bool prompt = n_tokens >= kPromptRows;
+  if (prompt) {
+    hipLaunchKernelGGL(k_rmsnorm, dim3(n_tokens), dim3(kThreads), 0, st, x, w->norm_w, eps, attn);
+    OI2_CHECK_LAUNCH();
+    ProjArgs a{};
+    a.w0 = w->wq;
+    a.w1 = w->wk;
+    a.w2 = w->wv;
+    a.blocks0 = w->n_q;
+    a.blocks1 = w->n_kv;
+    a.q = qb;
+    a.q_width = w->n_q * kHd;
+    a.k_cache = kb;
+    a.v_cache = vb;
+    a.n_kv = w->n_kv;
+    a.cap = n_tokens;
+    a.seq = n_tokens;
+    project(a, attn, n_tokens, w->n_q + 2 * w->n_kv, st);
+  } else {
+    GemvArgs a{};
+    a.x = x;
+    a.norm_w = w->norm_w;
+    a.eps = eps;
+    a.w0 = w->wq;
+    a.w1 = w->wk;
+    a.w2 = w->wv;
+    a.blocks0 = w->n_q;
+    a.blocks1 = w->n_kv;
+    a.q = qb;
+    a.q_width = w->n_q * kHd;
+    a.k_cache = kb;
+    a.v_cache = vb;
+    a.n_kv = w->n_kv;
+    a.cap = n_tokens;
+    a.seq = n_tokens;
+    launch_gemv(a, n_tokens, w->n_q + 2 * w->n_kv, st);
+  }
+  OI2_CHECK_LAUNCH();
+  if (int rc = oi2_kv_append(c, p, layer, OI2_DTYPE_F16, n_tokens, &k, &v, rotary, &q, qb, stream)) return rc;
+  if (int rc = oi2_kv_attend(c, p, layer, OI2_DTYPE_F16, n_tokens, &q, 1.0f / sqrtf((float)kHd), attn, ws + L.attend, attend,
+                             stream))
+    return rc;
+  if (prompt) {
+    ProjArgs a{};
+    a.w0 = w->wo;
+    a.blocks0 = kH / kHd;
+    a.mode = 1;
+    a.seq = n_tokens;
+    a.out = out;
+    a.residual = x_out ? x : nullptr;
+    a.x_out = x_out;
+    a.positions = p->positions;
+    project(a, attn, n_tokens, kH / kHd, st);
+  } else {
+    GemvArgs a{};
+    a.x = attn;
+    a.w0 = w->wo;
+    a.blocks0 = kH / kHd;
+    a.mode = 1;
+    a.out = out;
+    a.residual = x_out ? x : nullptr;
+    a.x_out = x_out;
+    a.positions = p->positions;
+    launch_gemv(a, n_tokens, kH / kHd, st);
   }
   OI2_CHECK_LAUNCH();
   return OI2_OK;

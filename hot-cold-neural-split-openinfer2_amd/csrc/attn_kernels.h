@@ -37,7 +37,7 @@ struct ProjArgs {
   uint16_t* k_cache;
   uint16_t* v_cache;
   int n_kv, cap, past, seq;
-  const float* cos;           // (seq, 64)
+  const float* cos;           // (seq, 64); null: q and k are not rotated
   const float* sin;
   uint32_t* counters;         // n_counters words that the launch clears
   int n_counters;
@@ -45,6 +45,7 @@ struct ProjArgs {
   uint16_t* out;              // (rows, H)
   const uint16_t* residual;   // (rows, H) or null
   uint16_t* x_out;
+  const int32_t* positions;   // (rows) or null: a negative one's out is 0
 };
 
 constexpr int kProjMaxRows = 0x7FFFFFFF / (2 * 4096) / 128 * 128;   // 32-bit byte offsets into the rows, whole tiles

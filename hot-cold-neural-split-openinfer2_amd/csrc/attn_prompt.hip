@@ -266,6 +266,7 @@ __global__ __launch_bounds__(256, KB == 64 ? 2 : 1) void k_proj(ProjArgs a, int 
     u32x4 v1 = *reinterpret_cast<const u32x4*>(y1 + r * kHalfHead + j);
     if (a.mode == 1) {
       const size_t o = (size_t)row * kH + hb * kHeadDim + j;
+      if (a.positions && a.positions[row] < 0) v0 = v1 = u32x4{0, 0, 0, 0};
       *reinterpret_cast<u32x4_a2*>(a.out + o) = v0;
       *reinterpret_cast<u32x4_a2*>(a.out + o + kHalfHead) = v1;
       if (a.residual) {
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(256, KB == 64 ? 2 : 1) void k_proj(ProjArgs a, int 
       continue;
     }
     const int bt = row / a.seq, t = row - bt * a.seq;
-    if (rot) {
+    if (rot && a.cos) {
       const f32x4_a4* pc = reinterpret_cast<const f32x4_a4*>(a.cos + (size_t)t * kHalfHead + j);
       const f32x4_a4* ps = reinterpret_cast<const f32x4_a4*>(a.sin + (size_t)t * kHalfHead + j);
       const f32x4 c[2] = {pc[0], pc[1]}, s[2] = {ps[0], ps[1]};
@@ -394,6 +395,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void k_proj_few(ProjArgs a) {
     y1 = round_f16(y1);
     if (a.mode == 1) {
       const size_t o = (size_t)row * kH + hb * kHeadDim + j;
+      if (a.positions && a.positions[row] < 0) y0 = y1 = 0.0f;
       a.out[o] = float_to_half_bits(y0);
       a.out[o + kHalfHead] = float_to_half_bits(y1);
       if (a.residual) {
@@ -404,7 +406,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void k_proj_few(ProjArgs a) {
     }
     const int bt = row / a.seq, tt = row - bt * a.seq;
     float o0 = y0, o1 = y1;
-    if (hb < a.blocks0 + a.blocks1) {
+    if (hb < a.blocks0 + a.blocks1 && a.cos) {
       const size_t e = (size_t)tt * kHalfHead + j;
       const RopePair o = rope_f16((_Float16)y0, (_Float16)y1, (_Float16)a.cos[e], (_Float16)a.sin[e]);
       o0 = (float)o.a;

@@ -26,6 +26,8 @@ import ctypes
 import torch
 
 from . import _lib
+from .paged import PagedKVCache, PagePlan
+from .rotary import Rotary
 
 HEAD_DIM = 128
 
@@ -177,3 +179,39 @@ class GroupedQueryAttention(torch.nn.Module):
             _lib.ptr(residual_out), ws.data_ptr(), nbytes, _lib.stream_handle(self.device)))
         self._len = past + T
         return out, (self._k[:, :, :past + T], self._v[:, :, :past + T])
+
+    def forward_paged(self, x: torch.Tensor, cache: PagedKVCache, plan: PagePlan, rotary: Rotary,
+                      layer: int | None = None, residual_out: torch.Tensor | None = None) -> torch.Tensor:
+        """The same for the packed tokens of a step over a paged cache of
+        requests of different lengths: x (tokens, H) fp16 in the order of
+        ``plan``, which ``cache.extend`` has laid out; ``layer`` of the cache,
+        this layer's index by default.  k and v go to the cache in 8 bits, and
+        every token attends, causally, to what its row's cache then holds.
+        Returns out (tokens, H); with ``residual_out`` like x, x + out goes
+        there.  Tokens without a position (of rejected rows, or past the step's
+        last one) give 0, and x in residual_out."""
+        if x.dtype != torch.float16 or x.dim() != 2 or x.shape[1] != self.hidden:
+            raise TypeError(f"x must be (tokens, {self.hidden}) fp16, got {tuple(x.shape)} {x.dtype}")
+        if (cache.n_q, cache.n_kv) != (self.n_q, self.n_kv):
+            raise ValueError(f"a cache of {cache.n_q} query and {cache.n_kv} kv heads for {self.n_q} and {self.n_kv}")
+        if rotary.head_dim != HEAD_DIM:
+            raise ValueError(f"rotary of head_dim {rotary.head_dim}, expected {HEAD_DIM}")
+        if not (x.device == cache.device == rotary.device == self.wq.device):
+            raise ValueError(f"x on {x.device}, weights on {self.wq.device}, cache on {cache.device}, rotary on {rotary.device}")
+        plan, layer = cache._plan(plan), cache._layer(self.layer_idx if layer is None else layer)
+        n = cache._tokens(x, plan)
+        if residual_out is not None and (residual_out.shape != x.shape or residual_out.dtype != torch.float16
+                                         or residual_out.device != x.device or not residual_out.is_contiguous()):
+            raise ValueError("residual_out must be a contiguous fp16 tensor shaped like x")
+        xc = x.contiguous()
+        L = _lib.lib()
+        with _lib.on_device(cache.device):
+            out = torch.empty_like(xc)
+            nbytes = L.oi2_attn_paged_workspace_bytes(ctypes.byref(cache._struct), plan.max_tokens, plan.max_new,
+                                                      max(n, 1))
+            ws = x.new_empty((nbytes,), dtype=torch.uint8)
+            _lib.check(L.oi2_attn_forward_paged(
+                xc.data_ptr(), n, ctypes.byref(self._struct), self.eps, ctypes.byref(rotary._struct),
+                ctypes.byref(cache._struct), ctypes.byref(plan._struct), layer, out.data_ptr(),
+                _lib.ptr(residual_out), ws.data_ptr(), nbytes, _lib.stream_handle(cache.device)))
+        return out

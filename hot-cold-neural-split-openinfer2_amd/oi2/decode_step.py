@@ -21,6 +21,8 @@ import torch
 
 from .attention import GroupedQueryAttention
 from .layer import SparseFFNLayer
+from .paged import PagedKVCache, PagePlan
+from .rotary import Rotary
 from .stack import DecodeStack
 
 
@@ -71,5 +73,40 @@ class DecoderStep:
             stack.layer(li, resid.reshape(H), out.reshape(H))         # FFN, and layer li + 1's set
             x = out
         return x, new_kv
+
+    def forward_paged(self, x: torch.Tensor, cache: PagedKVCache, plan: PagePlan, rotary: Rotary) -> torch.Tensor:
+        """The loop over a paged cache: x (tokens, H) fp16, the packed tokens of
+        the step that ``cache.extend`` laid out in ``plan`` for requests of
+        different lengths.  Layer li uses layer li of the cache.  The FFN takes
+        the tokens as one batch, which shares a predicted cold set (over a
+        DecodeStack: one token); tokens without a position take part in it, so
+        give them finite values.  Returns x after the last layer's FFN."""
+        if x.dim() != 2:
+            raise ValueError(f"x must be (tokens, hidden), got {tuple(x.shape)}")
+        N, H = x.shape
+        if cache.n_layers < len(self.attention_layers):
+            raise ValueError(f"a cache of {cache.n_layers} layers for {len(self.attention_layers)}")
+        if N == 0:
+            return x
+        x = x.contiguous()
+        stack = self.ffn_layers if isinstance(self.ffn_layers, DecodeStack) else None
+        if stack is not None:
+            if N != 1:
+                raise ValueError(f"a DecodeStack runs one token at a time, got {N}")
+            stack.predict(0, x.reshape(H))
+        else:
+            prefetch = self.ffn_layers[0].submit_cold_fetch(x[None])
+        for li, attn in enumerate(self.attention_layers):
+            resid = torch.empty_like(x)
+            attn.forward_paged(x, cache, plan, rotary, layer=li, residual_out=resid)
+            if stack is not None:
+                x = torch.empty_like(x)
+                stack.layer(li, resid.reshape(H), x.reshape(H))
+                continue
+            this = prefetch
+            if li + 1 < len(self.ffn_layers):
+                prefetch = self.ffn_layers[li + 1].submit_cold_fetch(resid[None])
+            x = self.ffn_layers[li](resid[None], this)[0]
+        return x
 
     __call__ = forward

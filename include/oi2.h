@@ -480,7 +480,10 @@ typedef struct oi2_page_plan {
   int32_t* slots;             /* (max_tokens) page * 64 + place in it, -1 none */
   int32_t* kv_len;            /* (n_seqs) positions of the row with the step's; 0: rejected */
   int32_t* rejected;          /* (n_seqs) 1 where the row could not grow */
-  int32_t* work;              /* oi2_page_plan_bytes bytes, 16-byte aligned: work lists */
+  int32_t* work;              /* oi2_page_plan_bytes bytes, 16-byte aligned, zeroed
+                                 before the first use: work lists, and counters
+                                 that every oi2_kv_attend leaves at zero.  So a
+                                 plan serves one attention at a time. */
 } oi2_page_plan;
 
 /* Bytes of a plan's work lists; 0 for sizes that are not supported. */
@@ -556,11 +559,28 @@ size_t oi2_kv_attend_workspace_bytes(const oi2_paged* c, int32_t max_tokens, int
  * q (n_tokens, n_q, 128) with strides, out (n_tokens, n_q, 128) dense, both of
  * `dtype` (OI2_DTYPE_F16 or _BF16).  Scores, the softmax's sums and the output
  * are fp32 until the one rounding of out; probabilities enter the products as
- * two fp16 parts.  The tokens of a rejected row give zeros; rows of out past
+ * two fp16 parts where out is fp16, and rounded to one where it is bf16.  The
+ * tokens of a rejected row give zeros; rows of out past
  * the step's last token are left as they were. */
 int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
                   const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes,
                   void* stream);
+
+/* Workspace bytes of oi2_attn_forward_paged; 0 for sizes that are not supported. */
+size_t oi2_attn_paged_workspace_bytes(const oi2_paged* c, int32_t max_tokens, int32_t max_new, int32_t n_tokens);
+
+/* GroupedQueryAttention.forward (engine.py:90-125) for the n_tokens packed
+ * tokens of the plan's step, x (n_tokens, H) fp16, over the paged cache:
+ * RMSNorm and projections as oi2_attn_forward, then oi2_kv_append with the
+ * rotary positions (the plan's; fp64, where the reference rounds its tables
+ * to fp16), oi2_kv_attend (causal, also behind a cache) and o_proj.  out
+ * (n_tokens, H) fp16; x_out, if not NULL, receives fp16(x + out).  out is 0
+ * for tokens without a position: those of rejected rows, and past the step's
+ * last one. */
+int oi2_attn_forward_paged(const uint16_t* x, int32_t n_tokens, const oi2_attn* w, float eps,
+                           const oi2_rotary* rotary, const oi2_paged* c, const oi2_page_plan* p, int32_t layer,
+                           uint16_t* out, uint16_t* x_out, void* workspace, size_t workspace_bytes,
+                           void* stream);
 
 /* ---- split writer ------------------------------------------------------- */
 /* Bytes of one cold_weights.bin section with n_cold records: the 16-byte

@@ -156,3 +156,36 @@ def test_null_structs_are_refused():
     assert lib.oi2_page_plan_bytes(None, 4, 4) == 0 and lib.oi2_page_plan_bytes(ref(c), 0, 4) == 0
     assert lib.oi2_kv_attend_workspace_bytes(ref(c), 4, 0) == 0
     assert lib.oi2_kv_append(ref(c), ref(p), 0, 2, 0, ref(h["k"]), ref(h["v"]), None, None, None, None) == 0    # no token: nothing to do
+
+
+@pytest.mark.parametrize("kw,says", [
+    (dict(n_kv=4), b"4 kv heads on a cache of 32 and 8"), (dict(n_q=16), b"16 query"), (dict(layer=2), b"layer"), (dict(pages=None), b"pages"),
+    (dict(cu=None), b"null"), (dict(head_dim=64, rotary_dim=64), b"head_dim"), (dict(n=17), b"17 tokens"), (dict(n=-1), b"-1 tokens"),
+    (dict(x=None), b"x must"), (dict(x=72), b"x must"), (dict(wq=None), b"null weight"), (dict(wo=72), b"weights must"),
+    (dict(norm_w=None), b"norm"), (dict(out=None), b"output"), (dict(ws=1000), b"workspace"),
+])
+def test_layer_refusals_of_the_c_abi(kw, says):
+    lib = oi2.load_library()
+    c, p, r, _ = _structs(**{k: v for k, v in kw.items() if k not in ("n_q", "n_kv")})
+    w = dict(wq=64, wk=64, wv=64, wo=64, n_q=32, n_kv=8, norm_w=64)
+    w = _lib.Attn(**{**w, **{k: v for k, v in kw.items() if k in w}})
+    ref = ctypes.byref
+
+    def call(n):
+        return lib.oi2_attn_forward_paged(kw.get("x", 64), n, ref(w), 1e-5, ref(r), ref(c), ref(p), kw.get("layer", 0),
+                                          kw.get("out", 64), None, 64, kw.get("ws", 1 << 40), None)
+    assert call(kw.get("n", 4)) == 1
+    assert says in lib.oi2_last_error(), lib.oi2_last_error()
+
+
+def test_layer_null_structs_and_no_tokens():
+    lib = oi2.load_library()
+    c, p, r, _ = _structs()
+    w = _lib.Attn(wq=64, wk=64, wv=64, wo=64, n_q=32, n_kv=8, norm_w=64)
+    ref = ctypes.byref
+    for drop in range(4):
+        a = [None if i == drop else ref(x) for i, x in enumerate((w, r, c, p))]
+        assert lib.oi2_attn_forward_paged(64, 4, a[0], 1e-5, a[1], a[2], a[3], 0, 64, None, 64, 1 << 40, None) == 1
+    assert lib.oi2_attn_forward_paged(64, 0, ref(w), 1e-5, ref(r), ref(c), ref(p), 0, 64, None, 64, 1 << 40, None) == 0
+    assert lib.oi2_attn_paged_workspace_bytes(None, 4, 4, 4) == 0
+    assert lib.oi2_attn_paged_workspace_bytes(ref(c), 4, 4, 5) == 0 and lib.oi2_attn_paged_workspace_bytes(ref(c), 4, 4, 0) == 0
