@@ -16,7 +16,7 @@ constexpr float kCodeMax = 448.0f;
 constexpr int kExpMin = -40, kExpMax = 60;
 
 // Query rows (tokens times query heads per kv head) of a workgroup of the
-// attention: up to 16 in the kernel for few rows, 256 in the one for many.
+// attention: up to 16 in the kernel for few rows, 128 in the one for many.
 constexpr int kFewRows = 16, kManyRows = 128;
 // Waves of a workgroup for few rows, each every fourth page.
 constexpr int kFewWaves = 4;

@@ -8,8 +8,12 @@
 // the sums and the lists; the positions and slots of the tokens are its own
 // work for short steps and a launch of many workgroups for long ones.
 //
-// Bound by the chain of barriers and dependent loads, not by bytes: a few
-// kilobytes for a decoding step.
+// Bound by the chain of barriers, dependent loads and fetches of its own code
+// (which every launch fetches anew), not by bytes: a few kilobytes for a
+// decoding step.  So counts are 32-bit and saturate, shares are products and
+// groups shifts, and plans of short rows leave out the lists for long ones:
+// 6 KB of code instead of 11, eight rows of a step 11.1 -> 7.6 us.  700 prompts
+// of 115 thousand tokens: 32 us and 5 for the positions and slots.
 #include "capi_util.h"
 #include "kv_cache.h"
 #include "oi2_device.h"
@@ -19,53 +23,65 @@ namespace {
 
 // Tokens up to which the one workgroup writes positions and slots itself.
 constexpr int kOneLaunchTokens = 4096;
+constexpr int kLogFew = 4, kLogMany = 7;
+static_assert(1 << kLogFew == kFewRows && 1 << kLogMany == kManyRows);
 
 struct ExtendArgs {
-  int n_seqs, max_len, width, n_pages, max_tokens, max_new, group;
-  int few_only;               // no row is long enough for the kernel for many rows
+  int n_seqs, max_len, width, n_pages, max_tokens, max_new, log2_group;
   int fill;                   // positions and slots are written here
   const int32_t* new_lens;
   int32_t *table, *lens, *stack, *n_free;
   int32_t *cu, *positions, *slots, *kv_len, *rejected, *work;
+  double per_part_few, per_part_many;   // 1 / parts
   PlanLayout l;
 };
 
 __device__ __forceinline__ int pages_of(int n) { return (int)(((int64_t)n + kPage - 1) / kPage); }
 
+// Counts saturate at kMost, so that sums of any lengths compare rightly with
+// the sizes that they are checked against, all of them below it.
+constexpr uint32_t kMost = 0x7FFFFFFF;
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return min(a + b, kMost); }
+
 // Inclusive prefix sum over the lanes of a wave: by row_shr 1, 2, 4, 8 within
 // rows of 16, then row_bcast:15 and row_bcast:31 from row to row.
 template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ int64_t dpp_i64(int64_t v) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROW_MASK, 0xF, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROW_MASK, 0xF, false);
-  return (int64_t)((uint64_t)hi << 32 | lo);
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xF, false);
 }
-__device__ __forceinline__ int64_t wave_scan(int64_t v) {
-  v += dpp_i64<0x111, 0xF>(v);
-  v += dpp_i64<0x112, 0xF>(v);
-  v += dpp_i64<0x114, 0xF>(v);
-  v += dpp_i64<0x118, 0xF>(v);
-  v += dpp_i64<0x142, 0xA>(v);
-  v += dpp_i64<0x143, 0xC>(v);
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = add_sat(v, dpp_u32<0x111, 0xF>(v));
+  v = add_sat(v, dpp_u32<0x112, 0xF>(v));
+  v = add_sat(v, dpp_u32<0x114, 0xF>(v));
+  v = add_sat(v, dpp_u32<0x118, 0xF>(v));
+  v = add_sat(v, dpp_u32<0x142, 0xA>(v));
+  v = add_sat(v, dpp_u32<0x143, 0xC>(v));
   return v;
 }
 
-// Exclusive prefix sum of one value per thread over the workgroup, and the
-// total.  s: 16 words that no one else uses until the next call's first barrier.
-__device__ __forceinline__ int64_t scan_excl(int64_t v, int64_t* s, int64_t& total) {
+// Exclusive prefix sums of N values per thread over the workgroup, and the
+// totals.  s: N * 16 words that no one else uses until the next call's first
+// barrier.
+template <int N>
+__device__ __forceinline__ void scan_excl(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t* s) {
   const int lane = lane_id(), wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int64_t x = wave_scan(v);
   __syncthreads();
-  if (lane == 63) s[wave] = x;
-  __syncthreads();
-  int64_t before = 0, all = 0;
-  for (int w = 0; w < waves; ++w) {
-    const int64_t t = s[w];
-    if (w < wave) before += t;
-    all += t;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    v[k] = wave_scan(v[k]);
+    if (lane == 63) s[wave * N + k] = v[k];
+    v[k] = dpp_u32<0x138, 0xF>(v[k]);      // wave_shr:1, 0 in lane 0
+    total[k] = 0;
   }
-  total = all;
-  return before + x - v;
+  __syncthreads();
+#pragma unroll 1
+  for (int w = 0; w < waves; ++w)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const uint32_t t = s[w * N + k];
+      if (w < wave) v[k] = add_sat(v[k], t);
+      total[k] = add_sat(total[k], t);
+    }
 }
 
 // The last row r with sum[r] <= i, of n rows with ascending exclusive sums:
@@ -86,21 +102,26 @@ __device__ __forceinline__ int page_id(const ExtendArgs& a, int id) {
 }
 
 // Page p of row r: a new one is still on the stack, whose top n_free is the
-// step's first; the others are in the table.
+// step's first; the others are in the table.  One load, by a chosen address: in
+// a short step the fetches of the code cost as much as the rest.
 __device__ __forceinline__ int row_page(const ExtendArgs& a, int r, int p, int past, int need, int n_free) {
   const int fresh = p - pages_of(past);
-  return page_id(a, fresh >= 0 ? a.stack[max(n_free - 1 - need - fresh, 0)] : a.table[(int64_t)r * a.width + p]);
+  const int32_t* at = fresh >= 0 ? a.stack + max(n_free - 1 - need - fresh, 0) : a.table + (int64_t)r * a.width + p;
+  return page_id(a, *at);
 }
 
-// Packed pairs of sums, high and low 32 bits, neither past 2^31.
-__device__ __forceinline__ int64_t pair(int64_t hi, int64_t lo) { return hi << 32 | lo; }
-
+// LONG: rows may be long enough for the attention's kernel for many rows.
+template <bool LONG>
 __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
   extern __shared__ int32_t lds[];
-  __shared__ int64_t s_scan[16];
-  __shared__ int s_taken;            // pages that rows take
+  __shared__ uint32_t s_scan[4 * 16];
+  __shared__ unsigned long long s_work[2];   // pages that tiles of few and of many rows see
+  __shared__ int s_taken;                    // pages that rows take
   const int n = a.n_seqs, nt = blockDim.x, tid = threadIdx.x;
-  if (tid == 0) s_taken = 0;
+  if (tid == 0) {
+    s_taken = 0;
+    s_work[0] = s_work[1] = 0;
+  }
   int32_t* s_tok = lds;              // exclusive sums over the rows: tokens (capped at max_tokens + 1),
   int32_t* s_need = s_tok + n;       // pages needed,
   int32_t* s_touch = s_need + n;     // pages touched,
@@ -108,149 +129,163 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
   int32_t* s_past = s_tile + n;
   int32_t* s_kv = s_past + n;
   int32_t* s_new = s_kv + n;         // tokens inside the buffer
-  const int per = (n + nt - 1) / nt, r0 = min(tid * per, n), r1 = min(r0 + per, n);
+  const int per = (n + nt - 1) >> (31 - __builtin_clz(nt));   // nt is a power of two
+  const int r0 = min(tid * per, n), r1 = min(r0 + per, n);
   const int n_free = min(max(a.n_free[0], 0), a.n_pages);
+  auto few_rows = [&](int tokens) { return !LONG || tokens <= kFewRows >> a.log2_group; };
 
   // tokens
-  int64_t mine = 0, total;
+  uint32_t at[1] = {0}, total[1];
+#pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const int t = max(a.new_lens[r], 0);
     s_past[r] = min(max(a.lens[r], 0), a.max_len);
     s_new[r] = t;
-    mine += t;
+    at[0] = add_sat(at[0], t);
   }
-  int64_t at = scan_excl(mine, s_scan, total);
-  if (tid == 0) a.cu[n] = (int)min(total, (int64_t)0x7FFFFFFF);
-  const int n_tokens = (int)min(total, (int64_t)a.max_tokens);
+  scan_excl<1>(at, total, s_scan);
+  if (tid == 0) a.cu[n] = (int)total[0];
+  const int n_tokens = min((int)total[0], a.max_tokens);
   // pages
-  int64_t need = 0;
+  uint32_t need[1] = {0}, all_need[1];
+#pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const int t = s_new[r];
-    a.cu[r] = (int)min(at, (int64_t)0x7FFFFFFF);
-    s_tok[r] = (int)min(at, (int64_t)a.max_tokens + 1);
-    at += t;
-    const int64_t len = (int64_t)s_past[r] + t;
-    const bool fits = len <= a.max_len && t <= a.max_new && at <= a.max_tokens;
+    a.cu[r] = (int)at[0];
+    s_tok[r] = (int)min(at[0], (uint32_t)a.max_tokens + 1);
+    at[0] = add_sat(at[0], t);
+    const uint32_t len = add_sat(s_past[r], t);
+    const bool fits = len <= (uint32_t)a.max_len && t <= a.max_new && at[0] <= (uint32_t)a.max_tokens;
     const int pages = fits ? pages_of((int)len) - pages_of(s_past[r]) : 0;
     s_kv[r] = fits ? (int)len : -1;
     s_need[r] = pages;
-    need += pages;
+    need[0] = add_sat(need[0], pages);
   }
-  int64_t all_need;
-  int64_t before = scan_excl(need, s_scan, all_need);
-  int64_t touch = 0, tiles = 0, pages_few = 0, pages_many = 0;
+  scan_excl<1>(need, all_need, s_scan);
+  uint32_t lists[2] = {0, 0}, in_lists[2];      // pages touched, tiles
+#pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const int pages = s_need[r], past = s_past[r], t = s_new[r];
-    s_need[r] = (int)min(before, (int64_t)0x7FFFFFFF);
-    before += pages;
-    const bool taken = s_kv[r] >= 0 && (pages == 0 || before <= (int64_t)n_free);
+    s_need[r] = (int)need[0];
+    need[0] = add_sat(need[0], pages);
+    const bool taken = s_kv[r] >= 0 && (pages == 0 || need[0] <= (uint32_t)n_free);
     const int kv = taken ? s_kv[r] : 0;
     a.kv_len[r] = kv;
     a.rejected[r] = taken ? 0 : 1;
     if (taken) a.lens[r] = kv;
     // the rows that the pool serves are the first ones that need pages
-    if (taken && pages > 0) atomicMax(&s_taken, (int)before);
+    if (taken && pages > 0) atomicMax(&s_taken, (int)need[0]);
     s_kv[r] = kv;
     const int in = max(0, min(t, a.max_tokens - s_tok[r]));
     s_new[r] = in;
     const int touched = taken && t > 0 ? pages_of(kv) - past / kPage : 0;
-    const bool few = a.few_only || (int64_t)in * a.group <= kFewRows;
-    const int tok = few ? a.l.few_tokens : a.l.many_tokens;
-    const int tl = (in + tok - 1) / tok;
-    const int64_t work = (int64_t)tl * pages_of(kv);
-    pages_few += few ? work : 0;
-    pages_many += few ? 0 : work;
+    const bool few = few_rows(in);
+    const int shift = (few ? kLogFew : kLogMany) - a.log2_group, tl = (in + (1 << shift) - 1) >> shift;
+    const uint64_t work = (uint64_t)tl * pages_of(kv);
+    if (work) atomicAdd(&s_work[LONG && !few], (unsigned long long)work);
     s_touch[r] = touched;
     s_tile[r] = tl;
-    touch += touched;
-    tiles += tl;
+    lists[0] += touched;
+    lists[1] += tl;
   }
-  int64_t both, all_few, all_many;
-  int64_t b = scan_excl(pair(touch, tiles), s_scan, both);
-  scan_excl(pages_few, s_scan, all_few);
-  scan_excl(pages_many, s_scan, all_many);
-  int bt = (int)(b >> 32), bl = (int)(b & 0xFFFFFFFF);
+  scan_excl<2>(lists, in_lists, s_scan);
+#pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const int t = s_touch[r], l = s_tile[r];
-    s_touch[r] = bt;
-    s_tile[r] = bl;
-    bt += t;
-    bl += l;
+    s_touch[r] = (int)lists[0];
+    s_tile[r] = (int)lists[1];
+    lists[0] += t;
+    lists[1] += l;
   }
-  const int n_touch = (int)(both >> 32), n_tile = (int)(both & 0xFFFFFFFF);
-  // pages of a part: an equal share of all of them, in whole rounds of a
-  // workgroup's four waves
-  auto share = [](int64_t all, int parts) {
-    return (int)min(max(((all + parts - 1) / parts + 3) / 4 * 4, (int64_t)4), (int64_t)1 << 26);
-  };
-  const int c_few = share(all_few, a.l.parts_few), c_many = share(all_many, a.l.parts_many);
+  const int n_touch = min((int)in_lists[0], a.l.cap_append), n_tile = (int)in_lists[1];
   __syncthreads();
 
-  const int taken = s_taken;
-  for (int i = tid; i < taken; i += nt) {
-    const int r = row_of(s_need, n, i), j = i - s_need[r];
-    a.table[(int64_t)r * a.width + pages_of(s_past[r]) + j] = page_id(a, a.stack[n_free - 1 - i]);
+  // Attention tiles, cut into parts.  Pages of a part: an equal share of all of
+  // them, rounded up (the product's error is far below 1 / parts), in whole
+  // rounds of a workgroup's four waves.
+  auto share = [&](int many) {
+    return ((int)min(max(ceil((double)s_work[many] * (many ? a.per_part_many : a.per_part_few)), 1.0), 0x1p26) + 3) / 4 * 4;
+  };
+  const int c_few = share(0), c_many = LONG ? share(1) : 0;
+  constexpr int kSums = LONG ? 4 : 2;        // items and partial sums, of few and of many rows
+  uint32_t base[kSums] = {};
+#pragma unroll 1
+  for (int i0 = 0; i0 < n_tile; i0 += nt) {
+    const int i = i0 + tid;
+    bool few = true;
+    int parts = 0, tok0 = 0, count = 0, r = 0, pages = 0, first = 0;
+    if (i < n_tile) {
+      r = row_of(s_tile, n, i);
+      few = few_rows(s_new[r]);
+      const int shift = (few ? kLogFew : kLogMany) - a.log2_group;
+      const int tl = (s_new[r] + (1 << shift) - 1) >> shift;
+      first = (tl - 1 - (i - s_tile[r])) << shift;        // the tiles that see most first
+      count = min(1 << shift, s_new[r] - first);
+      tok0 = s_tok[r] + first;
+      pages = s_kv[r] ? pages_of(min(s_past[r] + first + count, s_kv[r])) : 0;
+      const int c = few ? c_few : c_many;
+      parts = pages <= (few ? kFewWhole : kManyWhole) ? 1 : (int)((uint32_t)(pages + c - 1) / (uint32_t)c);
+    }
+    const uint32_t slots = parts > 1 ? parts : 0;
+    uint32_t x[kSums] = {few ? (uint32_t)parts : 0, few ? slots : 0}, in_all[kSums];
+    if constexpr (LONG) {
+      x[2] = few ? 0 : parts;
+      x[3] = few ? 0 : slots;
+    }
+    scan_excl<kSums>(x, in_all, s_scan);
+    if (i < n_tile) {
+      uint32_t item = base[0] + x[0], slot = base[1] + x[1];
+      AttendItem* list = reinterpret_cast<AttendItem*>(a.work + a.l.few);
+      if constexpr (LONG)
+        if (!few) {
+          item = base[2] + x[2];
+          slot = base[3] + x[3];
+          list = reinterpret_cast<AttendItem*>(a.work + a.l.many);
+        }
+      // at most c: as many parts, alike
+      const int each = parts > 1 ? (int)(((uint32_t)(pages + parts - 1) / (uint32_t)parts + 3) / 4 * 4) : pages;
+#pragma unroll 1
+      for (int k = 0; k < parts; ++k) {
+        AttendItem y{{r, tok0, count, s_past[r] + first, min(k * each, pages), min((k + 1) * each, pages),
+                      s_kv[r], k, parts, (int)slot, {0, 0}}, {}};
+        // pages past the part's are loaded like its last one
+#pragma unroll
+        for (int e = 0; e < kFewWaves; ++e)
+          y.ids[e] = row_page(a, r, max(min(y.page0 + e, y.page1 - 1), 0), s_past[r], s_need[r], n_free);
+        list[item + k] = y;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) base[k] += in_all[k];
   }
   if (tid == 0) {
     a.work[kNAppend] = n_touch;
-    a.n_free[0] = n_free - taken;
+    a.work[kNFew] = (int)base[0];
+    a.work[kNMany] = LONG ? (int)base[kSums - 2] : 0;
+    a.n_free[0] = n_free - s_taken;
+  }
+
+  // The other lists start at another wave each, so that in a short step their
+  // loads are under way together.
+  auto turned = [&](int k) { return (tid - 64 * k) & (nt - 1); };
+  const int taken = s_taken;
+#pragma unroll 1
+  for (int i = turned(1); i < taken; i += nt) {
+    const int r = row_of(s_need, n, i), j = i - s_need[r];
+    a.table[(int64_t)r * a.width + pages_of(s_past[r]) + j] = page_id(a, a.stack[n_free - 1 - i]);
   }
 
   AppendItem* ap = reinterpret_cast<AppendItem*>(a.work + a.l.append);
-  for (int i = tid; i < n_touch; i += nt) {
+#pragma unroll 1
+  for (int i = turned(2); i < n_touch; i += nt) {
     const int r = row_of(s_touch, n, i), past = s_past[r], p = past / kPage + i - s_touch[r];
     const int held = max(past - p * kPage, 0), upto = min(s_kv[r] - p * kPage, kPage);
     ap[i] = AppendItem{row_page(a, r, p, past, s_need[r], n_free), s_tok[r] + p * kPage + held - past, held, upto};
   }
 
-  // attention tiles, cut into parts
-  AttendItem* few_list = reinterpret_cast<AttendItem*>(a.work + a.l.few);
-  AttendItem* many_list = reinterpret_cast<AttendItem*>(a.work + a.l.many);
-  int64_t base_items = 0, base_slots = 0;
-  for (int i0 = 0; i0 < n_tile; i0 += nt) {
-    const int i = i0 + tid;
-    bool few = false;
-    int parts = 0, tok0 = 0, count = 0, r = 0, pages = 0, first = 0;
-    if (i < n_tile) {
-      r = row_of(s_tile, n, i);
-      few = a.few_only || (int64_t)s_new[r] * a.group <= kFewRows;
-      const int tok = few ? a.l.few_tokens : a.l.many_tokens;
-      const int tl = (s_new[r] + tok - 1) / tok;
-      const int j = tl - 1 - (i - s_tile[r]);        // the tiles that see most first
-      first = j * tok;
-      count = min(tok, s_new[r] - first);
-      tok0 = s_tok[r] + first;
-      pages = s_kv[r] ? pages_of(min(s_past[r] + first + count, s_kv[r])) : 0;
-      const int c = few ? c_few : c_many;
-      parts = pages <= (few ? kFewWhole : kManyWhole) ? 1 : (pages + c - 1) / c;
-    }
-    const int slots = parts > 1 ? parts : 0;
-    int64_t t_items, t_slots;
-    const int64_t x_items = scan_excl(few ? pair(0, parts) : pair(parts, 0), s_scan, t_items) + base_items;
-    const int64_t x_slots = scan_excl(few ? pair(0, slots) : pair(slots, 0), s_scan, t_slots) + base_slots;
-    base_items += t_items;
-    base_slots += t_slots;
-    if (i < n_tile) {
-      const int item = (int)(few ? x_items & 0xFFFFFFFF : x_items >> 32);
-      const int slot = (int)(few ? x_slots & 0xFFFFFFFF : x_slots >> 32);
-      AttendItem* list = few ? few_list : many_list;
-      const int each = parts > 1 ? ((pages + parts - 1) / parts + 3) / 4 * 4 : pages;   // at most c: as many parts, alike
-      for (int k = 0; k < parts; ++k) {
-        AttendItem x{{r, tok0, count, s_past[r] + first, min(k * each, pages), min((k + 1) * each, pages),
-                      s_kv[r], k, parts, slot, {0, 0}}, {}};
-#pragma unroll
-        for (int e = 0; e < kFewWaves; ++e)
-          if (few || e < 2) x.ids[e] = x.page0 + e < x.page1 ? row_page(a, r, x.page0 + e, s_past[r], s_need[r], n_free) : 0;
-        list[item + k] = x;
-      }
-    }
-  }
-  if (tid == 0) {
-    a.work[kNFew] = (int)(base_items & 0xFFFFFFFF);
-    a.work[kNMany] = (int)(base_items >> 32);
-  }
   if (a.fill)
-    for (int t = tid; t < a.max_tokens; t += nt) {
+#pragma unroll 1
+    for (int t = turned(3); t < a.max_tokens; t += nt) {
       int pos = -1, slot = -1;
       if (t < n_tokens) {
         const int r = row_of(s_tok, n, t);
@@ -294,27 +329,27 @@ struct RewindArgs {
 
 __global__ __launch_bounds__(1024) void k_page_rewind(RewindArgs a) {
   extern __shared__ int32_t lds[];
-  __shared__ int64_t s_scan[16];
+  __shared__ uint32_t s_scan[16];
   const int n = a.n_seqs, nt = blockDim.x, tid = threadIdx.x;
   int32_t* s_sum = lds;
   int32_t* s_keep = lds + n;
-  const int per = (n + nt - 1) / nt, r0 = min(tid * per, n), r1 = min(r0 + per, n);
+  const int per = (n + nt - 1) >> (31 - __builtin_clz(nt)), r0 = min(tid * per, n), r1 = min(r0 + per, n);
   const int n_free = min(max(a.n_free[0], 0), a.n_pages);
-  int64_t mine = 0, all;
+  uint32_t mine[1] = {0}, all[1];
   for (int r = r0; r < r1; ++r) {
     const int len = min(max(a.lens[r], 0), a.max_len), to = a.to[r], keep = to < 0 || to > len ? len : to;
     if (keep != len) a.lens[r] = keep;
     s_keep[r] = pages_of(keep);
     s_sum[r] = pages_of(len) - pages_of(keep);
-    mine += s_sum[r];
+    mine[0] = add_sat(mine[0], s_sum[r]);
   }
-  int64_t at = scan_excl(mine, s_scan, all);
+  scan_excl<1>(mine, all, s_scan);
   for (int r = r0; r < r1; ++r) {
     const int f = s_sum[r];
-    s_sum[r] = (int)at;
-    at += f;
+    s_sum[r] = (int)mine[0];
+    mine[0] = add_sat(mine[0], f);
   }
-  const int freed = (int)min(all, (int64_t)(a.n_pages - n_free));   // more than the pool has room for: damaged
+  const int freed = (int)min(all[0], (uint32_t)(a.n_pages - n_free));   // more than the pool has room for: damaged
   __syncthreads();
   for (int i = tid; i < freed; i += nt) {
     const int r = row_of(s_sum, n, i);
@@ -333,8 +368,7 @@ ExtendArgs extend_args(const oi2_paged* c, const oi2_page_plan* p, const int32_t
   a.n_pages = c->n_pages;
   a.max_tokens = p->max_tokens;
   a.max_new = p->max_new;
-  a.group = c->n_q / c->n_kv;
-  a.few_only = (int64_t)p->max_new * a.group <= kFewRows;
+  a.log2_group = __builtin_ctz((unsigned)(c->n_q / c->n_kv));
   a.fill = p->max_tokens <= kOneLaunchTokens;
   a.new_lens = new_lens;
   a.table = c->block_table;
@@ -348,6 +382,8 @@ ExtendArgs extend_args(const oi2_paged* c, const oi2_page_plan* p, const int32_t
   a.rejected = p->rejected;
   a.work = p->work;
   a.l = plan_layout(*c, p->max_tokens, p->max_new);
+  a.per_part_few = 1.0 / a.l.parts_few;
+  a.per_part_many = 1.0 / a.l.parts_many;
   return a;
 }
 
@@ -403,8 +439,9 @@ int oi2_page_extend(const oi2_paged* c, const oi2_page_plan* p, const int32_t* n
   const ExtendArgs a = extend_args(c, p, new_lens);
   hipStream_t st = (hipStream_t)stream;
   // short steps: fewer waves have less to wait for at each barrier
-  const int threads = a.n_seqs <= 64 && p->max_tokens <= 128 ? 64 : a.n_seqs <= 256 && p->max_tokens <= 1024 ? 256 : 1024;
-  hipLaunchKernelGGL(k_page_extend, dim3(1), dim3(threads), (size_t)a.n_seqs * 7 * 4, st, a);
+  const int threads = a.n_seqs <= 256 && p->max_tokens <= 1024 ? 256 : 1024;
+  const bool few_only = (int64_t)p->max_new << a.log2_group <= kFewRows;
+  hipLaunchKernelGGL(few_only ? k_page_extend<false> : k_page_extend<true>, dim3(1), dim3(threads), (size_t)a.n_seqs * 7 * 4, st, a);
   OI2_CHECK_LAUNCH();
   if (!a.fill) {
     hipLaunchKernelGGL(k_page_tokens, dim3((a.max_tokens + 255) / 256), dim3(256), (size_t)a.n_seqs * 4, st, a);
