@@ -208,12 +208,14 @@ def ptr(t) -> int | None:
     return t.data_ptr()
 
 
+_DTYPE_CODES = {torch.float16: DTYPE_F16, torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+
+
 def dtype_code(dtype) -> int:
     """The ABI's dtype code of a torch floating dtype (fp16, fp32, bf16)."""
-    codes = {torch.float16: DTYPE_F16, torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
-    if dtype not in codes:
+    if dtype not in _DTYPE_CODES:
         raise TypeError(f"dtype {dtype} is not float16, float32 or bfloat16")
-    return codes[dtype]
+    return _DTYPE_CODES[dtype]
 
 
 def stream_handle(device=None) -> int | None:
@@ -243,18 +245,22 @@ def gpu(device) -> torch.device:
 
 
 class on_device:
-    """``with on_device(d)``: d is the current device, which the kernels are
-    launched on.  Costs a comparison where it is already."""
+    """``with on_device(d) as stream``: d is the current device, which the
+    kernels are launched on, and ``stream`` its current stream as the C ABI
+    takes it.  For devices that hold tensors of the caller's; costs a comparison
+    where d is current already."""
     __slots__ = ("index", "before")
 
     def __init__(self, device: torch.device):
         self.index = device.index
 
     def __enter__(self):
-        torch.cuda.init()
+        if not torch.cuda.is_initialized():
+            torch.cuda.init()                 # raises in a forked child
         self.before = torch._C._cuda_getDevice()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index) or None
 
     def __exit__(self, *exc):
         if self.before != self.index:

@@ -204,14 +204,14 @@ class GroupedQueryAttention(torch.nn.Module):
                                          or residual_out.device != x.device or not residual_out.is_contiguous()):
             raise ValueError("residual_out must be a contiguous fp16 tensor shaped like x")
         xc = x.contiguous()
-        L = _lib.lib()
-        with _lib.on_device(cache.device):
+        L = _lib.load_library()
+        with _lib.on_device(cache.device) as stream:
             out = torch.empty_like(xc)
-            nbytes = L.oi2_attn_paged_workspace_bytes(ctypes.byref(cache._struct), plan.max_tokens, plan.max_new,
+            nbytes = L.oi2_attn_paged_workspace_bytes(cache._ref, plan.max_tokens, plan.max_new,
                                                       max(n, 1))
             ws = x.new_empty((nbytes,), dtype=torch.uint8)
             _lib.check(L.oi2_attn_forward_paged(
-                xc.data_ptr(), n, ctypes.byref(self._struct), self.eps, ctypes.byref(rotary._struct),
-                ctypes.byref(cache._struct), ctypes.byref(plan._struct), layer, out.data_ptr(),
-                _lib.ptr(residual_out), ws.data_ptr(), nbytes, _lib.stream_handle(cache.device)))
+                xc.data_ptr(), n, ctypes.byref(self._struct), self.eps, rotary._ref,
+                cache._ref, plan._ref, layer, out.data_ptr(),
+                _lib.ptr(residual_out), ws.data_ptr(), nbytes, stream))
         return out

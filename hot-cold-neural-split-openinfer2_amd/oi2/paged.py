@@ -48,7 +48,7 @@ class PagePlan:
         self.max_new = self.max_tokens if max_new is None else int(max_new)
         if self.max_tokens < 1 or self.max_new < 1:
             raise ValueError(f"a plan of {max_tokens} tokens, {max_new} a row: one at least")
-        nbytes = _lib.load_library().oi2_page_plan_bytes(ctypes.byref(cache._struct), self.max_tokens, self.max_new)
+        nbytes = _lib.load_library().oi2_page_plan_bytes(cache._ref, self.max_tokens, self.max_new)
         if not nbytes:
             raise ValueError(f"a plan of {max_tokens} tokens is too large")
 
@@ -65,8 +65,9 @@ class PagePlan:
         self._struct = _lib.PagePlan(self.max_tokens, self.max_new, self.cu.data_ptr(), self.positions.data_ptr(),
                                      self.slots.data_ptr(), self.kv_len.data_ptr(), self.rejected.data_ptr(),
                                      self.work.data_ptr())
+        self._ref = ctypes.byref(self._struct)
         self._attend_bytes = _lib.load_library().oi2_kv_attend_workspace_bytes(
-            ctypes.byref(cache._struct), self.max_tokens, self.max_new)
+            cache._ref, self.max_tokens, self.max_new)
 
 
 class PagedKVCache:
@@ -113,6 +114,7 @@ class PagedKVCache:
                                   self.block_table.data_ptr(), self.lens.data_ptr(), self.free.data_ptr(),
                                   self.n_free.data_ptr(), self.pages.data_ptr() or None,
                                   self._scales.data_ptr() or None)
+        self._ref = ctypes.byref(self._struct)
 
     # -- tables ---------------------------------------------------------------
     def new_plan(self, max_tokens: int, max_new: int | None = None) -> PagePlan:
@@ -140,10 +142,9 @@ class PagedKVCache:
         anything that converts to that.  Rejected rows are not an error here:
         ``plan.rejected`` tells, at the price of waiting for it."""
         plan, new_lens = self._plan(plan), self._lens(new_lens)
-        L = _lib.lib()
-        with _lib.on_device(self.device):
-            _lib.check(L.oi2_page_extend(ctypes.byref(self._struct), ctypes.byref(plan._struct), new_lens.data_ptr(),
-                                         _lib.stream_handle(self.device)))
+        L = _lib.load_library()
+        with _lib.on_device(self.device) as stream:
+            _lib.check(L.oi2_page_extend(self._ref, plan._ref, new_lens.data_ptr(), stream))
         return plan
 
     def rewind(self, lens) -> None:
@@ -151,19 +152,20 @@ class PagedKVCache:
         pages past them are free again; 0 ends the sequence, a negative value
         leaves the row.  The former plan's step is not to be used after it."""
         lens = self._lens(lens)
-        L = _lib.lib()
-        with _lib.on_device(self.device):
-            _lib.check(L.oi2_page_rewind(ctypes.byref(self._struct), lens.data_ptr(), _lib.stream_handle(self.device)))
+        L = _lib.load_library()
+        with _lib.on_device(self.device) as stream:
+            _lib.check(L.oi2_page_rewind(self._ref, lens.data_ptr(), stream))
 
     # -- pages ----------------------------------------------------------------
     def _rows(self, x: torch.Tensor, heads: int, what: str, like: torch.Tensor | None = None) -> torch.Tensor:
-        if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != HEAD_DIM:
-            raise ValueError(f"{what}: (tokens, {heads}, {HEAD_DIM}), got {tuple(x.shape)}")
+        shape = x.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != HEAD_DIM:
+            raise ValueError(f"{what}: (tokens, {heads}, {HEAD_DIM}), got {tuple(shape)}")
         if x.dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"{what}: float16 or bfloat16, got {x.dtype}")
         if x.device != self.device:
             raise ValueError(f"{what} on {x.device}, the cache on {self.device}")
-        if like is not None and (x.shape[0] != like.shape[0] or x.dtype != like.dtype):
+        if like is not None and (shape[0] != like.shape[0] or x.dtype != like.dtype):
             raise ValueError(f"{what} {tuple(x.shape)} {x.dtype} beside {tuple(like.shape)} {like.dtype}")
         return x if x.stride(2) == 1 else x.contiguous()
 
@@ -173,9 +175,10 @@ class PagedKVCache:
         return int(layer)
 
     def _tokens(self, x: torch.Tensor, plan: PagePlan) -> int:
-        if x.shape[0] > plan.max_tokens:
-            raise ValueError(f"{x.shape[0]} tokens in a plan of {plan.max_tokens}")
-        return x.shape[0]
+        n = x.shape[0]
+        if n > plan.max_tokens:
+            raise ValueError(f"{n} tokens in a plan of {plan.max_tokens}")
+        return n
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: PagePlan, q: torch.Tensor | None = None,
                rotary: Rotary | None = None, q_out: torch.Tensor | None = None):
@@ -201,13 +204,13 @@ class PagedKVCache:
                 raise ValueError("an output that is its own input must be contiguous")
         elif q_out is not None:
             raise ValueError("q_out without q")
-        L = _lib.lib()
-        with _lib.on_device(self.device):
+        L = _lib.load_library()
+        with _lib.on_device(self.device) as stream:
             _lib.check(L.oi2_kv_append(
-                ctypes.byref(self._struct), ctypes.byref(plan._struct), layer, _lib.dtype_code(k.dtype), n,
+                self._ref, plan._ref, layer, _lib.dtype_code(k.dtype), n,
                 ctypes.byref(_lib.heads(k)), ctypes.byref(_lib.heads(v)),
-                None if rotary is None else ctypes.byref(rotary._struct),
-                None if q is None else ctypes.byref(_lib.heads(q)), _lib.ptr(q_out), _lib.stream_handle(self.device)))
+                None if rotary is None else rotary._ref,
+                None if q is None else ctypes.byref(_lib.heads(q)), _lib.ptr(q_out), stream))
         return q_out
 
     def attend(self, layer: int, q: torch.Tensor, plan: PagePlan, scale: float | None = None,
@@ -225,14 +228,14 @@ class PagedKVCache:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor like q")
-        L = _lib.lib()
+        L = _lib.load_library()
         nbytes = plan._attend_bytes
-        with _lib.on_device(self.device):
+        with _lib.on_device(self.device) as stream:
             ws = q.new_empty((nbytes,), dtype=torch.uint8)
             _lib.check(L.oi2_kv_attend(
-                ctypes.byref(self._struct), ctypes.byref(plan._struct), layer, _lib.dtype_code(q.dtype), n,
+                self._ref, plan._ref, layer, _lib.dtype_code(q.dtype), n,
                 ctypes.byref(_lib.heads(q)), HEAD_DIM ** -0.5 if scale is None else float(scale), out.data_ptr(),
-                ws.data_ptr(), nbytes, _lib.stream_handle(self.device)))
+                ws.data_ptr(), nbytes, stream))
         return out
 
     # -- views ----------------------------------------------------------------

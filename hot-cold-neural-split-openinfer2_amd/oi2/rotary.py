@@ -109,10 +109,12 @@ class Rotary:
                                  device=self.device)
         self._struct = _lib.Rotary(self.head_dim, self.rotary_dim, int(layout == "interleaved"), self.magnitude,
                                    self.freq.data_ptr())
+        self._ref = ctypes.byref(self._struct)
 
     def _rows(self, x: torch.Tensor, what: str) -> torch.Tensor:
-        if x.dim() != 3 or x.shape[2] != self.head_dim:
-            raise ValueError(f"{what}: (tokens, heads, {self.head_dim}), got {tuple(x.shape)}")
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim:
+            raise ValueError(f"{what}: (tokens, heads, {self.head_dim}), got {tuple(shape)}")
         if x.dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"{what}: float16 or bfloat16, got {x.dtype}")
         if x.device != self.device:
@@ -145,11 +147,11 @@ class Rotary:
         for x, o in ((q, qo), (k, ko)):
             if x is not None and o.data_ptr() == x.data_ptr() and not x.is_contiguous():
                 raise ValueError("an output that is its own input must be contiguous")
-        L = _lib.lib()
-        with _lib.on_device(self.device):
+        L = _lib.load_library()
+        with _lib.on_device(self.device) as stream:
             _lib.check(L.oi2_rotary_apply(
-                ctypes.byref(self._struct), _lib.dtype_code(q.dtype), N, positions.contiguous().data_ptr(),
+                self._ref, _lib.dtype_code(q.dtype), N, positions.contiguous().data_ptr(),
                 ctypes.byref(_lib.heads(q)), qo.data_ptr(),
                 ctypes.byref(_lib.Heads() if k is None else _lib.heads(k)), _lib.ptr(ko),
-                _lib.stream_handle(self.device)))
+                stream))
         return qo, ko
