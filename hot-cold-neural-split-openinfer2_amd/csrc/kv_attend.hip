@@ -563,10 +563,12 @@ constexpr int kManyLds = 4 * kHalfLds + kHeadD * 4;
 template <bool BF16>
 __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t* s_page) {
   int* s_nan = reinterpret_cast<int*>(s_page + 4 * kHalfLds);
-  const int item = b / a.n_kv, g = b - item * a.n_kv;
+  // the last tiles, which see most, first
+  const int back = b / a.n_kv, g = b - back * a.n_kv;
+  const int item = min(scalar_load(a.work + kNMany), a.many.groups / a.n_kv) - 1 - back;
+  if (item < 0) return;
   const AttendItem& full = a.many.items[item];
   const ItemHead it = scalar_load(static_cast<const ItemHead*>(&full));
-  if (item >= scalar_load(a.work + kNMany)) return;
   const int n_tok = min(it.n_tokens, a.n_tokens - it.token0);
   if (n_tok <= 0 || item - it.part + it.n_parts > a.many.groups / a.n_kv) return;
   const int tid = threadIdx.x, lane = lane_id(), r = lane & 31, h = lane >> 5;

@@ -200,7 +200,8 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
   const int n_touch = min((int)in_lists[0], a.l.cap_append), n_tile = (int)in_lists[1];
   __syncthreads();
 
-  // Attention tiles, cut into parts.  Pages of a part: an equal share of all of
+  // Attention tiles in the order of their tokens, so that those of a call with
+  // fewer tokens come first, cut into parts.  Pages of a part: an equal share of all of
   // them, rounded up (the product's error is far below 1 / parts), in whole
   // rounds of a workgroup's four waves.
   auto share = [&](int many) {
@@ -218,8 +219,7 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
       r = row_of(s_tile, n, i);
       few = few_rows(s_new[r]);
       const int shift = (few ? kLogFew : kLogMany) - a.log2_group;
-      const int tl = (s_new[r] + (1 << shift) - 1) >> shift;
-      first = (tl - 1 - (i - s_tile[r])) << shift;        // the tiles that see most first
+      first = (i - s_tile[r]) << shift;
       count = min(1 << shift, s_new[r] - first);
       tok0 = s_tok[r] + first;
       pages = s_kv[r] ? pages_of(min(s_past[r] + first + count, s_kv[r])) : 0;

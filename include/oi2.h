@@ -560,8 +560,8 @@ size_t oi2_kv_attend_workspace_bytes(const oi2_paged* c, int32_t max_tokens, int
  * `dtype` (OI2_DTYPE_F16 or _BF16).  Scores, the softmax's sums and the output
  * are fp32 until the one rounding of out; probabilities enter the products as
  * two fp16 parts where out is fp16, and rounded to one where it is bf16.  The
- * tokens of a rejected row give zeros; rows of out past
- * the step's last token are left as they were. */
+ * tokens of a rejected row give zeros; rows of out past the step's last token
+ * are left as they were.  n_tokens below the step's: its first tokens alone. */
 int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
                   const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes,
                   void* stream);

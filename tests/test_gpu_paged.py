@@ -499,3 +499,38 @@ def test_a_run_of_steps(dev):
     k, v = c.read(1, 2)
     rk, rv = o[1].held(2, o[1].lens[2])
     assert np.array_equal(_np(k), rk) and np.array_equal(_np(v), rv)
+
+
+@pytest.mark.parametrize("past,new,max_new", [([0], [700], None), ([5000, 20], [400, 300], None), ([0, 3000, 9, 800], [1, 1, 1, 1], None),
+                                              ([3, 2000, 0], [60, 3, 500], None), ([0, 40, 5], [3, 4, 2], 4)])
+def test_calls_with_fewer_tokens_than_the_step(dev, past, new, max_new):
+    """The first tokens alone, with and without the rest of their row: their
+    outputs, and nothing past them."""
+    print(f"[attend] first tokens of {past} {new}", flush=True)
+    c, o, plan, ref, q = _filled(dev, 32, 8, past, new, torch.float16, 8, max_new=max_new)
+    want, bound = o.attend(_np(q), ref, D ** -0.5)
+    total = sum(new)
+    for n in sorted({1, 2, total // 3, total // 2, total - 1, total} - {0}):
+        out = torch.full_like(q, 7.0)
+        c.attend(0, q[:n], plan, out=out[:n])
+        _check_attend(out[:n], want[:n], bound[:n], torch.float16)
+        assert (out[n:] == 7.0).all()
+
+
+def test_append_of_the_first_tokens_leaves_the_rest(dev):
+    """Places of tokens that the call does not have keep their codes; those it
+    has are coded as the oracle does with the step cut there."""
+    for past, new, n in (([10, 100], [100, 60], 90), ([10, 100], [100, 60], 130), ([63, 0, 5], [2, 1, 2], 3)):
+        print(f"[append] first {n} of {past} {new}", flush=True)
+        g = torch.Generator(device=dev).manual_seed(9)
+        rows = len(past)
+        c, o = _pair(8, rows, 300, 12, dev)
+        first, plan = c.new_plan(sum(past)), c.new_plan(sum(new), max_new=max(new))
+        for p, lens, m in ((first, past, sum(past)), (plan, new, n)):
+            ref = _extend(c, o, p, lens)
+            k, v = (_values(g, (m, 8, D), torch.float16, dev) for _ in range(2))
+            c.append(0, k, v, p)
+            cut = [max(0, min(b, m) - a) for a, b in zip(ref["cu"], ref["cu"][1:])]
+            ref["kv_len"] = [a + b for a, b in zip(ref["past"], cut)]
+            o.append(_np(k), _np(v), ref)
+        _check_codes(c, o)
