@@ -210,6 +210,43 @@ __device__ __forceinline__ float upper(uint32_t d) {
   return widen<BF16>((uint16_t)(d >> 16));
 }
 
+// Largest of two 16-bit values each; the magnitudes of fp16 and bf16 are in the
+// order of their bits.
+__device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <bool BF16>
+constexpr uint32_t kInfBits = BF16 ? 0x7F80u : 0x7C00u;
+
+// The largest magnitude of 16 values in pairs, of the finite ones alone with FINITE.
+template <bool BF16, bool FINITE>
+__device__ __forceinline__ uint32_t top_of(const uint32_t (&x)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    uint32_t d = x[e] & 0x7FFF7FFFu;
+    if (FINITE) {
+      if ((d & 0xFFFFu) >= kInfBits<BF16>) d &= 0xFFFF0000u;
+      if (d >> 16 >= kInfBits<BF16>) d &= 0xFFFFu;
+    }
+    m = max_u16(m, d);
+  }
+  return max(m & 0xFFFFu, m >> 16);
+}
+__device__ __forceinline__ uint32_t wave_top(uint32_t top) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = max_u16(top, (uint32_t)__shfl_xor((int)top, d));
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)top);
+}
+
+// The codes of two pairs, whose values over the scale are 448 at most.
+template <bool BF16>
+__device__ __forceinline__ uint32_t codes4(uint32_t lo, uint32_t hi, float inv) {
+  const int x = __builtin_amdgcn_cvt_pk_fp8_f32(lower<BF16>(lo) * inv, upper<BF16>(lo) * inv, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lower<BF16>(hi) * inv, upper<BF16>(hi) * inv, x, true);
+}
+
 // ── many tokens ──────────────────────────────────────────────────────────────
 
 // Vectors of the codes in LDS, in the cache's order but for a swizzle that
@@ -224,7 +261,7 @@ constexpr int kPageThreads = 512;
 template <bool BF16, bool WIDE>
 __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int g0, int g1) {
   __shared__ __align__(16) uint8_t s_kc[kHalfBlock], s_vc[kHalfBlock];
-  __shared__ uint32_t s_max[2][2][kPageThreads / 64], s_nan[2];
+  __shared__ uint32_t s_max[2][kPageThreads / 64], s_nan[2];
   const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, u = tid & 7;
   const AppendItem it = reinterpret_cast<const AppendItem*>(a.work + a.append_at)[item];
   if (item >= a.work[kNAppend] || (unsigned)it.page >= (unsigned)a.n_pages) return;   // the whole workgroup
@@ -282,29 +319,17 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int g
           }
     }
 
-    // the largest finite values
-    uint32_t mk = 0, mv = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      mk = max(mk, max(finite_bits(lower<BF16>(kx[e])), finite_bits(upper<BF16>(kx[e]))));
-      mv = max(mv, max(finite_bits(lower<BF16>(vx[e])), finite_bits(upper<BF16>(vx[e]))));
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      mk = max(mk, (uint32_t)__shfl_xor((int)mk, d));
-      mv = max(mv, (uint32_t)__shfl_xor((int)mv, d));
-    }
-    if (lane == 0) {
-      s_max[par][0][wave] = mk;
-      s_max[par][1][wave] = mv;
-    }
+    // the largest finite values, k's in the low half
+    uint32_t top = top_of<BF16, false>(kx) | top_of<BF16, false>(vx) << 16;
+    top = wave_top(top);
+    const bool odd = (top & 0xFFFFu) >= kInfBits<BF16> || top >> 16 >= kInfBits<BF16>;   // the wave's
+    if (odd) top = wave_top(top_of<BF16, true>(kx) | top_of<BF16, true>(vx) << 16);
+    if (lane == 0) s_max[par][wave] = top;
     if (tid == 0) s_nan[par] = 0;
     __syncthreads();                       // the last head's codes have left LDS too
 #pragma unroll
-    for (int w = 0; w < kPageThreads / 64; ++w) {
-      mk = max(mk, s_max[par][0][w]);
-      mv = max(mv, s_max[par][1][w]);
-    }
+    for (int w = 0; w < kPageThreads / 64; ++w) top = max_u16(top, s_max[par][w]);
+    const uint32_t mk = as_u32(lower<BF16>(top)), mv = as_u32(upper<BF16>(top));
     int ek = exponent_for(mk), ev = exponent_for(mv);
     const int ek0 = exponent_of(before.x), ev0 = exponent_of(before.y);
     if (held > 0) {
@@ -314,40 +339,50 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int g
 
     // codes, in the cache's order
     const float ik = two_to(-ek), iv = two_to(-ev);
+    const bool plain = !odd && ek < kExpMax && ev < kExpMax;   // nothing past the codes
     bool nan = false;
     if (mine) {
-      uint32_t c[8];                       // codes of a pair
+      uint32_t c[4], y[4];                 // codes of two pairs each
+      if (plain) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) c[e] = code(lower<BF16>(kx[e]) * ik) | code(upper<BF16>(kx[e]) * ik) << 8;
-      if constexpr (WIDE) {
-        if (halves) {
+        for (int e = 0; e < 4; ++e) {
+          c[e] = codes4<BF16>(kx[2 * e], kx[2 * e + 1], ik);
+          y[e] = codes4<BF16>(vx[2 * e], vx[2 * e + 1], iv);
+        }
+      } else {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {    // every pair's first codes, then its second
-            const int d = q ? run.b : run.a;
-            const uint32_t sel = q ? 0x0c0c0501u : 0x0c0c0400u;   // byte q of either
-            const uint32_t x0 = __builtin_amdgcn_perm(c[1], c[0], sel) | __builtin_amdgcn_perm(c[3], c[2], sel) << 16;
-            const uint32_t x1 = __builtin_amdgcn_perm(c[5], c[4], sel) | __builtin_amdgcn_perm(c[7], c[6], sel) << 16;
-            *reinterpret_cast<u32x2v*>(s_kc + k_img(k_vec(p, d / 16)) + d % 16) = u32x2v{x0, x1};
+        for (int e = 0; e < 4; ++e) {
+          c[e] = y[e] = 0;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t kd = kx[2 * e + h], vd = vx[2 * e + h];
+            const uint32_t v0 = code(lower<BF16>(vd) * iv), v1 = code(upper<BF16>(vd) * iv);
+            c[e] |= (code(lower<BF16>(kd) * ik) | code(upper<BF16>(kd) * ik) << 8) << 16 * h;
+            y[e] |= (v0 | v1 << 8) << 16 * h;
+            nan = nan || v0 == 0x7F || v1 == 0x7F;
           }
+        }
+      }
+      if constexpr (WIDE) {
+        if (halves) {                      // every pair's first codes, then its second
+          *reinterpret_cast<u32x2v*>(s_kc + k_img(k_vec(p, run.a / 16)) + run.a % 16) =
+              u32x2v{__builtin_amdgcn_perm(c[1], c[0], 0x06040200u), __builtin_amdgcn_perm(c[3], c[2], 0x06040200u)};
+          *reinterpret_cast<u32x2v*>(s_kc + k_img(k_vec(p, run.b / 16)) + run.b % 16) =
+              u32x2v{__builtin_amdgcn_perm(c[1], c[0], 0x07050301u), __builtin_amdgcn_perm(c[3], c[2], 0x07050301u)};
         } else {
-          *reinterpret_cast<u32x4*>(s_kc + k_img(k_vec(p, u))) =
-              u32x4{c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16};
+          *reinterpret_cast<u32x4*>(s_kc + k_img(k_vec(p, u))) = u32x4{c[0], c[1], c[2], c[3]};
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const PairDims d = a.rotate ? pair_dims(8 * u + e, r.rot, r.interleaved) : PairDims{16 * u + 2 * e, 16 * u + 2 * e + 1};
-          s_kc[k_img(k_vec(p, d.a / 16)) + d.a % 16] = (uint8_t)c[e];
-          s_kc[k_img(k_vec(p, d.b / 16)) + d.b % 16] = (uint8_t)(c[e] >> 8);
+          s_kc[k_img(k_vec(p, d.a / 16)) + d.a % 16] = (uint8_t)(c[e / 2] >> 16 * (e % 2));
+          s_kc[k_img(k_vec(p, d.b / 16)) + d.b % 16] = (uint8_t)(c[e / 2] >> 16 * (e % 2) + 8);
         }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t x = code(lower<BF16>(vx[e]) * iv), y = code(upper<BF16>(vx[e]) * iv);
-        nan = nan || x == 0x7F || y == 0x7F;
-        s_vc[v_img(v_vec(16 * u + 2 * e, p / 16)) + p % 16] = (uint8_t)x;
-        s_vc[v_img(v_vec(16 * u + 2 * e + 1, p / 16)) + p % 16] = (uint8_t)y;
-      }
+      for (int e = 0; e < 16; ++e)
+        s_vc[v_img(v_vec(16 * u + e, p / 16)) + p % 16] = (uint8_t)(y[e / 4] >> 8 * (e % 4));
     }
     if (nan) s_nan[par] = 1;
     __syncthreads();
