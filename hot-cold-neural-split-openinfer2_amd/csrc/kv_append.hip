@@ -271,16 +271,39 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int g
   const int p = tid >> 3;
   const bool mine = p >= held && p < upto;
   const int64_t t = it.token0 + p - held;
-  CosSin cs[8];
+  // cosines and sines of this thread's pairs, for every head; in LDS, but for
+  // the last pair's (two workgroups share a CU's 160 KB), they leave the
+  // registers to the next head's loads
+  __shared__ __align__(16) CosSin s_cs[7][kPageThreads];
+  CosSin last{};
   if (a.rotate && mine) {
     const int pos = r.positions[t];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (2 * (8 * u + e) < r.rot) cs[e] = turn_of(r, 8 * u + e, pos);
+      if (2 * (8 * u + e) < r.rot) (e < 7 ? s_cs[e][tid] : last) = turn_of(r, 8 * u + e, pos);
   }
   // WIDE: the first dims of this thread's pairs' two runs of eight
   const PairDims run = a.rotate && 16 * u < r.rot && !r.interleaved ? PairDims{8 * u, 8 * u + r.rot / 2} : PairDims{16 * u, 16 * u + 8};
   const bool halves = a.rotate && 16 * u < r.rot && !r.interleaved;   // else the runs are 16 neighbouring dims
+  uint32_t raw[16];                        // k's and v's of the next head
+  auto load = [&](int g) {
+    const uint16_t* pk = a.src[0] + t * a.token_stride[0] + g * a.head_stride[0];
+    const uint16_t* pv = a.src[1] + t * a.token_stride[1] + g * a.head_stride[1] + 16 * u;
+    if constexpr (WIDE) {
+      *reinterpret_cast<u32x4*>(raw) = *reinterpret_cast<const u32x4*>(pk + run.a);
+      *reinterpret_cast<u32x4*>(raw + 4) = *reinterpret_cast<const u32x4*>(pk + run.b);
+      *reinterpret_cast<u32x4*>(raw + 8) = *reinterpret_cast<const u32x4*>(pv);
+      *reinterpret_cast<u32x4*>(raw + 12) = *reinterpret_cast<const u32x4*>(pv + 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const PairDims d = a.rotate ? pair_dims(8 * u + e, r.rot, r.interleaved) : PairDims{16 * u + 2 * e, 16 * u + 2 * e + 1};
+        raw[e] = pk[d.a] | (uint32_t)pk[d.b] << 16;
+        raw[8 + e] = pv[2 * e] | (uint32_t)pv[2 * e + 1] << 16;
+      }
+    }
+  };
+  if (mine) load(g0);
   for (int g = g0; g < g1; ++g) {
     const int par = (g - g0) & 1;          // the reduction's words: the last head's may still be read
     const PageHead ph = page_head(a, it, g);
@@ -289,32 +312,18 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int g
 #pragma unroll
     for (int e = 0; e < 8; ++e) kx[e] = vx[e] = 0;
     if (mine) {
-      const uint16_t* pk = a.src[0] + t * a.token_stride[0] + g * a.head_stride[0];
-      const uint16_t* pv = a.src[1] + t * a.token_stride[1] + g * a.head_stride[1] + 16 * u;
-      if constexpr (WIDE) {
-        const u32x4 x0 = *reinterpret_cast<const u32x4*>(pk + run.a), x1 = *reinterpret_cast<const u32x4*>(pk + run.b);
-        const u32x4 v0 = *reinterpret_cast<const u32x4*>(pv), v1 = *reinterpret_cast<const u32x4*>(pv + 8);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t lo = x0[q], hi = x1[q];
-          kx[2 * q] = halves ? __builtin_amdgcn_perm(hi, lo, 0x05040100u) : q < 2 ? x0[2 * q] : x1[2 * q - 4];
-          kx[2 * q + 1] = halves ? __builtin_amdgcn_perm(hi, lo, 0x07060302u) : q < 2 ? x0[2 * q + 1] : x1[2 * q - 3];
-          vx[q] = v0[q];
-          vx[q + 4] = v1[q];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const PairDims d = a.rotate ? pair_dims(8 * u + e, r.rot, r.interleaved) : PairDims{16 * u + 2 * e, 16 * u + 2 * e + 1};
-          kx[e] = pk[d.a] | (uint32_t)pk[d.b] << 16;
-          vx[e] = pv[2 * e] | (uint32_t)pv[2 * e + 1] << 16;
-        }
+      for (int e = 0; e < 8; ++e) {
+        vx[e] = raw[8 + e];
+        if (WIDE && halves) kx[e] = __builtin_amdgcn_perm(raw[4 + e / 2], raw[e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+        else kx[e] = raw[e];
       }
+      if (g + 1 < g1) load(g + 1);
       if (a.rotate)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (2 * (8 * u + e) < r.rot) {
-            const f32x2 o = turned(lower<BF16>(kx[e]), upper<BF16>(kx[e]), cs[e]);
+            const f32x2 o = turned(lower<BF16>(kx[e]), upper<BF16>(kx[e]), e < 7 ? s_cs[e][tid] : last);
             kx[e] = narrow<BF16>(o.x) | (uint32_t)narrow<BF16>(o.y) << 16;
           }
     }
