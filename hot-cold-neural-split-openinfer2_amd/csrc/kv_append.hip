@@ -425,7 +425,7 @@ template <bool BF16, bool WIDE>
 __global__ __launch_bounds__(256) void k_kv_append_few(AppendArgs a) {
   const int b = blockIdx.x;
   if (b < a.page_groups) append_few<BF16>(a, 4 * b + (int)(threadIdx.x >> 6));
-  else rotate_heads<BF16, WIDE>(a.rope, (uint32_t)(b - a.page_groups) * 256 + threadIdx.x);
+  else rotate_tokens<BF16, WIDE, 256>(a.rope, b - a.page_groups);
 }
 
 template <bool BF16, bool WIDE, bool KWIDE>
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(kPageThreads, 4) void k_kv_append(AppendArgs a) {
     const int per = (a.n_kv + a.heads_each - 1) / a.heads_each, item = b / per, g = (b - item * per) * a.heads_each;
     append_page<BF16, KWIDE>(a, item, g, min(g + a.heads_each, a.n_kv));
   } else {
-    rotate_heads<BF16, WIDE>(a.rope, (uint32_t)(b - a.page_groups) * kPageThreads + threadIdx.x);
+    rotate_tokens<BF16, WIDE, kPageThreads>(a.rope, b - a.page_groups);
   }
 }
 
@@ -501,7 +501,7 @@ extern "C" int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t
   if (r) {
     rotary_describe(a.rope, r, n_tokens, p->positions);
     wide = rotary_fill(a.rope, q, q_out, nullptr, nullptr);
-    rows = few ? (rotary_threads(a.rope) + 255) / 256 : (rotary_threads(a.rope) + kPageThreads - 1) / kPageThreads;
+    rows = rotary_workgroups(a.rope);
   }
   OI2_CHECK_ARG(pages + rows < 1 << 23, "%d tokens are too many for one call", n_tokens);
   a.page_groups = (int)pages;

@@ -4,9 +4,7 @@
 // Cosines, sines and products are fp64; a result is rounded to fp32 and then to
 // its type.  The append codes rotated keys to 4 bits, where an fp32 sum moves
 // one value in 2^16 across the edge of a code, and the operator's forms agree
-// bit for bit without being compiled alike.  It costs no time: the operator is
-// bound by its bytes (12001 tokens of 32 + 8 heads, half of each head rotated:
-// 54.4 us, with fp32 sums 58.2).
+// bit for bit without being compiled alike.
 #pragma once
 #include "decode_util.h"
 #include "oi2.h"
@@ -80,70 +78,98 @@ struct RotaryArgs {
   uint16_t* dst[2];           // dense
   int64_t token_stride[2], head_stride[2];
   int heads[2];
-  uint32_t per_head;          // threads of a head
-  uint32_t groups;            // threads' groups of heads of a token
-  int heads_each;             // heads of a thread
+  int per_head;               // threads of a head
+  int tokens_each;            // tokens of a workgroup
 };
 
-// Thread i of the tokens' heads.  WIDE: eight pairs of a head, 16-byte loads
-// and stores: pairs 8 u .. of the rotated part, or 16 dims of the part behind
-// it.  Needs a rotary_dim and head_dim that 16 divides and rows at 16-byte
-// addresses; otherwise one pair, or two dims behind the rotated part.
-template <bool BF16, bool WIDE>
-__device__ __forceinline__ void rotate_heads(const RotaryArgs& a, uint32_t i) {
+// Cosines and sines of a workgroup's tokens: kTurns at most.
+constexpr int kTurns = 256;
+
+// The heads of tokens_each tokens by a workgroup of NT threads.  Their cosines
+// and sines are made once, in LDS, while the first heads are on their way; a
+// thread takes eight pairs of a head in WIDE (16-byte loads and stores: pairs
+// 8 u .. of the rotated part, or 16 dims behind it; needs a rotary_dim and
+// head_dim that 16 divides and rows at 16-byte addresses), otherwise one pair,
+// and then the same of the head NT / per_head further on, whose loads are under
+// way while this one is turned.  12001 tokens of 32 + 8 heads out of cache 47 us
+// (5.2 TB/s); with the turns made by each thread for up to 8 heads of its own
+// 51.5, for 2 of them 56.
+template <bool BF16, bool WIDE, int NT>
+__device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int b) {
   constexpr int P = WIDE ? 8 : 1;
-  const uint32_t u = i % a.per_head, tg = i / a.per_head, t = tg / a.groups, g = tg % a.groups;
-  if (t >= (uint32_t)a.n_tokens) return;
-  const int pos = a.positions[t];
-  if (pos < 0) return;
-  const bool rotate = 2 * P * (int)u < a.rot;
-  const bool halves = rotate && !a.interleaved;
-  const int d0 = halves ? P * u : 2 * P * u, d1 = halves ? P * u + a.rot / 2 : 2 * P * u + P;
-  CosSin cs[P];
-#pragma unroll
-  for (int e = 0; e < P; ++e) {
-    cs[e] = rotate ? turn(a.freq[P * u + e], pos) : CosSin{1.0, 0.0};
-    cs[e].c *= a.magnitude;
-    cs[e].s *= a.magnitude;
-  }
-  const int all = a.heads[0] + a.heads[1], h1 = min((int)(g + 1) * a.heads_each, all);
-  for (int hh = (int)g * a.heads_each; hh < h1; ++hh) {
-    const int w = hh >= a.heads[0], h = w ? hh - a.heads[0] : hh;
-    const uint16_t* src = (w ? a.src[1] : a.src[0]) + (int64_t)t * (w ? a.token_stride[1] : a.token_stride[0]) +
-                          h * (w ? a.head_stride[1] : a.head_stride[0]);
-    uint16_t* dst = (w ? a.dst[1] : a.dst[0]) + ((int64_t)t * (w ? a.heads[1] : a.heads[0]) + h) * a.head_dim;
-    uint16_t v[2 * P];
+  static_assert(NT >= kTurns);
+  __shared__ __align__(16) CosSin s_turn[kTurns];
+  __shared__ int s_pos[kTurns];
+  const int tid = threadIdx.x, t0 = b * a.tokens_each, nt = min(a.tokens_each, a.n_tokens - t0);
+  const int pairs = a.rot / 2, lanes = pairs / P, all = a.heads[0] + a.heads[1];
+  const int slot = tid / a.per_head, slots = NT / a.per_head, u = tid - slot * a.per_head;
+  const bool rotate = u < lanes, halves = rotate && !a.interleaved;
+  const int d0 = halves ? P * u : 2 * P * u, d1 = halves ? P * u + pairs : 2 * P * u + P;
+  uint16_t v[2 * P], ahead[2 * P];
+  auto load = [&](uint16_t* x, int t, int h) {
+    const int w = h >= a.heads[0];
+    const uint16_t* p = (w ? a.src[1] : a.src[0]) + (int64_t)(t0 + t) * (w ? a.token_stride[1] : a.token_stride[0]) +
+                        (w ? h - a.heads[0] : h) * (w ? a.head_stride[1] : a.head_stride[0]);
     if constexpr (WIDE) {
-      *reinterpret_cast<u32x4*>(v) = *reinterpret_cast<const u32x4*>(src + d0);
-      *reinterpret_cast<u32x4*>(v + 8) = *reinterpret_cast<const u32x4*>(src + d1);
+      *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(p + d0);
+      *reinterpret_cast<u32x4*>(x + 8) = *reinterpret_cast<const u32x4*>(p + d1);
     } else {
-      v[0] = src[d0];
-      v[1] = src[d1];
+      x[0] = p[d0];
+      x[1] = p[d1];
     }
+  };
+  int t = slot / all, h = slot - t * all;
+  if (slot >= slots) t = nt;                     // threads past the last whole head
+  if (t < nt) load(v, t, h);
+  if (tid < nt) s_pos[tid] = a.positions[t0 + tid];
+  if (tid < nt * pairs) {
+    const int tok = tid / pairs, i = tid - tok * pairs;      // pair 8 u + e at e * lanes + u: no bank conflicts
+    CosSin x = turn(a.freq[WIDE ? i % lanes * P + i / lanes : i], a.positions[t0 + tok]);
+    x.c *= a.magnitude;
+    x.s *= a.magnitude;
+    s_turn[tid] = x;
+  }
+  __syncthreads();
+  while (t < nt) {
+    int next = t, nh = h + slots;
+    while (nh >= all) {
+      nh -= all;
+      ++next;
+    }
+    if (next < nt) load(ahead, next, nh);
     if (rotate) {
+      const CosSin* cs = s_turn + t * pairs + u;
       if (a.interleaved) {
 #pragma unroll
         for (int e = 0; e < P; ++e) {
-          const f32x2 o = turned(widen<BF16>(v[2 * e]), widen<BF16>(v[2 * e + 1]), cs[e]);
+          const f32x2 o = turned(widen<BF16>(v[2 * e]), widen<BF16>(v[2 * e + 1]), cs[e * lanes]);
           v[2 * e] = narrow<BF16>(o.x);
           v[2 * e + 1] = narrow<BF16>(o.y);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < P; ++e) {
-          const f32x2 o = turned(widen<BF16>(v[e]), widen<BF16>(v[e + P]), cs[e]);
+          const f32x2 o = turned(widen<BF16>(v[e]), widen<BF16>(v[e + P]), cs[e * lanes]);
           v[e] = narrow<BF16>(o.x);
           v[e + P] = narrow<BF16>(o.y);
         }
       }
     }
-    if constexpr (WIDE) {
-      *reinterpret_cast<u32x4*>(dst + d0) = *reinterpret_cast<const u32x4*>(v);
-      *reinterpret_cast<u32x4*>(dst + d1) = *reinterpret_cast<const u32x4*>(v + 8);
-    } else {
-      dst[d0] = v[0];
-      dst[d1] = v[1];
+    if (s_pos[t] >= 0) {
+      const int w = h >= a.heads[0];
+      uint16_t* p = (w ? a.dst[1] : a.dst[0]) + ((int64_t)(t0 + t) * (w ? a.heads[1] : a.heads[0]) + (w ? h - a.heads[0] : h)) * a.head_dim;
+      if constexpr (WIDE) {
+        *reinterpret_cast<u32x4*>(p + d0) = *reinterpret_cast<const u32x4*>(v);
+        *reinterpret_cast<u32x4*>(p + d1) = *reinterpret_cast<const u32x4*>(v + 8);
+      } else {
+        p[d0] = v[0];
+        p[d1] = v[1];
+      }
     }
+    t = next;
+    h = nh;
+#pragma unroll
+    for (int e = 0; e < 2 * P; ++e) v[e] = ahead[e];
   }
 }
 
@@ -173,16 +199,16 @@ inline bool rotary_fill(RotaryArgs& a, const oi2_heads* q, void* q_out, const oi
            in[w]->head_stride % 8 == 0;
   }
   a.per_head = a.head_dim / (wide ? 16 : 2);
-  const int all = a.heads[0] + a.heads[1];
-  // as many heads a thread as still leave 2^18 threads (4 waves a SIMD)
-  a.heads_each = 1;
-  auto groups = [&](int each) { return (all + each - 1) / each; };
-  while (a.heads_each < 8 && (int64_t)a.n_tokens * a.per_head * groups(2 * a.heads_each) >= 1 << 18) a.heads_each *= 2;
-  a.groups = groups(a.heads_each);
+  // as many tokens a workgroup as there is room for their turns, and as leave
+  // 512 workgroups
+  a.tokens_each = kTurns / (a.rot / 2);
+  while (a.tokens_each > 1 && a.n_tokens / a.tokens_each < 512) a.tokens_each /= 2;
   return wide;
 }
 
-inline int64_t rotary_threads(const RotaryArgs& a) { return (int64_t)a.n_tokens * a.per_head * a.groups; }
+inline int64_t rotary_workgroups(const RotaryArgs& a) {
+  return a.heads[0] + a.heads[1] ? ((int64_t)a.n_tokens + a.tokens_each - 1) / a.tokens_each : 0;
+}
 
 int check_rotary(const oi2_rotary* r);
 
