@@ -120,7 +120,7 @@ class PagedKVCache:
     def new_plan(self, max_tokens: int, max_new: int | None = None) -> PagePlan:
         """Room for the layout of steps of up to max_tokens tokens, max_new of
         one row (max_tokens by default).  A plan belongs to its cache and serves
-        one step at a time.  Decoding steps want max_new as small as it is:
+        one step, and one attend, at a time.  Decoding steps want max_new as small as it is:
         attention then leaves out its kernel for many rows."""
         return PagePlan(self, max_tokens, max_new)
 
@@ -129,6 +129,8 @@ class PagedKVCache:
             lens = torch.tensor(lens, dtype=torch.int32)
         if lens.shape != (self.n_seqs,) or lens.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"lengths: ({self.n_seqs},) int32, got {tuple(lens.shape)} {lens.dtype}")
+        if lens.dtype == torch.int64:
+            lens = lens.clamp(-1, 2 ** 31 - 1)       # not to wrap
         return lens.to(self.device, torch.int32).contiguous()
 
     def _plan(self, plan: PagePlan) -> PagePlan:
@@ -137,9 +139,10 @@ class PagedKVCache:
         return plan
 
     def extend(self, new_lens, plan: PagePlan) -> PagePlan:
-        """Row i grows by new_lens[i] positions (0: not in the step); the plan
-        is written and returned.  new_lens: (n_seqs) int32 on the device, or
-        anything that converts to that.  Rejected rows are not an error here:
+        """Row i grows by new_lens[i] positions (0 or less: not in the step); the
+        plan is written and returned.  new_lens: (n_seqs) int32 on the device, or
+        anything that converts to that (a list waits for its copy, and cannot be
+        captured into a graph).  Rejected rows are not an error here:
         ``plan.rejected`` tells, at the price of waiting for it."""
         plan, new_lens = self._plan(plan), self._lens(new_lens)
         L = _lib.load_library()

@@ -534,3 +534,50 @@ def test_append_of_the_first_tokens_leaves_the_rest(dev):
             ref["kv_len"] = [a + b for a, b in zip(ref["past"], cut)]
             o.append(_np(k), _np(v), ref)
         _check_codes(c, o)
+
+
+def test_lengths_of_64_bits_do_not_wrap(dev):
+    print("[tables] 64-bit lengths", flush=True)
+    c, o = _pair(1, 3, 200, 12, dev, n_q=1)
+    plan = c.new_plan(300)
+    big = 2 ** 32
+    c.extend(torch.tensor([70, big + 5, -big - 7], device=dev), plan)
+    assert plan.rejected.tolist() == [0, 1, 1] and c.lens.tolist() == [70, 0, 0]
+    c.rewind(torch.tensor([big + 1, -big, 0], device=dev))
+    assert c.lens.tolist() == [70, 0, 0]
+
+
+def test_pages_past_32_bit_offsets(dev):
+    """A pool of 10 GB whose last pages are used: the same outputs and codes as
+    in a small one."""
+    print("[paged] 10 GB pool", flush=True)
+    g = torch.Generator(device=dev).manual_seed(10)
+    n_kv, past, new = 32, [700, 64], [1, 90]
+    kv = [torch.randn((n, n_kv, D), generator=g, device=dev).half() for n in (sum(past), sum(past), sum(new), sum(new))]
+    q = torch.randn((sum(new), 32, D), generator=g, device=dev).half()
+    got = []
+    for n_pages in (20, 20000):
+        c = oi2.PagedKVCache(1, 32, n_kv, 2, 800, n_pages, device=dev)
+        c.free.copy_(torch.arange(n_pages, dtype=torch.int32))          # the last pages first
+        c.append(0, kv[0], kv[1], c.extend(past, c.new_plan(sum(past))))
+        few = c.new_plan(sum(new), max_new=90)
+        c.append(0, kv[2], kv[3], c.extend(new, few))
+        assert int(c.block_table.max()) == n_pages - 1
+        got.append((c.attend(0, q, few), *c.read(0, 0), *c.read(0, 1)))
+        del c
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_a_query_that_is_not_finite_harms_no_other(dev, dtype, bad):
+    print(f"[attend] query with {bad}", flush=True)
+    for past, new in (([700, 90], [3, 1]), ([300, 5000], [150, 40])):
+        c, o, plan, ref, q = _filled(dev, 32, 8, past, new, dtype, 11)
+        y = c.attend(0, q, plan)
+        t, h = sum(new) // 2, 9
+        q[t, h, 5] = bad
+        z = c.attend(0, q, plan)
+        assert z[t, h].isnan().all()
+        z[t, h] = y[t, h]
+        assert torch.equal(z, y)
