@@ -530,14 +530,17 @@ __device__ __forceinline__ f32x16 mfma32(h8 a, h8 b, f32x16 c) {
 
 // In LDS, fp16: two pages of k, rows of one position (256 bytes, 16 chunks of 8
 // dims), and two of v, rows of one dim (128 bytes, 8 chunks of 8 positions).
-// Chunks are swizzled within their rows so that staging stores and fragment
-// reads touch all banks: k's by position p = 16 a + 4 t + i with i | (a ^ t) << 2,
-// distinct for the 16 rows of a store (one t) and of a read (one a); v's by
+// Chunks are swizzled within their rows so that staging stores (16 lanes in a
+// row) and fragment reads touch all banks: k's by position p = 16 a + 4 t + i
+// with i | (t ^ 3 (a % 2) ^ 2 (a / 2)) << 2, distinct for the rows of a store (one
+// t) and for those that a 16-byte read takes in one cycle, which are lanes 0-3,
+// 12-15 and 20-27, or 4-11, 16-19 and 28-31 (with a ^ t they met in pairs: 5000
+// tokens 248 -> 233 us in bf16); v's by
 // d / 2.  Every address is a lane's base with constant bits flipped and a
 // constant added, which costs an instruction where a register each would spill.
 constexpr int kHalfLds = kPage * 256, kVLds = 2 * kHalfLds;
 static_assert(kHalfLds == kHeadD * 128, "a page of k and one of v");
-__device__ __forceinline__ int k_swz(int p) { return (p & 3) | ((((p >> 4) ^ (p >> 2)) & 3) << 2); }
+__device__ __forceinline__ int k_swz(int p) { return (p & 3) | (((p >> 2 & 3) ^ (p >> 4 & 3) ^ (p >> 3 & 2)) << 2); }
 __device__ __forceinline__ int k_lds(int p, int c) { return p * 256 + 16 * (c ^ k_swz(p)); }
 __device__ __forceinline__ int v_lds(int d, int c) { return kVLds + d * 128 + 16 * (c ^ ((d >> 1) & 7)); }
 
