@@ -119,10 +119,13 @@ __device__ __forceinline__ h8 q_frag(const uint16_t (&v)[8], int e, bool negate)
   return negate ? -r : r;
 }
 
-// Eight probabilities, times 2^kLift, as the operand of out^T = V^T P^T.  fp16
-// outputs take them in two fp16 parts (hi truncated, lo the rest: at least 21
-// bits), as one part's rounding would be as large as the output's own.  Of bf16
-// outputs, rounded to 8 bits, it is an eighth: one part, to nearest.
+// Eight probabilities, times 2^kLift, as the operand of out^T = V^T P^T.  One
+// fp16 part, to nearest, rounds them to half a step of fp16, an eighth of a bf16
+// output's own rounding.  Where the products cost no time (few rows, bound by
+// the pages' bytes) fp16 outputs take two parts (hi truncated, lo the rest: at least
+// 21 bits); with many rows the second part would be a third of all products
+// (5000 tokens 340 us instead of 239), for an error of 2.0e-4 instead of 2.7e-4 of the
+// values, whose codes keep 4 bits: one part.
 template <bool BF16>
 struct Probs {
   h8 hi, lo;
@@ -554,13 +557,17 @@ __device__ __forceinline__ int v_lds(int d, int c) { return kVLds + d * 128 + 16
 //
 // The next page's staging stands between the products of the scores, and a
 // fragment's exponentials between the products of the fragment before.  What
-// bounds it: matrix cores and vector unit are busy about half the time each, and
-// two waves a SIMD (206 registers) overlap little more than that by chance: 5000
-// tokens 325 us in fp16 (630 TFLOP/s), 240 in bf16 (853).  Tried without gain:
-// fragments read three steps ahead; raised priority around the products; one
-// wave a SIMD with 64 rows and the next page's scores between this one's
-// exponentials, whose accumulators in AGPRs cost more copies than the shared
-// fragments save (326 us in bf16); the same with 32 rows, which spilled (272).
+// bounds it: matrix cores, vector unit and LDS are busy about half the time each,
+// and two waves a SIMD overlap little more than that by chance: 5000 tokens 239
+// us in fp16 and 235 in bf16 (865 TFLOP/s); of 249, before k's conflicts went, the
+// exponentials alone made 38, staging 35, the fragments' reads 55, the products
+// 68.  Tried without gain: fragments read three steps ahead; raised priority around
+// the products; one wave a SIMD with 64 rows and the next page's scores between
+// this one's exponentials, whose accumulators in AGPRs cost more copies than the
+// shared fragments save (326 us in bf16); the same with 32 rows, which spilled
+// (272); eight waves over 256 rows, four of them half a page behind, products
+// beside the others' softmax: that hides the softmax, but leaves the 10 us of a
+// workgroup's start and end bare, with one workgroup a CU (251).
 constexpr int kManyLds = 4 * kHalfLds + kHeadD * 4;
 
 template <bool BF16>
@@ -725,21 +732,20 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
         sum[f] += e[j];
       }
     };
-    Probs<BF16> p;
+    h8 p;
     exps(0, 0, 8);
-    p = to_probs<BF16>(e);
+    p = to_probs<true>(e).hi;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         if (4 * f + d < 13) read_v(va, 4 * f + d + 3);
-        o[d] = mfma32(vf[d], p.hi, o[d]);
-        if (!BF16) o[d] = mfma32(vf[d], p.lo, o[d]);
+        o[d] = mfma32(vf[d], p, o[d]);
         if (f < 3) exps(f + 1, 2 * d, 2 * d + 2);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (f < 3) p = to_probs<BF16>(e);
+      if (f < 3) p = to_probs<true>(e).hi;
     }
     l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ldexp2(1.0f, -(int)ev), l);
   };

@@ -5,7 +5,7 @@ Tables, codes and scales are compared bit for bit.  Rotary outputs may be off
 by half a step of their type and of fp32, and the pair times 2^-40 (fp64 on both sides) and
 times what half a step of a 64-bit frequency makes at the token's position; attention outputs by half a step of their type
 and the oracle's bound on fp32 sums and on the probabilities' fp16 parts (two
-for fp16 outputs, one for bf16).
+for fp16 outputs of up to 16 query rows, otherwise one).
 """
 import math
 import random
