@@ -267,10 +267,14 @@ class on_device:
             torch.cuda.set_device(self.before)
 
 
-def heads(x: torch.Tensor) -> Heads:
-    """(tokens, heads, dim) as the C ABI takes it; the last dimension dense."""
+def heads(x: torch.Tensor, n: int) -> tuple[torch.Tensor, Heads]:
+    """(tokens, n heads, dim) as the C ABI takes it, and the tensor that it
+    points into: x, or a copy where its last dimension is not dense."""
     st = x.stride()
-    return Heads(x.data_ptr(), x.shape[1], st[0], st[1])
+    if st[2] != 1:
+        x = x.contiguous()
+        st = x.stride()
+    return x, Heads(x.data_ptr(), n, st[0], st[1])
 
 
 def logit_threshold(p: float) -> float:

@@ -160,7 +160,7 @@ class PagedKVCache:
             _lib.check(L.oi2_page_rewind(self._ref, lens.data_ptr(), stream))
 
     # -- pages ----------------------------------------------------------------
-    def _rows(self, x: torch.Tensor, heads: int, what: str, like: torch.Tensor | None = None) -> torch.Tensor:
+    def _rows(self, x: torch.Tensor, heads: int, what: str, like: torch.Tensor | None = None):
         shape = x.shape
         if len(shape) != 3 or shape[1] != heads or shape[2] != HEAD_DIM:
             raise ValueError(f"{what}: (tokens, {heads}, {HEAD_DIM}), got {tuple(shape)}")
@@ -170,7 +170,7 @@ class PagedKVCache:
             raise ValueError(f"{what} on {x.device}, the cache on {self.device}")
         if like is not None and (shape[0] != like.shape[0] or x.dtype != like.dtype):
             raise ValueError(f"{what} {tuple(x.shape)} {x.dtype} beside {tuple(like.shape)} {like.dtype}")
-        return x if x.stride(2) == 1 else x.contiguous()
+        return _lib.heads(x, heads)
 
     def _layer(self, layer: int) -> int:
         if not 0 <= int(layer) < self.n_layers:
@@ -192,8 +192,8 @@ class PagedKVCache:
         left out, in q's output too.  Each layer takes a step once: what a page
         holds is coded again when its scale grows."""
         plan, layer = self._plan(plan), self._layer(layer)
-        k = self._rows(k, self.n_kv, "k")
-        v = self._rows(v, self.n_kv, "v", k)
+        k, hk = self._rows(k, self.n_kv, "k")
+        v, hv = self._rows(v, self.n_kv, "v", k)
         n = self._tokens(k, plan)
         if rotary is None:
             if q is not None or q_out is not None:
@@ -201,7 +201,7 @@ class PagedKVCache:
         elif rotary.head_dim != HEAD_DIM or rotary.device != self.device:
             raise ValueError(f"a rotary of head_dim {HEAD_DIM} on {self.device}, got {rotary.head_dim} on {rotary.device}")
         if q is not None:
-            q = self._rows(q, q.shape[1] if q.dim() == 3 else self.n_q, "q", k)
+            q, hq = self._rows(q, q.shape[1] if q.dim() == 3 else self.n_q, "q", k)
             q_out = rotary._output(q_out, q, "q_out")
             if q_out.data_ptr() == q.data_ptr() and not q.is_contiguous():
                 raise ValueError("an output that is its own input must be contiguous")
@@ -211,9 +211,9 @@ class PagedKVCache:
         with _lib.on_device(self.device) as stream:
             _lib.check(L.oi2_kv_append(
                 self._ref, plan._ref, layer, _lib.dtype_code(k.dtype), n,
-                ctypes.byref(_lib.heads(k)), ctypes.byref(_lib.heads(v)),
+                ctypes.byref(hk), ctypes.byref(hv),
                 None if rotary is None else rotary._ref,
-                None if q is None else ctypes.byref(_lib.heads(q)), _lib.ptr(q_out), stream))
+                None if q is None else ctypes.byref(hq), _lib.ptr(q_out), stream))
         return q_out
 
     def attend(self, layer: int, q: torch.Tensor, plan: PagePlan, scale: float | None = None,
@@ -225,7 +225,7 @@ class PagedKVCache:
         128) like q: zeros for the tokens of rejected rows; rows past the step's
         last token are not written."""
         plan, layer = self._plan(plan), self._layer(layer)
-        q = self._rows(q, self.n_q, "q")
+        q, hq = self._rows(q, self.n_q, "q")
         n = self._tokens(q, plan)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -237,7 +237,7 @@ class PagedKVCache:
             ws = q.new_empty((nbytes,), dtype=torch.uint8)
             _lib.check(L.oi2_kv_attend(
                 self._ref, plan._ref, layer, _lib.dtype_code(q.dtype), n,
-                ctypes.byref(_lib.heads(q)), HEAD_DIM ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                ctypes.byref(hq), HEAD_DIM ** -0.5 if scale is None else float(scale), out.data_ptr(),
                 ws.data_ptr(), nbytes, stream))
         return out
 

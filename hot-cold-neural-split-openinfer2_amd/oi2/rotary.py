@@ -111,7 +111,7 @@ class Rotary:
                                    self.freq.data_ptr())
         self._ref = ctypes.byref(self._struct)
 
-    def _rows(self, x: torch.Tensor, what: str) -> torch.Tensor:
+    def _rows(self, x: torch.Tensor, what: str):
         shape = x.shape
         if len(shape) != 3 or shape[2] != self.head_dim:
             raise ValueError(f"{what}: (tokens, heads, {self.head_dim}), got {tuple(shape)}")
@@ -119,7 +119,7 @@ class Rotary:
             raise TypeError(f"{what}: float16 or bfloat16, got {x.dtype}")
         if x.device != self.device:
             raise ValueError(f"{what} on {x.device}, the rotary frequencies on {self.device}")
-        return x if x.stride(2) == 1 else x.contiguous()
+        return _lib.heads(x, shape[1])
 
     def _output(self, out, x: torch.Tensor, what: str) -> torch.Tensor:
         if out is None:
@@ -133,10 +133,11 @@ class Rotary:
         or None, fp16 or bf16, any strides; positions (tokens) int32.  q_out and
         k_out: contiguous outputs, which may be the inputs themselves.  A token
         at a negative position is left out: its output rows are not written."""
-        q = self._rows(q, "q")
+        q, hq = self._rows(q, "q")
         N = q.shape[0]
+        hk = _lib.Heads()
         if k is not None:
-            k = self._rows(k, "k")
+            k, hk = self._rows(k, "k")
             if k.shape[0] != N or k.dtype != q.dtype:
                 raise ValueError(f"k {tuple(k.shape)} {k.dtype} beside q {tuple(q.shape)} {q.dtype}")
         if positions.shape != (N,) or positions.dtype != torch.int32 or positions.device != self.device:
@@ -151,7 +152,7 @@ class Rotary:
         with _lib.on_device(self.device) as stream:
             _lib.check(L.oi2_rotary_apply(
                 self._ref, _lib.dtype_code(q.dtype), N, positions.contiguous().data_ptr(),
-                ctypes.byref(_lib.heads(q)), qo.data_ptr(),
-                ctypes.byref(_lib.Heads() if k is None else _lib.heads(k)), _lib.ptr(ko),
+                ctypes.byref(hq), qo.data_ptr(),
+                ctypes.byref(hk), _lib.ptr(ko),
                 stream))
         return qo, ko
