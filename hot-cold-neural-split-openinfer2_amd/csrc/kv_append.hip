@@ -12,8 +12,10 @@
 // only where its scale grows.  q has workgroups of its own behind them in the
 // same launch.
 //
-// Bound by the bytes of k, v and q in prompts; a step of single tokens by the
-// chain of its loads, the reduction and the stores.
+// Bound by the bytes of k, v and q in prompts (7110 tokens of 32 + 8 + 8 heads,
+// out of cache, 35.8 us, 4.4 TB/s; k and v alone 17, the chain of a page's
+// heads); a step of single tokens by the chain of its loads, the reduction and
+// the stores (16 rows 4.5 us, 40 rows of four tokens 8.7).
 #include "capi_util.h"
 #include "kv_cache.h"
 #include "rotary.h"

@@ -303,6 +303,13 @@ constexpr int kFewLds = (kFewWaves * kFewRows * (kORow + 2) + kHeadD) * 4;
 // the score of query row r at position 16 grp + 4 t + i: in 4 tiles a lane has
 // positions 16 grp .. 16 grp + 15 of its query row, which are the positions of
 // the 16 bytes of V^T that it loads for each dim.
+//
+// A wave takes every fourth page, loads the next one (k and v, 16 KB) while it
+// works on this one, and its page number by a scalar load two ahead; the four
+// meet in LDS at the end.  Bound by the pages' bytes: 56 tokens of 300 to 14000
+// positions 72 us (5.3 TB/s), three of 40 to 110 thousand 46 (5.2); one of 700
+// positions 8.0, three rounds and the merge.  Tried without gain: 8 and 16
+// waves, pages dealt out in equal shares whatever row they belong to.
 template <bool BF16>
 __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* smem) {
   const int item = b / a.n_kv, g = b - item * a.n_kv;
