@@ -49,11 +49,14 @@ template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xF, false);
 }
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+__device__ __forceinline__ uint32_t row_scan(uint32_t v) {
   v = add_sat(v, dpp_u32<0x111, 0xF>(v));
   v = add_sat(v, dpp_u32<0x112, 0xF>(v));
   v = add_sat(v, dpp_u32<0x114, 0xF>(v));
-  v = add_sat(v, dpp_u32<0x118, 0xF>(v));
+  return add_sat(v, dpp_u32<0x118, 0xF>(v));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = row_scan(v);
   v = add_sat(v, dpp_u32<0x142, 0xA>(v));
   v = add_sat(v, dpp_u32<0x143, 0xC>(v));
   return v;
@@ -64,24 +67,22 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 // barrier.
 template <int N>
 __device__ __forceinline__ void scan_excl(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t* s) {
-  const int lane = lane_id(), wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = blockDim.x >> 6;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     v[k] = wave_scan(v[k]);
     if (lane == 63) s[wave * N + k] = v[k];
     v[k] = dpp_u32<0x138, 0xF>(v[k]);      // wave_shr:1, 0 in lane 0
-    total[k] = 0;
   }
   __syncthreads();
-#pragma unroll 1
-  for (int w = 0; w < waves; ++w)
+  // the waves' sums, up to 16, by the lanes of one row
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const uint32_t t = s[w * N + k];
-      if (w < wave) v[k] = add_sat(v[k], t);
-      total[k] = add_sat(total[k], t);
-    }
+  for (int k = 0; k < N; ++k) {
+    const uint32_t t = row_scan(lane < waves ? s[lane * N + k] : 0);
+    total[k] = (uint32_t)__builtin_amdgcn_readlane((int)t, 15);
+    if (wave > 0) v[k] = add_sat(v[k], (uint32_t)__builtin_amdgcn_readlane((int)t, wave - 1));
+  }
 }
 
 // The last row r with sum[r] <= i, of n rows with ascending exclusive sums:
