@@ -12,8 +12,8 @@
 // (which every launch fetches anew), not by bytes: a few kilobytes for a
 // decoding step.  So counts are 32-bit and saturate, shares are products and
 // groups shifts, and plans of short rows leave out the lists for long ones:
-// 6 KB of code instead of 11, eight rows of a step 11.1 -> 7.6 us.  700 prompts
-// of 115 thousand tokens: 32 us and 5 for the positions and slots.
+// 6 KB of code instead of 11, eight rows of a step 11.1 -> 7.2 us.  700 prompts
+// of 115 thousand tokens: 28 us and 5 for the positions and slots.
 #include "capi_util.h"
 #include "kv_cache.h"
 #include "oi2_device.h"
