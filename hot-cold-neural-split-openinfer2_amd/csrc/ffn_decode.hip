@@ -28,6 +28,7 @@
 // the compiler wait for all of them where the branches join.)
 #include "capi_util.h"
 #include "ffn_kernels.h"
+#include "kv_cache.h"
 #include "decode_util.h"
 
 namespace oi2 {
@@ -1105,6 +1106,58 @@ __global__ __launch_bounds__(kThreads) void k_query(const uint16_t* x, int rows,
   }
 }
 
+// The same query for the packed tokens of a step over the paged cache, whose
+// mean is over the last token of every row that is taken and has tokens in the
+// call (tokens of rejected rows and past the step's end have no say, whatever
+// they hold).  A workgroup a row finds that token and its norm; then a thread
+// a column takes the rows in order, so that the sums round as k_query's.  The
+// rows' loads are independent of each other there, where k_query waits for a
+// reduction a row.
+__global__ __launch_bounds__(kThreads) void k_row_norms(const uint16_t* x, int n_tokens, const int32_t* cu,
+                                                        const int32_t* kv_len, int norm, float eps, int32_t* tok,
+                                                        float* rnorm) {
+  __shared__ float s_parts[kThreads];
+  const int i = blockIdx.x, t0 = cu[i], t1 = min(cu[i + 1], n_tokens);
+  const bool live = kv_len[i] > 0 && t0 >= 0 && t0 < t1;
+  const float r = live && norm ? block_rnorm(x + (size_t)(t1 - 1) * kH, eps, s_parts) : 1.0f;
+  if (threadIdx.x == 0) {
+    tok[i] = live ? t1 - 1 : -1;
+    rnorm[i] = r;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void k_query_rows(const uint16_t* x, int n_seqs, const int32_t* tok,
+                                                         const float* rnorm, const uint16_t* w, int to_bf16, float* q) {
+  __shared__ int32_t s_tok[OI2_MAX_SEQS];
+  __shared__ float s_r[OI2_MAX_SEQS];
+  __shared__ int s_n;
+  if (threadIdx.x < 64) {                  // the rows with a token, in order
+    int n = 0;
+    for (int i0 = 0; i0 < n_seqs; i0 += 64) {
+      const int i = i0 + threadIdx.x, t = i < n_seqs ? tok[i] : -1;
+      const uint64_t is = __ballot(t >= 0);
+      if (t >= 0) {
+        const int at = n + __popcll(is & ((1ull << threadIdx.x) - 1));
+        s_tok[at] = t;
+        s_r[at] = rnorm[i];
+      }
+      n += __popcll(is);
+    }
+    if (threadIdx.x == 0) s_n = n;
+  }
+  __syncthreads();
+  const int n = s_n, col = blockIdx.x * kThreads + threadIdx.x;
+  const float wv = w ? half_bits_to_float(w[col]) : 1.0f;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) {
+    const float v = half_bits_to_float(x[(size_t)s_tok[i] * kH + col]);
+    sum += w ? xn_exact(v, s_r[i], wv) : v;
+  }
+  const float m = n ? round_f16(sum / (float)n) : 0.0f;
+  q[col] = to_bf16 ? round_bf16(m) : m;
+}
+
 // One hidden-state row of any supported dtype cast to the predictor dtype
 // (predictor.py:455: hidden_state.to(parameter dtype)), as fp32 values: fp16
 // and bf16 widen exactly; fp32 is kept, or rounded to bf16 for a bf16
@@ -1420,6 +1473,12 @@ size_t oi2_predict_workspace_bytes(const oi2_predictor* p) {
   return pred_ws_ssq_off(rank) + (size_t)kDownWG * sizeof(float);
 }
 
+// With a token and a norm per row of the cache behind it.
+size_t oi2_predict_packed_workspace_bytes(const oi2_predictor* p, int32_t n_seqs) {
+  if (n_seqs < 1 || n_seqs > OI2_MAX_SEQS) return 0;
+  return oi2_predict_workspace_bytes(p) + (size_t)n_seqs * 8;
+}
+
 int launch_predictor(const TokenIn& tok, const uint16_t* norm_w, const float* q,
                      const oi2_predictor* p, float thr, const int32_t* lut, int32_t* slots,
                      int32_t* ids, int32_t* counts, float* logits, float* probs, uint8_t* mask,
@@ -1527,6 +1586,38 @@ int oi2_predict_select(const uint16_t* x, int32_t batch, const uint16_t* norm_w,
     OI2_CHECK_LAUNCH();
   }
   return OI2_OK;
+}
+
+int oi2_predict_select_packed(const uint16_t* x, int32_t n_tokens, const oi2_paged* c, const oi2_page_plan* plan,
+                              const uint16_t* norm_w, float eps, const oi2_predictor* p, float threshold_logit,
+                              const int32_t* lut, int32_t* slots, int32_t* ids, int32_t* counts, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  clear_error();
+  int rc = validate_pred(p);
+  if (rc) return rc;
+  if ((rc = check_paged(c, 0, false))) return rc;
+  if ((rc = check_plan(c, plan))) return rc;
+  OI2_CHECK_ARG(n_tokens >= 1 && n_tokens <= plan->max_tokens, "%d tokens in a plan of %d", n_tokens, plan->max_tokens);
+  OI2_CHECK_ARG(x && (uintptr_t)x % 16 == 0, "x must be non-null and 16-byte aligned");
+  OI2_CHECK_ARG(!norm_w || (uintptr_t)norm_w % 16 == 0, "norm_w must be 16-byte aligned");
+  OI2_CHECK_ARG(slots && ids && counts, "selection outputs are null");
+  OI2_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0 &&
+                    workspace_bytes >= oi2_predict_packed_workspace_bytes(p, c->n_seqs),
+                "predict workspace too small");
+  hipStream_t st = (hipStream_t)stream;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  float* q = reinterpret_cast<float*>(ws);
+  double* z = reinterpret_cast<double*>(ws + pred_ws_z_off());
+  int32_t* tok = reinterpret_cast<int32_t*>(ws + oi2_predict_workspace_bytes(p));
+  float* rnorm = reinterpret_cast<float*>(tok + c->n_seqs);
+  hipLaunchKernelGGL(k_row_norms, dim3(c->n_seqs), dim3(kThreads), 0, st, x, n_tokens, plan->cu, plan->kv_len,
+                     norm_w ? 1 : 0, eps, tok, rnorm);
+  OI2_CHECK_LAUNCH();
+  hipLaunchKernelGGL(k_query_rows, dim3(kH / kThreads), dim3(kThreads), 0, st, x, c->n_seqs, tok, rnorm, norm_w,
+                     p->dtype == OI2_DTYPE_BF16 ? 1 : 0, q);
+  OI2_CHECK_LAUNCH();
+  return launch_predictor(TokenIn{nullptr, nullptr, nullptr, 0.0f, 0}, nullptr, q, p, threshold_logit, lut, slots, ids, counts,
+                          nullptr, nullptr, nullptr, z, st);
 }
 
 }  // extern "C"

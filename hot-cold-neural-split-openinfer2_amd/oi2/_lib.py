@@ -159,6 +159,10 @@ _SIGS = {
     "oi2_attn_forward_paged": (c_int32, [c_void_p, c_int32, POINTER(Attn), c_float, POINTER(Rotary),
                                          POINTER(Paged), POINTER(PagePlan), c_int32, c_void_p, c_void_p,
                                          c_void_p, c_size_t, c_void_p]),
+    "oi2_predict_packed_workspace_bytes": (c_size_t, [POINTER(Predictor), c_int32]),
+    "oi2_predict_select_packed": (c_int32, [c_void_p, c_int32, POINTER(Paged), POINTER(PagePlan), c_void_p, c_float,
+                                            POINTER(Predictor), c_float, c_void_p, c_void_p, c_void_p, c_void_p,
+                                            c_void_p, c_size_t, c_void_p]),
     "oi2_section_bytes": (c_size_t, [c_int32]),
     "oi2_quantize_section": (c_int32, [c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,

@@ -78,14 +78,17 @@ class DecoderStep:
         """The loop over a paged cache: x (tokens, H) fp16, the packed tokens of
         the step that ``cache.extend`` laid out in ``plan`` for requests of
         different lengths.  Layer li uses layer li of the cache.  The FFN takes
-        the tokens as one batch, which shares a predicted cold set (over a
-        DecodeStack: one token); tokens without a position take part in it, so
-        give them finite values.  Returns x after the last layer's FFN."""
+        the tokens as one batch, which shares a cold set: ``forward``'s, predicted
+        from the mean over the rows' last tokens, of the rows that are taken
+        and have tokens in the step (over a DecodeStack: one token).  Tokens
+        without a position (of rejected rows, or past the step's last one) have
+        no part in it.  Returns x after the last layer's FFN."""
         if x.dim() != 2:
             raise ValueError(f"x must be (tokens, hidden), got {tuple(x.shape)}")
         N, H = x.shape
         if cache.n_layers < len(self.attention_layers):
             raise ValueError(f"a cache of {cache.n_layers} layers for {len(self.attention_layers)}")
+        cache._tokens(x, cache._plan(plan))
         if N == 0:
             return x
         x = x.contiguous()
@@ -95,7 +98,9 @@ class DecoderStep:
                 raise ValueError(f"a DecodeStack runs one token at a time, got {N}")
             stack.predict(0, x.reshape(H))
         else:
-            prefetch = self.ffn_layers[0].submit_cold_fetch(x[None])
+            # one token: the query is that token's, whatever the plan says
+            step = plan if N > 1 else None
+            prefetch = self.ffn_layers[0].submit_cold_fetch(x, step)
         for li, attn in enumerate(self.attention_layers):
             resid = torch.empty_like(x)
             attn.forward_paged(x, cache, plan, rotary, layer=li, residual_out=resid)
@@ -105,7 +110,7 @@ class DecoderStep:
                 continue
             this = prefetch
             if li + 1 < len(self.ffn_layers):
-                prefetch = self.ffn_layers[li + 1].submit_cold_fetch(resid[None])
+                prefetch = self.ffn_layers[li + 1].submit_cold_fetch(resid, step)
             x = self.ffn_layers[li](resid[None], this)[0]
         return x
 

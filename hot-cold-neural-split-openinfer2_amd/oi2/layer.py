@@ -28,6 +28,7 @@ import torch
 
 from . import _lib
 from .hot import HotWeights
+from .paged import PagePlan
 from .store import ColdSection, ColdWeightStore
 
 HIDDEN = _lib.HIDDEN
@@ -315,7 +316,7 @@ class SparseFFNLayer(torch.nn.Module):
             ids.extend(cpu_ids[c * sel.chunk: c * sel.chunk + n].tolist())
         return ids
 
-    def _select(self, x: torch.Tensor, normed: bool) -> ColdNeurons:
+    def _select(self, x: torch.Tensor, normed: bool, plan: PagePlan | None = None) -> ColdNeurons:
         sec = self._section
         if sec is None:
             return ColdNeurons(None, None, None, 0, 0)
@@ -329,7 +330,7 @@ class SparseFFNLayer(torch.nn.Module):
             return ColdNeurons(sec, slots, torch.tensor([slots.shape[0]], dtype=torch.int32,
                                                         device=self.device),
                                1, max(1, int(slots.shape[0])))
-        q = x[:, -1, :] if x.dim() == 3 else x.reshape(-1, HIDDEN)
+        q = x[:, -1, :] if x.dim() == 3 and plan is None else x.reshape(-1, HIDDEN)
         q = q.to(torch.float16).contiguous()
         nc = self._n_chunks
         dev = self.device
@@ -338,6 +339,15 @@ class SparseFFNLayer(torch.nn.Module):
         counts = torch.empty(nc, dtype=torch.int32, device=dev)
         p = pred.struct()
         L = _lib.lib()
+        if plan is not None:
+            ws_bytes = L.oi2_predict_packed_workspace_bytes(ctypes.byref(p), plan.cache.n_seqs)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            _lib.check(L.oi2_predict_select_packed(
+                q.data_ptr(), q.shape[0], plan.cache._ref, plan._ref,
+                None if normed else self.norm_weight.data_ptr(), self.eps, ctypes.byref(p),
+                _lib.logit_threshold(self.threshold), sec.lut.data_ptr(), slots.data_ptr(), ids.data_ptr(),
+                counts.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_handle(dev)))
+            return ColdNeurons(sec, slots, counts, nc, _lib.SEL_CHUNK, ids=ids)
         ws_bytes = L.oi2_predict_workspace_bytes(ctypes.byref(p))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         _lib.check(L.oi2_predict_select(
@@ -347,10 +357,10 @@ class SparseFFNLayer(torch.nn.Module):
             None, ws.data_ptr(), ws_bytes, _lib.stream_handle(dev)))
         return ColdNeurons(sec, slots, counts, nc, _lib.SEL_CHUNK, ids=ids)
 
-    def _cold_slots_host(self, x: torch.Tensor, normed: bool) -> np.ndarray:
+    def _cold_slots_host(self, x: torch.Tensor, normed: bool, plan: PagePlan | None = None) -> np.ndarray:
         """The record slots of _cold_ids_for's list, ascending neuron id, on
         the host (the list the reference hands its executor, engine.py:289)."""
-        sel = self._select(x, normed)
+        sel = self._select(x, normed, plan)
         if sel.empty():
             return np.zeros(0, np.int32)
         counts = sel.counts.cpu().tolist()
@@ -374,16 +384,24 @@ class SparseFFNLayer(torch.nn.Module):
         cold.event = staged.event
         return cold
 
-    def submit_cold_fetch(self, x: torch.Tensor):
+    def submit_cold_fetch(self, x: torch.Tensor, plan: PagePlan | None = None):
         """engine.py:285-290: predict this layer's cold set from x (normalised
         with this layer's norm) and return an object with ``.result()``.  With
         a device-resident store the work is only enqueued on the stream, so
         the returned future is already complete; with file residency the
-        fetch runs on the executor (inline without one)."""
+        fetch runs on the executor (inline without one).
+
+        The set is predicted from the mean over the batch's last tokens.  With
+        ``plan`` x (tokens, H) holds the packed tokens of that step over a
+        paged cache, and the batch is its rows: those that are taken and have
+        tokens in x, each with the last of them."""
         with torch.no_grad():
+            if plan is not None and (plan.cache.device != x.device or x.numel() // HIDDEN > plan.max_tokens):
+                raise ValueError(f"x {tuple(x.shape)} on {x.device} for a plan of {plan.max_tokens} tokens "
+                                 f"on {plan.cache.device}")
             if not self._file:
-                return _Ready(self._select(x, normed=False))
-            slots = self._cold_slots_host(x, normed=False)
+                return _Ready(self._select(x, normed=False, plan=plan))
+            slots = self._cold_slots_host(x, normed=False, plan=plan)
             if self.executor is not None:
                 return self.executor.submit(self._fetch_file, slots)
             return _Ready(self._fetch_file(slots))

@@ -583,6 +583,17 @@ int oi2_attn_forward_paged(const uint16_t* x, int32_t n_tokens, const oi2_attn* 
                            uint16_t* out, uint16_t* x_out, void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/* oi2_predict_select for the n_tokens packed tokens of the plan's step, x
+ * (n_tokens, H) fp16: the query is the mean over the last token of every row
+ * that is taken and has tokens among them, as the batch of those tokens gives
+ * it (engine.py:275-277).  Tokens of rejected rows and past the step's last one
+ * are not read; without any row the query is 0. */
+size_t oi2_predict_packed_workspace_bytes(const oi2_predictor* p, int32_t n_seqs);
+int oi2_predict_select_packed(const uint16_t* x, int32_t n_tokens, const oi2_paged* c, const oi2_page_plan* plan,
+                              const uint16_t* norm_w, float eps, const oi2_predictor* p, float threshold_logit,
+                              const int32_t* lut, int32_t* slots, int32_t* ids, int32_t* counts, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* ---- split writer ------------------------------------------------------- */
 /* Bytes of one cold_weights.bin section with n_cold records: the 16-byte
  * <HHIq header, n_cold x 6400, zero padding to a 4096 multiple
