@@ -119,36 +119,26 @@ __device__ __forceinline__ h8 q_frag(const uint16_t (&v)[8], int e, bool negate)
   return negate ? -r : r;
 }
 
-// Eight probabilities, times 2^kLift, as the operand of out^T = V^T P^T.  One
-// fp16 part, to nearest, rounds them to half a step of fp16, an eighth of a bf16
-// output's own rounding.  Where the products cost no time (few rows, bound by
-// the pages' bytes) fp16 outputs take two parts (hi truncated, lo the rest: at least
-// 21 bits); with many rows the second part would be a third of all products
-// (5000 tokens 340 us instead of 239), for an error of 2.0e-4 instead of 2.7e-4 of the
-// values, whose codes keep 4 bits: one part.
-template <bool BF16>
+// Eight probabilities, times 2^kLift, as the operand of out^T = V^T P^T: two fp16
+// parts (hi truncated, lo the rest), 21 bits at least.  One part, to nearest,
+// is off by 2^-12 of a probability, as much as an fp16 output's own rounding
+// and an eighth of a bf16 one's: where values cancel that is most of the result,
+// and a token would get other bits in a prompt than in a step of its own.  It
+// would save a third of the products of many rows (a call of 5000 tokens 220 us
+// instead of 292) and nothing of few ones, which the pages' loads bound.
 struct Probs {
   h8 hi, lo;
 };
-template <bool BF16>
-__device__ __forceinline__ Probs<BF16> to_probs(const float (&e)[8]) {
-  Probs<BF16> p;
-  if constexpr (BF16) {
-    typedef float f8 __attribute__((ext_vector_type(8)));
-    p.hi = __builtin_convertvector((f8{e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]}), h8);
-  } else {
-    u32x4 uh, ul;
+__device__ __forceinline__ Probs to_probs(const float (&e)[8]) {
+  u32x4 uh, ul;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(e[2 * k], e[2 * k + 1]));
-      uh[k] = hi;
-      ul[k] = __builtin_bit_cast(
-          uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(half_lo(hi), -1.0f, e[2 * k]), fmaf(half_hi(hi), -1.0f, e[2 * k + 1])));
-    }
-    p.hi = __builtin_bit_cast(h8, uh);
-    p.lo = __builtin_bit_cast(h8, ul);
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(e[2 * k], e[2 * k + 1]));
+    uh[k] = hi;
+    ul[k] = __builtin_bit_cast(
+        uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(half_lo(hi), -1.0f, e[2 * k]), fmaf(half_hi(hi), -1.0f, e[2 * k + 1])));
   }
-  return p;
+  return {__builtin_bit_cast(h8, uh), __builtin_bit_cast(h8, ul)};
 }
 
 // A page's scores are dot * score_scale + ev, with q negated where the scale of
@@ -439,7 +429,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
     }
     const float rel = ev - ((m == ninf ? 0.0f : m) - kLift);
     float sum[2] = {0.0f, 0.0f};
-    Probs<BF16> p[2];
+    Probs p[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float e[8];
@@ -448,7 +438,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
         e[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + j], ksc, rel));
         sum[h] += e[j];
       }
-      p[h] = to_probs<BF16>(e);
+      p[h] = to_probs(e);
     }
     l = fmaf(sum[0] + sum[1], ldexp2(1.0f, -(int)ev), l);
     // places behind the row's end hold whatever their page held before
@@ -469,7 +459,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
       for (int h = 0; h < 2; ++h) {
         const h8 vf = widen8(vr[d][2 * h], vr[d][2 * h + 1]);
         o[d] = mfma16(vf, p[h].hi, o[d]);
-        if (!BF16) o[d] = mfma16(vf, p[h].lo, o[d]);
+        o[d] = mfma16(vf, p[h].lo, o[d]);
       }
     __builtin_amdgcn_sched_barrier(0);
     load8(vr, rn, kHalfBlock);
@@ -565,10 +555,11 @@ __device__ __forceinline__ int v_lds(int d, int c) { return kVLds + d * 128 + 16
 // The next page's staging stands between the products of the scores, and a
 // fragment's exponentials between the products of the fragment before.  What
 // bounds it: matrix cores, vector unit and LDS are busy about half the time each,
-// and two waves a SIMD overlap little more than that by chance: 5000 tokens 239
-// us in fp16 and 235 in bf16 (865 TFLOP/s); of 249, before k's conflicts went, the
-// exponentials alone made 38, staging 35, the fragments' reads 55, the products
-// 68.  Tried without gain: fragments read three steps ahead; raised priority around
+// and two waves a SIMD overlap little more than that by chance: a call of 5000
+// tokens 292 us in fp16 and 289 in bf16 (700 TFLOP/s).  With one fp16 part of a
+// probability, of 249 us before k's conflicts went, the exponentials alone made
+// 38, staging 35, the fragments' reads 55, the products 68, and there was tried
+// without gain: fragments read three steps ahead; raised priority around
 // the products; one wave a SIMD with 64 rows and the next page's scores between
 // this one's exponentials, whose accumulators in AGPRs cost more copies than the
 // shared fragments save (326 us in bf16); the same with 32 rows, which spilled
@@ -739,20 +730,21 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
         sum[f] += e[j];
       }
     };
-    h8 p;
+    Probs p;
     exps(0, 0, 8);
-    p = to_probs<true>(e).hi;
+    p = to_probs(e);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         if (4 * f + d < 13) read_v(va, 4 * f + d + 3);
-        o[d] = mfma32(vf[d], p, o[d]);
+        o[d] = mfma32(vf[d], p.hi, o[d]);
+        o[d] = mfma32(vf[d], p.lo, o[d]);
         if (f < 3) exps(f + 1, 2 * d, 2 * d + 2);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (f < 3) p = to_probs<true>(e).hi;
+      if (f < 3) p = to_probs(e);
     }
     l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ldexp2(1.0f, -(int)ev), l);
   };

@@ -558,10 +558,8 @@ size_t oi2_kv_attend_workspace_bytes(const oi2_paged* c, int32_t max_tokens, int
  *   out = softmax(scale q k^T) v,  k and v the codes times their scales
  * q (n_tokens, n_q, 128) with strides, out (n_tokens, n_q, 128) dense, both of
  * `dtype` (OI2_DTYPE_F16 or _BF16).  Scores, the softmax's sums and the output
- * are fp32 until the one rounding of out; probabilities enter the products
- * rounded to fp16, and as two fp16 parts where out is fp16 and the row has at
- * most 16 / (n_q / n_kv) tokens in the step.  The tokens of a rejected row give
- * zeros; rows of out past the step's last token are left as they were.
+ * are fp32 until the one rounding of out; probabilities enter the products as
+ * two fp16 parts.  The tokens of a rejected row give zeros; rows of out past the step's last token are left as they were.
  * n_tokens below the step's: its first tokens alone. */
 int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
                   const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes,

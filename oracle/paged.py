@@ -134,9 +134,8 @@ class Cache:
     def attend(self, q, plan, scale, one_part=False):
         """(out, bound): out (tokens, n_q, 128) float64, zeros for rejected rows;
         bound is what sum p |v| and the scores' error give: per output, the
-        absolute error of fp32 sums (see attend_bound).  one_part: all rows'
-        probabilities go in one fp16 part; rows of more than 16 query rows' do
-        anyway."""
+        absolute error of fp32 sums (see attend_bound).  one_part: where
+        probabilities may go in one fp16 part instead of two."""
         n_q = q.shape[1]
         group = n_q // self.n_kv
         out = np.zeros((plan["cu"][-1], n_q, D))
@@ -161,7 +160,7 @@ class Cache:
                     y = p @ np.where(nan, 0.0, vv)
                     y[((~hide).astype(float) @ nan.astype(float)) > 0] = np.nan
                 out[t0:t0 + n, h] = y
-                bound[t0:t0 + n, h] = attend_bound(mag.max(1), np.abs(np.where(hide, 0, s)).max(1), now, one_part or n * group > 16)[:, None] * (p @ np.abs(np.where(nan, 0.0, vv)))
+                bound[t0:t0 + n, h] = attend_bound(mag.max(1), np.abs(np.where(hide, 0, s)).max(1), now, one_part)[:, None] * (p @ np.abs(np.where(nan, 0.0, vv)))
         return out, bound
 
 

@@ -1,0 +1,69 @@
+"""What the paged attention keeps of its inputs' bits.
+
+Every bar is half a step of the output's type and the oracle's bound for fp32
+sums and two fp16 parts of a probability (attend_bound, one_part=False),
+whatever the type and the number of query rows.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as P
+from tests.test_gpu_paged import _check_attend, _extend, _np, _pair, dev  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+D = 128
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def _step(dev, n_q, n_kv, past, new, k, v, dtype):
+    """Caches holding past positions and then the step's, of k and v (past + new
+    positions a row, n_kv, 128) row after row; the plan of the step."""
+    total = [a + b for a, b in zip(past, new)]
+    c, o = _pair(n_kv, len(past), max(total), sum(P.pages_of(t) for t in total), dev, n_q=n_q, shuffle=1)
+    at = np.cumsum([0] + total)
+    for lens, lo in ((past, [0] * len(past)), (new, past)):
+        plan = c.new_plan(max(sum(lens), 1), max_new=max(max(lens), 1))
+        ref = _extend(c, o, plan, lens)
+        rows = torch.tensor([at[i] + lo[i] + t for i, n in enumerate(lens) for t in range(n)], device=dev, dtype=torch.long)
+        if len(rows):
+            c.append(0, k[rows], v[rows], plan)
+            o.append(_np(k[rows]), _np(v[rows]), ref)
+    return c, o, plan, ref
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("past,new", [([3, 6, 1], [1, 1, 1]), ([2, 0], [2, 4]), ([0], [40]), ([0, 2], [200, 30]), ([1200], [33])])
+def test_values_that_cancel(dev, dtype, past, new):
+    """Nearly even weights on values 1 and -1: the result is the weights'
+    difference, and shows what they were rounded to."""
+    print(f"[cancel] {dtype} {past} {new}", flush=True)
+    g = torch.Generator(device=dev).manual_seed(2)
+    n_q, n_kv, n = 16, 4, sum(past) + sum(new)
+    k = (torch.randn((n, n_kv, D), generator=g, device=dev) * 0.25).to(dtype)
+    sign = 1.0 - 2.0 * (torch.arange(n, device=dev) % 2)
+    v = (sign[:, None, None] * torch.ones((n, n_kv, D), device=dev)).to(dtype)
+    c, o, plan, ref = _step(dev, n_q, n_kv, past, new, k, v, dtype)
+    q = torch.randn((sum(new), n_q, D), generator=g, device=dev).to(dtype)
+    want, bound = o.attend(_np(q), ref, D ** -0.5)
+    _check_attend(c.attend(0, q, plan), want, bound, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_token_has_its_result_whatever_step_it_comes_in(dev, dtype):
+    """Rows of a prompt against the same tokens in steps of one and of four, over
+    the same cache: off by no more than two results of the same formula may be."""
+    print(f"[steps] {dtype}", flush=True)
+    g = torch.Generator(device=dev).manual_seed(4)
+    n_q, n_kv, n = 8, 2, 90
+    k, v = (torch.randn((n, n_kv, D), generator=g, device=dev).to(dtype) for _ in range(2))
+    q = torch.randn((n, n_q, D), generator=g, device=dev).to(dtype)
+    c, o, plan, ref = _step(dev, n_q, n_kv, [0], [n], k, v, dtype)
+    whole = c.attend(0, q, plan)
+    want, bound = o.attend(_np(q), ref, D ** -0.5)
+    _check_attend(whole, want, bound, dtype)
+    for t0, size in ((89, 1), (86, 4), (70, 1), (64, 4)):
+        c.rewind([t0])
+        p = c.extend([size], c.new_plan(size))
+        y = c.attend(0, q[t0:t0 + size], p)       # the codes are still there
+        _check_attend(y, want[t0:t0 + size], bound[t0:t0 + size], dtype)
