@@ -108,8 +108,9 @@ __device__ __forceinline__ void take_nans(u32x4& x, int pos, int* first) {   // 
 __device__ __forceinline__ float ldexp2(float x, int e) { return __builtin_ldexpf(x, e); }
 
 // Eight consecutive q values as fp16 times 2^-e (bf16; fp16 comes as it is).
-// A row of bf16 values over its largest one's power of two is exact in fp16 but
-// for what lies 2^-24 below that one.
+// The largest of a bf16 row is put at the top of fp16's range, at 2^15: every
+// value down to 2^-29 of it is exact, smaller ones are off by 2^-40 of it.
+constexpr int kTopExp = 15;
 template <bool BF16>
 __device__ __forceinline__ h8 q_frag(const uint16_t (&v)[8], int e, bool negate) {
   h8 r;
@@ -346,7 +347,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(bf16_bits_to_float(qv[i][e])));
     top = quad_max(top);
-    qe = min(max((int)(as_u32(top) >> 23) - 127, -126), 126);
+    qe = min(max((int)(as_u32(top) >> 23) - 127 - kTopExp, -126), 126);
   }
   h8 qf[4];
 #pragma unroll
@@ -609,7 +610,7 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(bf16_bits_to_float(qv[st][e])));
       top = fmaxf(top, __shfl_xor(top, 32));
-      qe = min(max((int)(as_u32(top) >> 23) - 127, -126), 126);
+      qe = min(max((int)(as_u32(top) >> 23) - 127 - kTopExp, -126), 126);
     }
 #pragma unroll
     for (int st = 0; st < 8; ++st) qf[st] = q_frag<BF16>(qv[st], qe, a.scale < 0.0f);

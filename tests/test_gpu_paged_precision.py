@@ -49,6 +49,28 @@ def test_values_that_cancel(dev, dtype, past, new):
     _check_attend(c.attend(0, q, plan), want, bound, dtype)
 
 
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_small_values_beside_large_ones_in_bf16_queries(dev, new):
+    """A query's largest value meets keys of 0; the scores come from one 2^-18
+    and one 2^-27 times as large, whose eight bits all count."""
+    print(f"[bf16 query] {new}", flush=True)
+    g = torch.Generator(device=dev).manual_seed(3)
+    n_q, n_kv, past = 8, 2, 100
+    n = past + new
+    for small in (18, 27):
+        k = torch.zeros((n, n_kv, D), device=dev)
+        k[:, :, 1] = torch.randint(-7, 8, (n, n_kv), generator=g, device=dev) * 64.0
+        v = torch.randn((n, n_kv, D), generator=g, device=dev).bfloat16()
+        c, o, plan, ref = _step(dev, n_q, n_kv, [past], [new], k.bfloat16(), v, torch.bfloat16)
+        q = torch.zeros((new, n_q, D), device=dev)
+        q[..., 0] = 1.5
+        q[..., 1] = (1 + torch.randint(0, 128, (new, n_q), generator=g, device=dev) / 128) * 2.0 ** -small
+        q = q.bfloat16()
+        scale = 2.0 ** (small - 8)
+        want, bound = o.attend(_np(q), ref, scale)
+        _check_attend(c.attend(0, q, plan, scale=scale), want, bound, torch.bfloat16)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_a_token_has_its_result_whatever_step_it_comes_in(dev, dtype):
     """Rows of a prompt against the same tokens in steps of one and of four, over
