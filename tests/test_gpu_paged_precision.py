@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+import oi2
 from oracle import paged as P
 from tests.test_gpu_paged import _check_attend, _extend, _np, _pair, dev  # noqa: F401
 
@@ -89,3 +90,34 @@ def test_a_token_has_its_result_whatever_step_it_comes_in(dev, dtype):
         p = c.extend([size], c.new_plan(size))
         y = c.attend(0, q[t0:t0 + size], p)       # the codes are still there
         _check_attend(y, want[t0:t0 + size], bound[t0:t0 + size], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("past,new", [(100000, 4096), (40000, 1)])
+def test_many_small_weights_behind_a_large_one(dev, dtype, past, new):
+    """One position 2^22 to 2^30 times as heavy as each of the others, whose
+    values differ from its own: the others count together.  Where a workgroup
+    has all of a row's pages (16 heads of 4096 tokens), a wave cuts every one of
+    their weights; a weight's two parts end 2^-30 below the largest one."""
+    print(f"[small weights] {dtype} {past} + {new}", flush=True)
+    heads = 16
+    k = torch.zeros((past, heads, D), device=dev, dtype=dtype)
+    v = torch.ones_like(k)
+    k[0, :, 0], v[0] = 1.0, -1.0
+    c = oi2.PagedKVCache(1, heads, heads, 1, past + new, P.pages_of(past + new), device=dev)
+    c.append(0, k, v, c.extend([past], c.new_plan(past)))
+    plan = c.extend([new], c.new_plan(new))
+    c.append(0, torch.zeros((new, heads, D), device=dev, dtype=dtype), torch.ones((new, heads, D), device=dev, dtype=dtype), plan)
+    q = torch.zeros((new, heads, D), device=dev, dtype=dtype)
+    for bits in (22, 24, 25, 25.5, 26, 26.5, 27, 28, 30):
+        q[:, :, 0] = bits * np.log(2)
+        gap = q[0, 0, 0].item()
+        y = _np(c.attend(0, q, plan, scale=1.0)[[0, -1]])
+        for t, out in ((0, y[0]), (new - 1, y[1])):
+            w = (past + t) * np.exp(-gap)
+            want = (w - 1) / (w + 1)
+            # half a step; the cut, of every weight; fp32: a score of up to 44 in
+            # powers of two, 2^-18, and an exponential's and a sum's few steps
+            # of the small weights
+            tol = torch.finfo(dtype).eps / 2 * abs(want) + (past + t) * 2.0 ** -30 + 2 * w * 2.0 ** -17
+            assert np.abs(out - want).max() <= tol, (bits, t, np.abs(out - want).max() / tol)
