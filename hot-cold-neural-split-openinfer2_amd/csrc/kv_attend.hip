@@ -42,7 +42,7 @@ constexpr float kLift = 6.0f, kSlack = 9.0f;
 struct PartArgs {             // of one of the two kernels
   const AttendItem* items;
   int groups;                 // workgroups of the launch
-  int32_t* count;             // (slot, kv head) arrivals, zero between calls
+  int32_t* count;             // (slot, kv head) arrivals, zero before the launch
   float* o;                   // (slot, kv head, rows, 128)
   float* ml;                  // (slot, kv head, rows, 2)
 };
@@ -175,7 +175,6 @@ __device__ __forceinline__ bool arrive(const PartArgs& pa, const ItemHead& it, i
     int32_t* c = pa.count + (int64_t)it.slot0 * n_kv + g;
     const int old = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s_last = old + 1 == it.n_parts;
-    if (s_last) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
   }
   __syncthreads();
   return s_last;
@@ -840,9 +839,20 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendArgs a) {
   else attend_few<BF16>(a, b - a.many.groups, smem);
 }
 
-// The workspace: the partial sums of either kernel's parts, out and then m, l.
+// Arrivals of the parts: in the workspace, which is the call's own, and cleared
+// by the call, so that calls of one plan (other layers, other queries) may run
+// at the same time.
+__global__ __launch_bounds__(1024) void k_clear(int32_t* count, int n) {
+  const int i = blockIdx.x * 1024 + threadIdx.x;
+  if (i < n) count[i] = 0;
+}
+
+// The workspace: the partial sums of either kernel's parts, out and then m, l;
+// the parts' counters.
 size_t few_floats(const PlanLayout& l, int n_kv) { return (size_t)l.cap_parts_few * n_kv * kFewRows * (kHeadD + 2); }
 size_t many_floats(const PlanLayout& l, int n_kv) { return (size_t)l.cap_parts_many * n_kv * kManyRows * (kHeadD + 2); }
+size_t counters(const PlanLayout& l, int n_kv) { return (size_t)(l.cap_parts_few + l.cap_parts_many) * n_kv; }
+size_t attend_bytes(const PlanLayout& l, int n_kv) { return (few_floats(l, n_kv) + many_floats(l, n_kv) + counters(l, n_kv)) * 4; }
 
 }  // namespace
 }  // namespace oi2
@@ -854,7 +864,7 @@ extern "C" {
 size_t oi2_kv_attend_workspace_bytes(const oi2_paged* c, int32_t max_tokens, int32_t max_new) {
   if (!oi2_page_plan_bytes(c, max_tokens, max_new)) return 0;
   const PlanLayout l = plan_layout(*c, max_tokens, max_new);
-  const size_t n = (few_floats(l, c->n_kv) + many_floats(l, c->n_kv)) * 4;
+  const size_t n = attend_bytes(l, c->n_kv);
   return n ? n : 16;
 }
 
@@ -872,7 +882,7 @@ int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int
   OI2_CHECK_ARG(q->data && (uintptr_t)q->data % 2 == 0, "q must be non-null and 2-byte aligned");
   OI2_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "out must be non-null and 16-byte aligned");
   const PlanLayout l = plan_layout(*c, p->max_tokens, p->max_new), now = plan_layout(*c, n_tokens, p->max_new);
-  const size_t need = (few_floats(l, c->n_kv) + many_floats(l, c->n_kv)) * 4;
+  const size_t need = attend_bytes(l, c->n_kv);
   OI2_CHECK_ARG(!need || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
                 "workspace of %zu bytes, %zu needed, 16-byte aligned", workspace_bytes, need);
   AttendArgs a{};
@@ -899,14 +909,19 @@ int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int
   OI2_CHECK_ARG(few + many < 1 << 23, "%d tokens are too many for one call", n_tokens);
   a.few.items = reinterpret_cast<const AttendItem*>(p->work + l.few);
   a.few.groups = (int)few;
-  a.few.count = p->work + l.count_few;
   a.few.o = (float*)workspace;
   a.few.ml = a.few.o + (size_t)l.cap_parts_few * c->n_kv * kFewRows * kHeadD;
   a.many.items = reinterpret_cast<const AttendItem*>(p->work + l.many);
   a.many.groups = (int)many;
-  a.many.count = p->work + l.count_many;
   a.many.o = a.few.o + few_floats(l, c->n_kv);
   a.many.ml = a.many.o + (size_t)l.cap_parts_many * c->n_kv * kManyRows * kHeadD;
+  a.few.count = (int32_t*)(a.few.o + few_floats(l, c->n_kv) + many_floats(l, c->n_kv));
+  a.many.count = a.few.count + (size_t)l.cap_parts_few * c->n_kv;
+  if (need) {
+    const int n = (int)counters(l, c->n_kv);
+    hipLaunchKernelGGL(k_clear, dim3((n + 1023) / 1024), dim3(1024), 0, st, a.few.count, n);
+    OI2_CHECK_LAUNCH();
+  }
   const dim3 grid((uint32_t)(few + many)), block(kThreads);
   if (many && bf) hipLaunchKernelGGL(k_attend<true>, grid, block, 0, st, a);
   else if (many) hipLaunchKernelGGL(k_attend<false>, grid, block, 0, st, a);

@@ -47,7 +47,7 @@ struct PlanLayout {           // offsets in ints into oi2_page_plan.work
   int32_t cap_append, cap_few, cap_many, cap_parts_few, cap_parts_many;
   int32_t few_tokens, many_tokens;        // tokens of a workgroup
   int32_t parts_few, parts_many;          // parts per kv head that the work is cut for
-  int64_t append, few, many, count_few, count_many, ints;   // count: arrivals of the parts of (slot0, kv head)
+  int64_t append, few, many, ints;
 };
 // counts at the head of the work lists
 enum { kNAppend = 0, kNFew, kNMany, kHeadInts = 16 };
@@ -80,9 +80,7 @@ inline PlanLayout plan_layout(const oi2_paged& c, int32_t n_tokens, int32_t max_
   l.append = kHeadInts;
   l.few = l.append + 4 * (int64_t)l.cap_append;
   l.many = l.few + kItemInts * (int64_t)l.cap_few;
-  l.count_few = l.many + kItemInts * (int64_t)l.cap_many;
-  l.count_many = l.count_few + (int64_t)l.cap_parts_few * c.n_kv;
-  l.ints = l.count_many + (int64_t)l.cap_parts_many * c.n_kv;
+  l.ints = l.many + kItemInts * (int64_t)l.cap_many;
   return l;
 }
 

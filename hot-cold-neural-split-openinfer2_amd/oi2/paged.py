@@ -15,8 +15,10 @@ work lists live on the GPU and nothing waits on the host, so a step can be
 captured into a graph.  ``rewind`` cuts rows back: rejected drafts, or the end
 of a sequence.
 
-Calls on one cache write its tables and pages: they have to be ordered, on one
-stream or by events.
+``extend``, ``rewind`` and ``append`` on one cache write its tables and pages:
+they, and what reads the cache, have to be ordered, on one stream or by events.
+``attend`` only reads: of one step, for several layers or queries, it may run on
+several streams at once.
 """
 from __future__ import annotations
 
@@ -120,7 +122,7 @@ class PagedKVCache:
     def new_plan(self, max_tokens: int, max_new: int | None = None) -> PagePlan:
         """Room for the layout of steps of up to max_tokens tokens, max_new of
         one row (max_tokens by default).  A plan belongs to its cache and serves
-        one step, and one attend, at a time.  Decoding steps want max_new as small as it is:
+        one step at a time.  Decoding steps want max_new as small as it is:
         attention then leaves out its kernel for many rows."""
         return PagePlan(self, max_tokens, max_new)
 

@@ -481,9 +481,8 @@ typedef struct oi2_page_plan {
   int32_t* kv_len;            /* (n_seqs) positions of the row with the step's; 0: rejected */
   int32_t* rejected;          /* (n_seqs) 1 where the row could not grow */
   int32_t* work;              /* oi2_page_plan_bytes bytes, 16-byte aligned, zeroed
-                                 before the first use: work lists, and counters
-                                 that every oi2_kv_attend leaves at zero.  So a
-                                 plan serves one attention at a time. */
+                                 before the first use: work lists, which
+                                 oi2_page_extend alone writes */
 } oi2_page_plan;
 
 /* Bytes of a plan's work lists; 0 for sizes that are not supported. */
@@ -549,7 +548,8 @@ int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int
                   void* stream);
 
 /* Workspace bytes of oi2_kv_attend over a plan of these sizes: the partial
- * sums of rows whose pages are cut into parts. */
+ * sums of rows whose pages are cut into parts.  Its contents on entry do not
+ * matter; calls that may run at the same time need one each. */
 size_t oi2_kv_attend_workspace_bytes(const oi2_paged* c, int32_t max_tokens, int32_t max_new);
 
 /* Attention of the plan's tokens (engine.py:110-122, causal) over the pages of
