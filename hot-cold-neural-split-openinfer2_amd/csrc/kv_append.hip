@@ -460,6 +460,8 @@ extern "C" int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t
   clear_error();
   if (int rc = check_paged(c, layer, true)) return rc;
   if (int rc = check_plan(c, p)) return rc;
+  const bool zero = dtype & OI2_ZERO_LEFT_OUT;
+  dtype &= ~OI2_ZERO_LEFT_OUT;
   OI2_CHECK_ARG(dtype == OI2_DTYPE_F16 || dtype == OI2_DTYPE_BF16, "dtype %d: fp16 or bf16", dtype);
   OI2_CHECK_ARG(n_tokens >= 0 && n_tokens <= p->max_tokens, "%d tokens in a plan of %d", n_tokens, p->max_tokens);
   OI2_CHECK_ARG(k && v && k->heads == c->n_kv && v->heads == c->n_kv, "k and v need the cache's %d heads", c->n_kv);
@@ -502,7 +504,7 @@ extern "C" int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t
   bool wide = true;
   a.rotate = r ? 1 : 0;
   if (r) {
-    rotary_describe(a.rope, r, n_tokens, p->positions);
+    rotary_describe(a.rope, r, n_tokens, p->positions, zero);
     wide = rotary_fill(a.rope, q, q_out, nullptr, nullptr);
     rows = rotary_workgroups(a.rope);
   }

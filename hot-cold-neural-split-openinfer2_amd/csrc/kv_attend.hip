@@ -59,6 +59,8 @@ struct AttendArgs {
   int wide;                   // 16-byte loads of q
   float scale;                // of the scores, times log2 e
   uint16_t* out;
+  const int32_t* total;       // tokens of the step
+  int zero_groups;            // workgroups for the rows past them, or none
 };
 
 __device__ __forceinline__ h8 widen8(uint32_t d0, uint32_t d1) {
@@ -822,12 +824,22 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
     }
 }
 
+// Zeros for the rows past the step's last token.
+__device__ __forceinline__ void zero_rest(const AttendArgs& a, int b) {
+  const int row = a.n_q * (kHeadD / 8);    // 16-byte vectors of a token
+  u32x4* out = reinterpret_cast<u32x4*>(a.out);
+  for (int t = max(scalar_load(a.total), 0) + b; t < a.n_tokens; t += a.zero_groups)
+    for (int i = threadIdx.x; i < row; i += kThreads) out[(int64_t)t * row + i] = u32x4{0, 0, 0, 0};
+}
+
 // Steps whose rows all have few query rows, and steps with rows of either kind:
 // the long tiles first, the others fill the chip behind and beside them.
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void k_attend_few(AttendArgs a) {
   __shared__ __align__(16) uint8_t smem[kFewLds];
-  attend_few<BF16>(a, blockIdx.x, smem);
+  const int b = blockIdx.x;
+  if (b < a.few.groups) attend_few<BF16>(a, b, smem);
+  else zero_rest(a, b - a.few.groups);
 }
 
 template <bool BF16>
@@ -836,7 +848,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendArgs a) {
   __shared__ __align__(1024) uint8_t smem[kManyLds];
   const int b = blockIdx.x;
   if (b < a.many.groups) attend_many<BF16>(a, b, smem);
-  else attend_few<BF16>(a, b - a.many.groups, smem);
+  else if (b - a.many.groups < a.few.groups) attend_few<BF16>(a, b - a.many.groups, smem);
+  else zero_rest(a, b - a.many.groups - a.few.groups);
 }
 
 // Arrivals of the parts: in the workspace, which is the call's own, and cleared
@@ -874,6 +887,8 @@ int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int
   clear_error();
   if (int rc = check_paged(c, layer, true)) return rc;
   if (int rc = check_plan(c, p)) return rc;
+  const bool zero = dtype & OI2_ZERO_LEFT_OUT;
+  dtype &= ~OI2_ZERO_LEFT_OUT;
   OI2_CHECK_ARG(dtype == OI2_DTYPE_F16 || dtype == OI2_DTYPE_BF16, "dtype %d: fp16 or bf16", dtype);
   OI2_CHECK_ARG(n_tokens >= 0 && n_tokens <= p->max_tokens, "%d tokens in a plan of %d", n_tokens, p->max_tokens);
   OI2_CHECK_ARG(q && q->heads == c->n_q, "q needs the cache's %d query heads", c->n_q);
@@ -922,7 +937,9 @@ int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int
     hipLaunchKernelGGL(k_clear, dim3((n + 1023) / 1024), dim3(1024), 0, st, a.few.count, n);
     OI2_CHECK_LAUNCH();
   }
-  const dim3 grid((uint32_t)(few + many)), block(kThreads);
+  a.total = p->cu + c->n_seqs;
+  a.zero_groups = zero ? (n_tokens < 128 ? n_tokens : 128) : 0;
+  const dim3 grid((uint32_t)(few + many + a.zero_groups)), block(kThreads);
   if (many && bf) hipLaunchKernelGGL(k_attend<true>, grid, block, 0, st, a);
   else if (many) hipLaunchKernelGGL(k_attend<false>, grid, block, 0, st, a);
   else if (bf) hipLaunchKernelGGL(k_attend_few<true>, grid, block, 0, st, a);

@@ -80,6 +80,7 @@ struct RotaryArgs {
   int heads[2];
   int per_head;               // threads of a head
   int tokens_each;            // tokens of a workgroup
+  int zero;                   // tokens at negative positions get zeros
 };
 
 // Cosines and sines of a workgroup's tokens: kTurns at most.
@@ -155,7 +156,12 @@ __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int b) {
         }
       }
     }
-    if (s_pos[t] >= 0) {
+    const bool left_out = s_pos[t] < 0;
+    if (left_out) {
+#pragma unroll
+      for (int e = 0; e < 2 * P; ++e) v[e] = 0;
+    }
+    if (!left_out || a.zero) {
       const int w = h >= a.heads[0];
       uint16_t* p = (w ? a.dst[1] : a.dst[0]) + ((int64_t)(t0 + t) * (w ? a.heads[1] : a.heads[0]) + (w ? h - a.heads[0] : h)) * a.head_dim;
       if constexpr (WIDE) {
@@ -173,7 +179,7 @@ __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int b) {
   }
 }
 
-inline void rotary_describe(RotaryArgs& a, const oi2_rotary* r, int n_tokens, const int32_t* positions) {
+inline void rotary_describe(RotaryArgs& a, const oi2_rotary* r, int n_tokens, const int32_t* positions, bool zero) {
   a.freq = r->freq;
   a.positions = positions;
   a.magnitude = r->magnitude;
@@ -181,6 +187,7 @@ inline void rotary_describe(RotaryArgs& a, const oi2_rotary* r, int n_tokens, co
   a.head_dim = r->head_dim;
   a.rot = r->rotary_dim;
   a.interleaved = r->interleaved ? 1 : 0;
+  a.zero = zero ? 1 : 0;
 }
 
 // The tensors, how the work is cut, and whether the wide form serves them.

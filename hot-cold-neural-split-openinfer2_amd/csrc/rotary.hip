@@ -33,6 +33,8 @@ extern "C" int oi2_rotary_apply(const oi2_rotary* r, int32_t dtype, int32_t n_to
                                 const oi2_heads* q, void* q_out, const oi2_heads* k, void* k_out, void* stream) {
   clear_error();
   if (int rc = check_rotary(r)) return rc;
+  const bool zero = dtype & OI2_ZERO_LEFT_OUT;
+  dtype &= ~OI2_ZERO_LEFT_OUT;
   OI2_CHECK_ARG(dtype == OI2_DTYPE_F16 || dtype == OI2_DTYPE_BF16, "dtype %d: fp16 or bf16", dtype);
   OI2_CHECK_ARG(n_tokens >= 0, "%d tokens", n_tokens);
   OI2_CHECK_ARG(q && k && q->heads >= 0 && k->heads >= 0 && q->heads <= 1 << 16 && k->heads <= 1 << 16, "null q or k, or heads out of range");
@@ -40,7 +42,7 @@ extern "C" int oi2_rotary_apply(const oi2_rotary* r, int32_t dtype, int32_t n_to
   OI2_CHECK_ARG((!q->heads || (q->data && q_out)) && (!k->heads || (k->data && k_out)), "null q or k data");
   OI2_CHECK_ARG(positions, "null positions");
   RotaryArgs a{};
-  rotary_describe(a, r, n_tokens, positions);
+  rotary_describe(a, r, n_tokens, positions, zero);
   const bool wide = rotary_fill(a, q, q_out, k, k_out);
   for (int w = 0; w < 2; ++w)
     OI2_CHECK_ARG(!a.heads[w] || ((uintptr_t)a.src[w] % 2 == 0 && (uintptr_t)a.dst[w] % 2 == 0), "q and k must be 2-byte aligned");

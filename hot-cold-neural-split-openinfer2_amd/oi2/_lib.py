@@ -18,6 +18,7 @@ OI2_OK = 0
 OI2_EUNSUPPORTED = 4
 ACT_SILU, ACT_RELU = 0, 1
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+ZERO_LEFT_OUT = 0x100       # with a dtype: rows of tokens without a position get zeros
 ABI_VERSION = 2
 HIDDEN = 4096
 SEL_CHUNK = 256

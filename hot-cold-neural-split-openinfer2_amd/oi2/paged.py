@@ -190,8 +190,9 @@ class PagedKVCache:
         """k and v (tokens, n_kv, 128) of the step, fp16 or bf16 with any
         strides, into the layer's pages.  With ``rotary`` k is rotated first, to
         the bits that ``rotary`` itself gives, and so is q (tokens, heads, 128)
-        if given; returns the rotated q, else None.  Tokens of rejected rows are
-        left out, in q's output too.  Each layer takes a step once: what a page
+        if given; returns the rotated q, else None.  Tokens of rejected rows and
+        past the step's last one are left out: their rows of q_out are not
+        written, those of a new q are 0.  Each layer takes a step once: what a page
         holds is coded again when its scale grows."""
         plan, layer = self._plan(plan), self._layer(layer)
         k, hk = self._rows(k, self.n_kv, "k")
@@ -204,6 +205,7 @@ class PagedKVCache:
             raise ValueError(f"a rotary of head_dim {HEAD_DIM} on {self.device}, got {rotary.head_dim} on {rotary.device}")
         if q is not None:
             q, hq = self._rows(q, q.shape[1] if q.dim() == 3 else self.n_q, "q", k)
+            new = q_out is None
             q_out = rotary._output(q_out, q, "q_out")
             if q_out.data_ptr() == q.data_ptr() and not q.is_contiguous():
                 raise ValueError("an output that is its own input must be contiguous")
@@ -212,7 +214,7 @@ class PagedKVCache:
         L = _lib.load_library()
         with _lib.on_device(self.device) as stream:
             _lib.check(L.oi2_kv_append(
-                self._ref, plan._ref, layer, _lib.dtype_code(k.dtype), n,
+                self._ref, plan._ref, layer, _lib.dtype_code(k.dtype) | (_lib.ZERO_LEFT_OUT if q is not None and new else 0), n,
                 ctypes.byref(hk), ctypes.byref(hv),
                 None if rotary is None else rotary._ref,
                 None if q is None else ctypes.byref(hq), _lib.ptr(q_out), stream))
@@ -225,12 +227,14 @@ class PagedKVCache:
         [0, t] of it.  q (tokens, n_q, 128) fp16 or bf16 with any strides;
         ``scale`` of the scores 1 / sqrt(128) by default.  Returns (tokens, n_q,
         128) like q: zeros for the tokens of rejected rows; rows past the step's
-        last token are not written."""
+        last token are 0 in a new tensor, and not written in ``out``."""
         plan, layer = self._plan(plan), self._layer(layer)
         q, hq = self._rows(q, self.n_q, "q")
         n = self._tokens(q, plan)
+        dtype = _lib.dtype_code(q.dtype)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            dtype |= _lib.ZERO_LEFT_OUT
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor like q")
         L = _lib.load_library()
@@ -238,7 +242,7 @@ class PagedKVCache:
         with _lib.on_device(self.device) as stream:
             ws = q.new_empty((nbytes,), dtype=torch.uint8)
             _lib.check(L.oi2_kv_attend(
-                self._ref, plan._ref, layer, _lib.dtype_code(q.dtype), n,
+                self._ref, plan._ref, layer, dtype, n,
                 ctypes.byref(hq), HEAD_DIM ** -0.5 if scale is None else float(scale), out.data_ptr(),
                 ws.data_ptr(), nbytes, stream))
         return out

@@ -121,9 +121,9 @@ class Rotary:
             raise ValueError(f"{what} on {x.device}, the rotary frequencies on {self.device}")
         return _lib.heads(x, shape[1])
 
-    def _output(self, out, x: torch.Tensor, what: str) -> torch.Tensor:
+    def _output(self, out, x: torch.Tensor, what: str, zeros: bool = False) -> torch.Tensor:
         if out is None:
-            return torch.empty_like(x, memory_format=torch.contiguous_format)
+            return (torch.zeros_like if zeros else torch.empty_like)(x, memory_format=torch.contiguous_format)
         if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
             raise ValueError(f"{what} must be a contiguous tensor like its input")
         return out
@@ -132,7 +132,8 @@ class Rotary:
         """(q, k) rotated: q (tokens, n_q, head_dim), k (tokens, n_kv, head_dim)
         or None, fp16 or bf16, any strides; positions (tokens) int32.  q_out and
         k_out: contiguous outputs, which may be the inputs themselves.  A token
-        at a negative position is left out: its output rows are not written."""
+        at a negative position is left out: its rows of these are not written,
+        those of new outputs are 0."""
         q, hq = self._rows(q, "q")
         N = q.shape[0]
         hk = _lib.Heads()
@@ -143,15 +144,16 @@ class Rotary:
         if positions.shape != (N,) or positions.dtype != torch.int32 or positions.device != self.device:
             raise ValueError(f"positions: ({N},) int32 on {self.device}, got {tuple(positions.shape)} "
                              f"{positions.dtype} on {positions.device}")
-        qo = self._output(q_out, q, "q_out")
-        ko = None if k is None else self._output(k_out, k, "k_out")
+        new = q_out is None and (k is None or k_out is None)
+        qo = self._output(q_out, q, "q_out", not new)
+        ko = None if k is None else self._output(k_out, k, "k_out", not new)
         for x, o in ((q, qo), (k, ko)):
             if x is not None and o.data_ptr() == x.data_ptr() and not x.is_contiguous():
                 raise ValueError("an output that is its own input must be contiguous")
         L = _lib.load_library()
         with _lib.on_device(self.device) as stream:
             _lib.check(L.oi2_rotary_apply(
-                self._ref, _lib.dtype_code(q.dtype), N, positions.contiguous().data_ptr(),
+                self._ref, _lib.dtype_code(q.dtype) | (_lib.ZERO_LEFT_OUT if new else 0), N, positions.contiguous().data_ptr(),
                 ctypes.byref(hq), qo.data_ptr(),
                 ctypes.byref(hk), _lib.ptr(ko),
                 stream))

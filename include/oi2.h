@@ -529,6 +529,11 @@ typedef struct oi2_heads {
   int64_t head_stride;
 } oi2_heads;
 
+/* Added to the dtype of oi2_rotary_apply, oi2_kv_append (q_out) and
+ * oi2_kv_attend: output rows that the call leaves as they were, of tokens that
+ * have no position, get zeros instead, as new memory wants. */
+enum { OI2_ZERO_LEFT_OUT = 0x100 };
+
 /* The rotary positions of q and k (either may have no heads) of n_tokens
  * tokens at positions (device memory): the arithmetic of engine.py:140-157
  * with each token at its own position, in fp64.  q_out and k_out are dense
