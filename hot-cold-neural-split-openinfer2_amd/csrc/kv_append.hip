@@ -509,6 +509,9 @@ extern "C" int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t
     rows = rotary_workgroups(a.rope);
   }
   OI2_CHECK_ARG(pages + rows < 1 << 23, "%d tokens are too many for one call", n_tokens);
+  OI2_CHECK_ARG(!q || (!clashes(true, q_out, q->heads, q, n_tokens, kHeadD) && !clashes(false, q_out, q->heads, k, n_tokens, kHeadD) &&
+                       !clashes(false, q_out, q->heads, v, n_tokens, kHeadD)),
+                "q's output shares memory with q, and is not q, or with k or v");
   a.page_groups = (int)pages;
   hipStream_t st = (hipStream_t)stream;
   const uint32_t groups = (uint32_t)(pages + rows);

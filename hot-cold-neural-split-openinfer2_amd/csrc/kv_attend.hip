@@ -900,6 +900,7 @@ int oi2_kv_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int
   const size_t need = attend_bytes(l, c->n_kv);
   OI2_CHECK_ARG(!need || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
                 "workspace of %zu bytes, %zu needed, 16-byte aligned", workspace_bytes, need);
+  OI2_CHECK_ARG(!clashes(true, out, c->n_q, q, n_tokens, kHeadD), "out shares memory with q, and is not q");
   AttendArgs a{};
   a.work = p->work;
   a.table = c->block_table;

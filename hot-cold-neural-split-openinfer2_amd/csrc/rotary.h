@@ -219,4 +219,20 @@ inline int64_t rotary_workgroups(const RotaryArgs& a) {
 
 int check_rotary(const oi2_rotary* r);
 
+// Whether the dense (n_tokens, out_heads, dim) values at out share memory with
+// in's: a workgroup would read what another has written.  own: in is what out
+// is computed from, and may be it where it is as dense: every value of it is
+// read by the thread that writes it, or before.
+inline bool clashes(bool own, const void* out, int out_heads, const oi2_heads* in, int n_tokens, int dim) {
+  if (!in || !in->heads || !out_heads || n_tokens < 1) return false;
+  if (own && out == in->data && out_heads == in->heads && in->head_stride == dim &&
+      (n_tokens == 1 || in->token_stride == (int64_t)in->heads * dim))
+    return false;
+  int64_t lo = 0, hi = dim;                // of in, in elements
+  const int64_t far[2] = {(n_tokens - 1) * in->token_stride, (in->heads - 1) * in->head_stride};
+  for (int64_t f : far) (f < 0 ? lo : hi) += f;
+  const intptr_t o0 = (intptr_t)out, o1 = o0 + 2 * (int64_t)n_tokens * out_heads * dim, i = (intptr_t)in->data;
+  return o0 < i + 2 * hi && i + 2 * lo < o1;
+}
+
 }  // namespace oi2

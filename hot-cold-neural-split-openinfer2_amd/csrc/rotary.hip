@@ -48,6 +48,12 @@ extern "C" int oi2_rotary_apply(const oi2_rotary* r, int32_t dtype, int32_t n_to
     OI2_CHECK_ARG(!a.heads[w] || ((uintptr_t)a.src[w] % 2 == 0 && (uintptr_t)a.dst[w] % 2 == 0), "q and k must be 2-byte aligned");
   const int64_t groups = rotary_workgroups(a);
   OI2_CHECK_ARG(groups < 1 << 23, "%d tokens of %d heads are too many for one call", n_tokens, q->heads + k->heads);
+  const oi2_heads ko{k_out, k->heads, (int64_t)k->heads * r->head_dim, r->head_dim};
+  const int d = r->head_dim;
+  OI2_CHECK_ARG(!clashes(true, q_out, q->heads, q, n_tokens, d) && !clashes(true, k_out, k->heads, k, n_tokens, d) &&
+                    !clashes(false, q_out, q->heads, k, n_tokens, d) && !clashes(false, k_out, k->heads, q, n_tokens, d) &&
+                    !clashes(false, q_out, q->heads, &ko, n_tokens, d),
+                "an output shares memory with an input, and is not that input, or with the other output");
   const dim3 grid((uint32_t)groups), block(256);
   hipStream_t st = (hipStream_t)stream;
   const bool bf = dtype == OI2_DTYPE_BF16;

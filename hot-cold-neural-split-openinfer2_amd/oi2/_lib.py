@@ -282,6 +282,16 @@ def heads(x: torch.Tensor, n: int) -> tuple[torch.Tensor, Heads]:
     return x, Heads(x.data_ptr(), n, st[0], st[1])
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the spans of memory of two tensors meet."""
+    def span(x):
+        return x.data_ptr(), x.data_ptr() + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+    if not (a.numel() and b.numel()):
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def logit_threshold(p: float) -> float:
     """The logit cut the kernels apply for predict_mask's ``sigmoid(l) >= p``
     (predictor.py:77-79): l >= log(p / (1 - p)) for 0 < p < 1.  At the edges

@@ -203,6 +203,9 @@ class GroupedQueryAttention(torch.nn.Module):
         if residual_out is not None and (residual_out.shape != x.shape or residual_out.dtype != torch.float16
                                          or residual_out.device != x.device or not residual_out.is_contiguous()):
             raise ValueError("residual_out must be a contiguous fp16 tensor shaped like x")
+        if (residual_out is not None and x.is_contiguous() and residual_out.data_ptr() != x.data_ptr()
+                and _lib.overlap(residual_out, x)):
+            raise ValueError("residual_out shares memory with x, and is not x")
         xc = x.contiguous()
         L = _lib.load_library()
         with _lib.on_device(cache.device) as stream:

@@ -538,7 +538,7 @@ enum { OI2_ZERO_LEFT_OUT = 0x100 };
  * tokens at positions (device memory): the arithmetic of engine.py:140-157
  * with each token at its own position, in fp64.  q_out and k_out are dense
  * (n_tokens, heads, head_dim) and may be the inputs themselves where those
- * are dense.  A token at a negative position is left out: its rows in the
+ * are dense; other overlaps are refused.  A token at a negative position is left out: its rows in the
  * outputs are not written. */
 int oi2_rotary_apply(const oi2_rotary* r, int32_t dtype, int32_t n_tokens, const int32_t* positions,
                      const oi2_heads* q, void* q_out, const oi2_heads* k, void* k_out, void* stream);
@@ -546,7 +546,8 @@ int oi2_rotary_apply(const oi2_rotary* r, int32_t dtype, int32_t n_tokens, const
 /* k and v (n_tokens, n_kv, 128) of the plan's step into the pages of `layer`;
  * with r not NULL, k is rotated first (rounded to its type, then coded: the
  * codes of oi2_rotary_apply's k) and q, if given, is rotated into q_out
- * (n_tokens, q heads, 128).  The plan's tokens past n_tokens are left out.
+ * (n_tokens, q heads, 128), which may be q itself where that is dense and
+ * shares no other memory with q, k or v.  The plan's tokens past n_tokens are left out.
  * A row's step is appended once per layer, in the order of the extends. */
 int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
                   const oi2_heads* k, const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q, void* q_out,
@@ -561,8 +562,8 @@ size_t oi2_kv_attend_workspace_bytes(const oi2_paged* c, int32_t max_tokens, int
  * `layer`, after the step's own tokens were appended: the token at position t
  * of row i sees positions [0, t] of the row.
  *   out = softmax(scale q k^T) v,  k and v the codes times their scales
- * q (n_tokens, n_q, 128) with strides, out (n_tokens, n_q, 128) dense, both of
- * `dtype` (OI2_DTYPE_F16 or _BF16).  Scores, the softmax's sums and the output
+ * q (n_tokens, n_q, 128) with strides, out (n_tokens, n_q, 128) dense (q itself,
+ * where that is dense, or other memory), both of `dtype` (OI2_DTYPE_F16 or _BF16).  Scores, the softmax's sums and the output
  * are fp32 until the one rounding of out; probabilities enter the products as
  * two fp16 parts.  The tokens of a rejected row give zeros; rows of out past the step's last token are left as they were.
  * n_tokens below the step's: its first tokens alone. */
