@@ -42,7 +42,8 @@ def rotary_frequencies(rotary_dim: int, theta: float, scaling: dict | None = Non
     yarn        pairs are slowed by ``factor`` from the one that turns
                 ``beta_slow`` times over ``original_len`` positions on, stay up
                 to the one that turns ``beta_fast`` times, linear in j between;
-                the rotated values grow by 0.1 ln(factor) + 1
+                the rotated values grow by 0.1 ln(factor) + 1; a factor of at
+                least 1, and ``beta_fast`` no less than ``beta_slow``
     """
     theta = float(theta)
     if not (math.isfinite(theta) and theta > 1.0):
@@ -61,6 +62,10 @@ def rotary_frequencies(rotary_dim: int, theta: float, scaling: dict | None = Non
             if rotary_dim <= 2:
                 raise ValueError("rotary scaling 'ntk' needs more than one pair")
             theta *= s["factor"] ** (rotary_dim / (rotary_dim - 2))
+        if kind == "yarn" and s["factor"] < 1:
+            raise ValueError("rotary scaling 'yarn' lengthens contexts: a factor of at least 1")
+        if kind == "yarn" and s["beta_fast"] < s["beta_slow"]:
+            raise ValueError("rotary scaling 'yarn': beta_fast below beta_slow")
         if kind == "wavelength" and s["high_factor"] <= s["low_factor"]:
             raise ValueError("rotary scaling 'wavelength': high_factor above low_factor")
     f = [theta ** (-2.0 * j / rotary_dim) for j in range(rotary_dim // 2)]
