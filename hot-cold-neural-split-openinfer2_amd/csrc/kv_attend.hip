@@ -150,8 +150,11 @@ __device__ __forceinline__ Probs to_probs(const float (&e)[8]) {
 
 // A page's scores are dot * score_scale + ev, with q negated where the scale of
 // the scores is negative, so that the largest dot is the largest score; a scale
-// of zero counts as 2^-120, because a masked dot is minus infinity.
-__device__ __forceinline__ float score_scale(float sc, float k_scale) { return fmaxf(fabsf(sc) * k_scale, 7.52316385e-37f); }
+// of zero counts as 2^-120, because a masked dot is minus infinity, and one past
+// fp32 as its largest number, because a dot may be zero.
+__device__ __forceinline__ float score_scale(float sc, float k_scale) {
+  return __builtin_amdgcn_fmed3f(fabsf(sc) * k_scale, 7.52316385e-37f, 3.40282347e38f);
+}
 
 __device__ __forceinline__ float quad_max(float v) {   // over the lanes l, l ^ 16, l ^ 32, l ^ 48
   v = fmaxf(v, __shfl_xor(v, 16));

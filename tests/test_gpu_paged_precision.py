@@ -121,3 +121,26 @@ def test_many_small_weights_behind_a_large_one(dev, dtype, past, new):
             # of the small weights
             tol = torch.finfo(dtype).eps / 2 * abs(want) + (past + t) * 2.0 ** -30 + 2 * w * 2.0 ** -17
             assert np.abs(out - want).max() <= tol, (bits, t, np.abs(out - want).max() / tol)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_scores_past_fp32_beside_scores_of_zero(dev, new):
+    """A query and a key whose product passes fp32: minus infinity weighs nothing,
+    and the other positions, whose keys are 0, share the rest."""
+    print(f"[large scores] {new}", flush=True)
+    past, n_q, n_kv = 70, 4, 2
+    n = past + new
+    k = torch.zeros((n, n_kv, D), device=dev)
+    k[3, :, 0] = -2.0 ** 60
+    v = torch.randint(-7, 8, (n, n_kv, D), generator=torch.Generator(device=dev).manual_seed(6), device=dev).float()
+    c, o, plan, ref = _step(dev, n_q, n_kv, [past], [new], k.bfloat16(), v.bfloat16(), torch.bfloat16)
+    q = torch.zeros((new, n_q, D), device=dev)
+    q[..., 0] = 2.0 ** 100
+    y = _np(c.attend(0, q.bfloat16(), plan, scale=1.0))
+    v = _np(v)
+    for t in range(new):
+        seen = np.delete(v[:past + t + 1], 3, 0)
+        for h in range(n_q):
+            x = seen[:, h // (n_q // n_kv)]
+            tol = 2.0 ** -8 * np.abs(x.mean(0)) + P.attend_bound(0.0, 0.0, n, False) * np.abs(x).mean(0)
+            assert (np.abs(y[t, h] - x.mean(0)) <= tol).all()
