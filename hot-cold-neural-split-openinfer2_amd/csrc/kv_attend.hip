@@ -305,10 +305,12 @@ constexpr int kFewLds = (kFewWaves * kFewRows * (kORow + 2) + kHeadD) * 4;
 //
 // A wave takes every fourth page, loads the next one (k and v, 16 KB) while it
 // works on this one, and its page number by a scalar load two ahead; the four
-// meet in LDS at the end.  Bound by the pages' bytes: 56 tokens of 300 to 14000
-// positions 72 us (5.3 TB/s), three of 40 to 110 thousand 46 (5.2); one of 700
-// positions 8.0, three rounds and the merge.  Tried without gain: 8 and 16
-// waves, pages dealt out in equal shares whatever row they belong to.
+// meet in LDS at the end.  Bound by the pages' loads: 56 tokens of 300 to 14000
+// positions 71 us (378 MB, 5.3 TB/s), three of 40 to 110 thousand 46 (241 MB,
+// 5.2); the same blocks, scattered over the pool and read alone, take 57 and 37
+// (6.5 TB/s), so a fifth is the start, the last round, and the join.  One token
+// of 700 positions 8.1, three rounds and the merge.  Tried without gain: 8 and
+// 16 waves, pages dealt out in equal shares whatever row they belong to.
 template <bool BF16>
 __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* smem) {
   const int item = b / a.n_kv, g = b - item * a.n_kv;
@@ -563,9 +565,11 @@ __device__ __forceinline__ int v_lds(int d, int c) { return kVLds + d * 128 + 16
 //
 // The next page's staging stands between the products of the scores, and a
 // fragment's exponentials between the products of the fragment before.  What
-// bounds it: matrix cores, vector unit and LDS are busy about half the time each,
-// and two waves a SIMD overlap little more than that by chance: a call of 5000
-// tokens 292 us in fp16 and 289 in bf16 (700 TFLOP/s).  With one fp16 part of a
+// bounds it: the products, a third of them for the probabilities' low parts;
+// the matrix cores are busy 60 % of the time, and two waves a SIMD fill the rest
+// by chance.  A call of 5000 tokens 288 to 306 us, boxes differ, in fp16 and 285 to
+// 302 in bf16 (670 to 720 TFLOP/s of the formula's operations, a third more with
+// the low parts'), 6 chunks beside 3 short rows 98 to 102.  With one fp16 part of a
 // probability, of 249 us before k's conflicts went, the exponentials alone made
 // 38, staging 35, the fragments' reads 55, the products 68, and there was tried
 // without gain: fragments read three steps ahead; raised priority around

@@ -81,7 +81,9 @@ class PagedKVCache:
     block_table (n_seqs, ceil(max_len / 64)), lens (n_seqs), free (n_pages, a
     stack) and n_free (1) are the tables, int32 on the device.  A row is
     rejected (``plan.rejected``) and stays as it was when it would pass max_len
-    or the plan's sizes, or when the pool runs out of pages."""
+    or the plan's sizes, or when the pool runs out of pages.  With 0 layers there
+    are the tables alone, and plan.slots say where a caller's own pages of 64
+    positions hold the step's tokens."""
 
     def __init__(self, n_layers: int, n_q: int, n_kv: int, n_seqs: int, max_len: int, n_pages: int, device="cuda"):
         self.n_layers, self.n_q, self.n_kv = int(n_layers), int(n_q), int(n_kv)
