@@ -225,7 +225,7 @@ int check_rotary(const oi2_rotary* r);
 // read by the thread that writes it, or before.
 inline bool clashes(bool own, const void* out, int out_heads, const oi2_heads* in, int n_tokens, int dim) {
   if (!in || !in->heads || !out_heads || n_tokens < 1) return false;
-  if (own && out == in->data && out_heads == in->heads && in->head_stride == dim &&
+  if (own && out == in->data && out_heads == in->heads && (in->heads == 1 || in->head_stride == dim) &&
       (n_tokens == 1 || in->token_stride == (int64_t)in->heads * dim))
     return false;
   int64_t lo = 0, hi = dim;                // of in, in elements

@@ -73,3 +73,19 @@ def test_layer_residual_into_its_input(dev, n):
     if n > 1:
         with pytest.raises(ValueError):
             attn.forward_paged(buf[:n], c, plan, rot, residual_out=buf[1:])
+
+
+def test_one_head_in_place(dev):
+    """A tensor of one head is dense whatever its stride of heads says."""
+    rot = oi2.Rotary(D, 1e4, device=dev)
+    x = torch.randn(9, D, device=dev).half()
+    pos = torch.arange(9, device=dev, dtype=torch.int32)
+    want = rot(x[:, None], None, pos)[0]
+    q = x.clone().as_strided((9, 1, D), (D, 999, 1))
+    assert q.is_contiguous() and rot(q, None, pos, q_out=q)[0] is q and torch.equal(q, want)
+    c = oi2.PagedKVCache(1, 1, 1, 1, 64, 1, device=dev)
+    plan = c.extend([9], c.new_plan(9))
+    k = torch.randn(9, 1, D, device=dev).half()
+    c.append(0, k, k, plan)
+    y = c.attend(0, q, plan)
+    assert c.attend(0, q, plan, out=q) is q and torch.equal(q, y)
