@@ -210,7 +210,7 @@ __global__ __launch_bounds__(1024) void k_page_extend(ExtendArgs a) {
   // whole rounds of a workgroup's four waves.  A tile ends in half a part more on
   // average; those of many rows take that into the share while half a round of
   // parts is left, so that all of them run at once: 33 tiles of 11 to 68 pages
-  // beside three of single tokens 102 -> 87 us.  Few rows, bound by their bytes,
+  // beside three of single tokens took 0.85 of the time.  Few rows, bound by their bytes,
   // lose by it (56 of 5 to 218 pages 71.8 -> 74).
   auto share = [](uint64_t pages, double per_part) {
     return ((int)min(max(ceil((double)pages * per_part), 1.0), 0x1p26) + 3) / 4 * 4;

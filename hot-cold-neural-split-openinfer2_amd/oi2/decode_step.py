@@ -98,9 +98,9 @@ class DecoderStep:
                 raise ValueError(f"a DecodeStack runs one token at a time, got {N}")
             stack.predict(0, x.reshape(H))
         else:
-            # one token: the query is that token's, whatever the plan says
-            step = plan if N > 1 else None
-            prefetch = self.ffn_layers[0].submit_cold_fetch(x, step)
+            def fetch(ffn, x):      # one token: the query is that token's, whatever the plan says
+                return ffn.submit_cold_fetch(x, plan) if N > 1 else ffn.submit_cold_fetch(x[None])
+            prefetch = fetch(self.ffn_layers[0], x)
         for li, attn in enumerate(self.attention_layers):
             resid = torch.empty_like(x)
             attn.forward_paged(x, cache, plan, rotary, layer=li, residual_out=resid)
@@ -110,7 +110,7 @@ class DecoderStep:
                 continue
             this = prefetch
             if li + 1 < len(self.ffn_layers):
-                prefetch = self.ffn_layers[li + 1].submit_cold_fetch(resid, step)
+                prefetch = fetch(self.ffn_layers[li + 1], resid)
             x = self.ffn_layers[li](resid[None], this)[0]
         return x
 
