@@ -82,7 +82,7 @@ class DecoderStep:
         from the mean over the rows' last tokens, of the rows that are taken
         and have tokens in the step (over a DecodeStack: one token).  Tokens
         without a position (of rejected rows, or past the step's last one) have
-        no part in it.  Returns x after the last layer's FFN."""
+        no part in it, whatever they hold.  Returns x after the last layer's FFN."""
         if x.dim() != 2:
             raise ValueError(f"x must be (tokens, hidden), got {tuple(x.shape)}")
         N, H = x.shape

@@ -230,3 +230,27 @@ def test_cold_set_from_files(dev):
         finally:
             for s in stores:
                 s.close()
+
+
+@pytest.mark.parametrize("pad", [1, 12, 37, 100])
+def test_padding_that_is_not_finite_harms_no_row(dev, split, pad):
+    """Tokens without a position hold NaN and infinities: the live rows' results
+    keep their bits (up to 16 tokens, whose FFN sums are in a fixed order) or the
+    FFN's bar."""
+    print(f"[cold set] padding of {pad} that is not finite", flush=True)
+    g = torch.Generator(device=dev).manual_seed(13)
+    past, new = [40, 9], [2, 1]
+    prompt = torch.randn((sum(past), H), generator=g, device=dev).half()
+    x = torch.randn((3 + pad, H), generator=g, device=dev).half()
+    ys = []
+    for bad in (0.0, float("nan"), float("inf")):
+        if bad:
+            x[3:] = bad
+        attn, ffn, c, rot = _start(split, dev, prompt, past)
+        plan = c.extend(new, c.new_plan(3 + pad))
+        ys.append(DecoderStep(attn, ffn).forward_paged(x, c, plan, rot)[:3].clone())
+    for y in ys[1:]:
+        if pad <= 13:
+            assert torch.equal(y, ys[0])
+        else:
+            assert_ffn_close(y.float().cpu().numpy(), ys[0].float().cpu().numpy(), tol=1e-3, cos_min=0.999999, what="padding")
