@@ -206,24 +206,6 @@ __device__ __forceinline__ void append_few(const AppendArgs& a, int task) {
   if (j == 0) *ph.scale = float2{two_to(ek), flag ? -two_to(ev) : two_to(ev)};
 }
 
-template <bool BF16>
-__device__ __forceinline__ float lower(uint32_t d) {
-  return widen<BF16>((uint16_t)(d & 0xFFFFu));
-}
-template <bool BF16>
-__device__ __forceinline__ float upper(uint32_t d) {
-  return widen<BF16>((uint16_t)(d >> 16));
-}
-
-// Largest of two 16-bit values each; the magnitudes of fp16 and bf16 are in the
-// order of their bits.
-__device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
-}
-template <bool BF16>
-constexpr uint32_t kInfBits = BF16 ? 0x7F80u : 0x7C00u;
-
 // The largest magnitude of 16 values in pairs, of the finite ones alone with FINITE.
 template <bool BF16, bool FINITE>
 __device__ __forceinline__ uint32_t top_of(const uint32_t (&x)[8]) {
@@ -453,17 +435,11 @@ void launch_append(const AppendArgs& a, bool few, bool kwide, uint32_t groups, h
 }
 
 }  // namespace
-}  // namespace oi2
 
-using namespace oi2;
-
-extern "C" int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
-                             const oi2_heads* k, const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q,
-                             void* q_out, void* stream) {
-  clear_error();
-  if (int rc = check_paged(c, layer, true)) return rc;
-  if (int rc = check_plan(c, p)) return rc;
-  const bool zero = dtype & OI2_ZERO_LEFT_OUT;
+// dtype without its flag, which goes to zero.
+int check_append(const oi2_paged* c, const oi2_page_plan* p, int32_t& dtype, bool& zero, int32_t n_tokens, const oi2_heads* k,
+                 const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q, const void* q_out) {
+  zero = dtype & OI2_ZERO_LEFT_OUT;
   dtype &= ~OI2_ZERO_LEFT_OUT;
   OI2_CHECK_ARG(dtype == OI2_DTYPE_F16 || dtype == OI2_DTYPE_BF16, "dtype %d: fp16 or bf16", dtype);
   OI2_CHECK_ARG(n_tokens >= 0 && n_tokens <= p->max_tokens, "%d tokens in a plan of %d", n_tokens, p->max_tokens);
@@ -477,6 +453,25 @@ extern "C" int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t
   OI2_CHECK_ARG(k->data && v->data && (uintptr_t)k->data % 2 == 0 && (uintptr_t)v->data % 2 == 0, "k and v must be non-null and 2-byte aligned");
   OI2_CHECK_ARG(!q || (q->heads >= 1 && q->heads <= 1 << 16 && q->data && q_out && (uintptr_t)q->data % 2 == 0 && (uintptr_t)q_out % 2 == 0),
                 "q and its output must be non-null and 2-byte aligned, with heads");
+  OI2_CHECK_ARG(!q || (!clashes(true, q_out, q->heads, q, n_tokens, kHeadD) && !clashes(false, q_out, q->heads, k, n_tokens, kHeadD) &&
+                       !clashes(false, q_out, q->heads, v, n_tokens, kHeadD)),
+                "q's output shares memory with q, and is not q, or with k or v");
+  return OI2_OK;
+}
+
+}  // namespace oi2
+
+using namespace oi2;
+
+extern "C" int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
+                             const oi2_heads* k, const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q,
+                             void* q_out, void* stream) {
+  clear_error();
+  if (int rc = check_paged(c, layer, true)) return rc;
+  if (int rc = check_plan(c, p)) return rc;
+  bool zero;
+  if (int rc = check_append(c, p, dtype, zero, n_tokens, k, v, r, q, q_out)) return rc;
+  if (n_tokens == 0) return OI2_OK;
   AppendArgs a{};
   const PlanLayout l = plan_layout(*c, p->max_tokens, p->max_new), now = plan_layout(*c, n_tokens, p->max_new);
   a.work = p->work;
@@ -512,9 +507,6 @@ extern "C" int oi2_kv_append(const oi2_paged* c, const oi2_page_plan* p, int32_t
     rows = rotary_workgroups(a.rope);
   }
   OI2_CHECK_ARG(pages + rows < 1 << 23, "%d tokens are too many for one call", n_tokens);
-  OI2_CHECK_ARG(!q || (!clashes(true, q_out, q->heads, q, n_tokens, kHeadD) && !clashes(false, q_out, q->heads, k, n_tokens, kHeadD) &&
-                       !clashes(false, q_out, q->heads, v, n_tokens, kHeadD)),
-                "q's output shares memory with q, and is not q, or with k or v");
   a.page_groups = (int)pages;
   hipStream_t st = (hipStream_t)stream;
   const uint32_t groups = (uint32_t)(pages + rows);

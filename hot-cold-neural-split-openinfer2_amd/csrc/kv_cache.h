@@ -1,5 +1,5 @@
-// The paged 8-bit KV cache's layout, its plans' work lists and the sizes that
-// host and kernels agree on.
+// The paged KV caches' plans' work lists, the 8-bit one's layout, and the sizes
+// that host and kernels agree on.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -87,5 +87,8 @@ inline PlanLayout plan_layout(const oi2_paged& c, int32_t n_tokens, int32_t max_
 // Checks of the arguments that the entry points share; OI2_OK or an error set.
 int check_paged(const oi2_paged* c, int32_t layer, bool pool);
 int check_plan(const oi2_paged* c, const oi2_page_plan* p);
+int check_paged4(const oi2_paged* c, int32_t layer);     // of the 4-bit cache, which has no scales besides its pages
+int check_append(const oi2_paged* c, const oi2_page_plan* p, int32_t& dtype, bool& zero, int32_t n_tokens, const oi2_heads* k,
+                 const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q, const void* q_out);
 
 }  // namespace oi2

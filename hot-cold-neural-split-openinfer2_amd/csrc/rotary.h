@@ -69,6 +69,25 @@ __device__ __forceinline__ uint16_t narrow(float v) {
   return float_to_half_bits(v);
 }
 
+// Pairs of them in a dword.
+template <bool BF16>
+__device__ __forceinline__ float lower(uint32_t d) {
+  return widen<BF16>((uint16_t)(d & 0xFFFFu));
+}
+template <bool BF16>
+__device__ __forceinline__ float upper(uint32_t d) {
+  return widen<BF16>((uint16_t)(d >> 16));
+}
+
+// Largest of two 16-bit values each; the magnitudes of fp16 and bf16 are in the
+// order of their bits.
+__device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <bool BF16>
+constexpr uint32_t kInfBits = BF16 ? 0x7F80u : 0x7C00u;
+
 struct RotaryArgs {
   const uint64_t* freq;
   const int32_t* positions;
