@@ -1,0 +1,308 @@
+// Attention of a step's query tokens over the paged 4-bit KV cache: the plan, the
+// parts and the products of the 8-bit cache's, on pages whose groups of 32 dims
+// have a scale at every position.
+//
+// Codes times scales, exact in fp16, are the products' operands, so that scales
+// cost one packed multiplication for two values and nothing behind it:
+//   p = exp2(score - m),  out = sum p v,  l = sum p
+// The cache stores a page so that a lane's 16 bytes of k are 32 dims of one
+// position, one group, and its 16 bytes of v 8 dims, of one group, of four
+// positions: a scale serves all that a lane has of a position.
+#include "attend.h"
+#include "kv4.h"
+
+namespace oi2 {
+namespace {
+
+// A dword of k, dims in order, times its scale.
+__device__ __forceinline__ h8 k_values(uint32_t d, f16x2 s) {
+  const uint32_t lo = low4(d), hi = high4(d);
+  const f16x2 a = whole2(lo, false) * s, b = whole2(lo, true) * s, c = whole2(hi, false) * s, e = whole2(hi, true) * s;
+  return h8{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
+}
+__device__ __forceinline__ f16x2 twice(uint32_t d, bool hi) {
+  return as_f16x2(__builtin_amdgcn_perm(d, d, hi ? 0x03020302u : 0x01000100u));
+}
+
+// Dims 2 q and 2 q + 1 of two positions' dwords x, y as e4m3 bytes: (x, y) of the
+// first, (x, y) of the second.
+__device__ __forceinline__ uint32_t v_bytes(uint32_t x, uint32_t y, int q) {
+  return __builtin_amdgcn_perm(y, x, q & 1 ? 0x07030602u : 0x05010400u);
+}
+
+// Scales of v at positions pos, pos + 1 .. in pairs: behind the row's end 0,
+// whatever the page held before; a NaN that some row may not see 0, and noted for
+// the 8 dims from dim0 on.
+template <int N>
+__device__ __forceinline__ void fix_scales(uint32_t (&s)[N], int pos, int kv_len, int dim0, int* nan) {
+#pragma unroll
+  for (int k = 0; k < 2 * N; ++k) {
+    const uint32_t shift = 16 * (k & 1);
+    const bool out = pos + k >= kv_len, odd = (s[k / 2] >> shift & 0x7C00u) == 0x7C00u;
+    if (out || odd) s[k / 2] &= ~(0xFFFFu << shift);
+    if (odd && !out)
+      for (int e = 0; e < 8; ++e) atomicMin(&nan[dim0 + e], pos + k);
+  }
+}
+
+// ── few rows ─────────────────────────────────────────────────────────────────
+
+// Lane (r = lane % 16, grp = lane / 16).  K's 16-row tile t of a page: row
+// r = 4 a + i is position 16 a + 4 t + i, and the lane has dims 32 grp .. of it,
+// eight a step; D's element i of lane (r, grp) is the score of query row r at
+// position 16 grp + 4 t + i: in 4 tiles a lane has positions 16 grp .. 16 grp + 15
+// of its query row.  V's row r of tile d is dim 8 r + d, at those positions.
+//
+// A wave takes every fourth page, loads the next one (9 KB) while it works on
+// this one, and its page number by a scalar load two ahead; the four meet in
+// LDS at the end.
+template <bool BF16>
+__device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* smem) {
+  const FewLds lds(smem);
+  FewTile t;
+  if (!few_open<BF16>(a, b, lds, t, [](int grp, int i) { return 32 * grp + 8 * i; })) return;
+  const ItemHead& it = t.it;
+  const int g = t.g, w = t.w, lane = t.lane, r = t.r, grp = t.grp, lim = t.lim, all_see = t.all_see;
+
+  const float ninf = -__builtin_inff();
+  f32x4 o[8];
+#pragma unroll
+  for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = ninf, l = 0.0f;
+  const float ksc = score_scale(t.sc, 1.0f);
+
+  const int32_t* table = a.table + (int64_t)it.row * a.width;
+  auto block_of = [&](int page) {
+    int id = scalar_load(table + min(page, it.page1 - 1));
+    id = (unsigned)id < (unsigned)a.n_pages ? id : 0;
+    return (int64_t)id * a.n_kv + g;
+  };
+  // Past the last page the descriptor's range is empty: nothing is read.
+  auto page_rsrc = [&](int64_t block, int page) { return rsrc(a.pages + block * k4Block, page < it.page1 ? k4Block : 0); };
+  u32x4 kr[4], vr[4];
+  u32x2v ks;
+  uint32_t vs[8];
+  auto load_k = [&](rsrc_t x) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) kr[n] = wld16(x, 1024 * n + 16 * lane);
+    ks = wld8(x, k4KScale + 8 * lane);
+  };
+  auto load_v = [&](rsrc_t x) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) vr[n] = wld16(x, k4V + 1024 * n + 16 * lane);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const u32x4 s = wld16(x, k4VScale + 128 * (r >> 2) + 32 * grp + 16 * n);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) vs[4 * n + k] = s[k];
+    }
+  };
+  const int first = it.page0 + w;
+  int64_t next = 0;
+  if (first < it.page1) {
+    const rsrc_t r0 = page_rsrc((int64_t)scalar_load(t.full->ids + w) * a.n_kv + g, first);
+    load_k(r0);
+    load_v(r0);
+    next = block_of(first + kFewWaves);
+  }
+  for (int page = first; page < it.page1; page += kFewWaves) {
+    const rsrc_t rn = page_rsrc(next, page + kFewWaves);
+    next = block_of(page + 2 * kFewWaves);
+
+    float s[16];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      const f16x2 sk = twice(k < 2 ? ks.x : ks.y, k & 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc = mfma16(k_values(kr[k][i], sk), t.q[i], acc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * k + i] = acc[i];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(rn);
+    __builtin_amdgcn_sched_barrier(0);
+    const int p0 = page * kPage + 16 * grp;
+    const bool whole = page * kPage + kPage <= all_see;
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] = p0 + j < lim ? s[j] : ninf;
+      fix_scales(vs, p0, it.kv_len, 8 * r, lds.nan);
+    }
+    float cm = s[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) cm = fmaxf(cm, s[j]);
+    cm = quad_max(cm) * ksc;
+    const bool up = cm > m + kSlack;
+    if (__any(up)) {
+      const float mn = up ? cm : m;
+      const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) o[d] *= alpha;
+      m = mn;
+    }
+    const float rel = kLift - (m == ninf ? 0.0f : m);
+    float sum[2] = {0.0f, 0.0f};
+    Probs p[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + j], ksc, rel));
+        sum[h] += e[j];
+      }
+      p[h] = to_probs(e);
+    }
+    l += sum[0] + sum[1];
+    // positions 16 grp + 8 h + 2 k, + 1 are dwords 2 (k % 2), + 1 of vector 2 h + k / 2
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {        // dims 8 r + 2 q, + 1
+        f16x2 v0[4], v1[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t x = vr[2 * h + k / 2][2 * (k % 2)], y = vr[2 * h + k / 2][2 * (k % 2) + 1];
+          const uint32_t d = q < 2 ? v_bytes(low4(x), low4(y), q) : v_bytes(high4(x), high4(y), q);
+          const f16x2 sv = as_f16x2(vs[4 * h + k]);
+          v0[k] = whole2(d, false) * sv;
+          v1[k] = whole2(d, true) * sv;
+        }
+        const h8 f0 = {v0[0][0], v0[0][1], v0[1][0], v0[1][1], v0[2][0], v0[2][1], v0[3][0], v0[3][1]};
+        const h8 f1 = {v1[0][0], v1[0][1], v1[1][0], v1[1][1], v1[2][0], v1[2][1], v1[3][0], v1[3][1]};
+        o[2 * q] = mfma16(f0, p[h].hi, o[2 * q]);
+        o[2 * q] = mfma16(f0, p[h].lo, o[2 * q]);
+        o[2 * q + 1] = mfma16(f1, p[h].hi, o[2 * q + 1]);
+        o[2 * q + 1] = mfma16(f1, p[h].lo, o[2 * q + 1]);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(rn);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)              // dims 8 (4 grp + i) ..
+#pragma unroll
+    for (int d = 0; d < 8; d += 4)
+      *reinterpret_cast<f32x4*>(&lds.o[w][r][8 * (4 * grp + i) + d]) = f32x4{o[d][i], o[d + 1][i], o[d + 2][i], o[d + 3][i]};
+  if (grp == 0) {
+    lds.m[w][r] = m;
+    lds.l[w][r] = l;
+  }
+  few_close<BF16>(a, t, lds, smem);
+}
+
+// ── many rows ────────────────────────────────────────────────────────────────
+
+// Thread (n = tid / 64, lane): the 16 bytes of k of one position and group, and
+// those of v of positions 16 grp + 4 n .. + 3, dims 8 r ...  Row 16 e + r of V^T
+// in LDS is dim 8 r + e, so that a wave's stores are to 16 rows side by side.
+struct Pages4 {
+  const AttendArgs& a;
+  const ItemHead& it;
+  int tid, *nan;
+  int k_st, v_st;                      // lane bases of the staging stores
+  int at_ks, at_vs;                    // of the scales in a block
+  u32x4 kr, vr;
+  uint32_t ks, vs[2];
+
+  __device__ __forceinline__ Pages4(const AttendArgs& args, const ItemHead& item, int thread, int* s_nan)
+      : a(args), it(item), tid(thread), nan(s_nan) {
+    const int n = tid >> 6, hi = (tid >> 4) & 3, r = tid & 15;    // hi: k's group, v's grp
+    k_st = k_lds(16 * (r >> 2) + 4 * n + (r & 3), 4 * hi);
+    v_st = v_lds(r, 2 * hi + (n >> 1)) + 8 * (n & 1);
+    at_ks = k4KScale + 8 * (tid & 63) + 2 * n;
+    at_vs = k4VScale + 128 * (r >> 2) + 2 * (16 * hi + 4 * n);
+  }
+  __device__ __forceinline__ int first_pos() const { return 16 * ((tid >> 4) & 3) + 4 * (tid >> 6); }
+  __device__ __forceinline__ void load(int64_t block) {
+    const uint8_t* b = a.pages + block * k4Block;
+    kr = load16(b + 16 * tid);
+    vr = load16(b + k4V + 16 * tid);
+    ks = *reinterpret_cast<const uint16_t*>(b + at_ks);
+    const u32x2v s = *reinterpret_cast<const u32x2v*>(b + at_vs);
+    vs[0] = s.x;
+    vs[1] = s.y;
+  }
+  __device__ __forceinline__ float2 scale_of(int64_t) const { return float2{1.0f, 1.0f}; }
+  __device__ __forceinline__ void fix(int page, float) {
+    if (page * kPage + kPage > min(it.pos0 + 1, it.kv_len)) fix_scales(vs, page * kPage + first_pos(), it.kv_len, 8 * (tid & 15), nan);
+  }
+  __device__ __forceinline__ void put_k(uint8_t* s_page, int ka, int q) const {
+    *reinterpret_cast<h8*>(s_page + (ka ^ (16 * q))) = k_values(kr[q], twice(ks, false));
+  }
+  __device__ __forceinline__ void put_v(uint8_t* s_page, int va, int q) const {   // dims 8 r + 2 q, + 1: rows 32 q + r, + 16
+    f16x2 v[2][2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t x = vr[2 * k], y = vr[2 * k + 1];
+      const uint32_t d = q < 2 ? v_bytes(low4(x), low4(y), q) : v_bytes(high4(x), high4(y), q);
+      v[0][k] = whole2(d, false) * as_f16x2(vs[k]);
+      v[1][k] = whole2(d, true) * as_f16x2(vs[k]);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<u32x2v*>(s_page + va + 128 * (32 * q + 16 * e)) =
+          u32x2v{__builtin_bit_cast(uint32_t, v[e][0]), __builtin_bit_cast(uint32_t, v[e][1])};
+  }
+  // element j of o[d] in half h is row 32 d + 8 (j / 4) + j % 4, + 4 h, of V^T
+  static __device__ __forceinline__ int dim(int row, int h) { return 8 * ((row & 15) + 4 * h) + (row >> 4); }
+  template <class F>
+  static __device__ __forceinline__ void each_four(const f32x16 (&o)[4], int h, F f) {   // of dims 4 chunk ..
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)          // dims 8 (8 q + 4 h + e) ..: rows 16 apart
+#pragma unroll
+        for (int d = 0; d < 4; d += 2)
+          f(2 * (8 * q + 4 * h + e) + d / 2,
+            f32x4{o[d][4 * q + e], o[d][8 + 4 * q + e], o[d + 1][4 * q + e], o[d + 1][8 + 4 * q + e]});
+  }
+};
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void k_kv4_attend_few(AttendArgs a) {
+  __shared__ __align__(16) uint8_t smem[kFewLds];
+  const int b = blockIdx.x;
+  if (b < a.few.groups) attend_few<BF16>(a, b, smem);
+  else zero_rest(a, b - a.few.groups);
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void k_kv4_attend(AttendArgs a) {
+  static_assert(kManyLds >= kFewLds && kThreads == 64 * kFewWaves, "one workgroup for either");
+  __shared__ __align__(1024) uint8_t smem[kManyLds];
+  const int b = blockIdx.x;
+  if (b < a.many.groups) attend_many<BF16, Pages4>(a, b, smem);
+  else if (b - a.many.groups < a.few.groups) attend_few<BF16>(a, b - a.many.groups, smem);
+  else zero_rest(a, b - a.many.groups - a.few.groups);
+}
+
+}  // namespace
+}  // namespace oi2
+
+using namespace oi2;
+
+extern "C" int oi2_kv4_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
+                              const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  clear_error();
+  if (int rc = check_paged4(c, layer)) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  AttendCall call;
+  if (int rc = attend_call(call, c, p, dtype, n_tokens, q, scale, out, workspace, workspace_bytes, st)) return rc;
+  if (!call.groups) return OI2_OK;
+  AttendArgs& a = call.a;
+  a.pages = c->pages + (size_t)layer * c->n_pages * c->n_kv * k4Block;
+  const dim3 grid(call.groups), block(kThreads);
+  if (a.many.groups && call.bf16) hipLaunchKernelGGL(k_kv4_attend<true>, grid, block, 0, st, a);
+  else if (a.many.groups) hipLaunchKernelGGL(k_kv4_attend<false>, grid, block, 0, st, a);
+  else if (call.bf16) hipLaunchKernelGGL(k_kv4_attend_few<true>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(k_kv4_attend_few<false>, grid, block, 0, st, a);
+  OI2_CHECK_LAUNCH();
+  return OI2_OK;
+}

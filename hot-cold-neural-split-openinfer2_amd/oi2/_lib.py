@@ -156,6 +156,16 @@ _SIGS = {
     "oi2_kv_attend_workspace_bytes": (c_size_t, [POINTER(Paged), c_int32, c_int32]),
     "oi2_kv_attend": (c_int32, [POINTER(Paged), POINTER(PagePlan), c_int32, c_int32, c_int32,
                                 POINTER(Heads), c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "oi2_kv4_append": (c_int32, [POINTER(Paged), POINTER(PagePlan), c_int32, c_int32, c_int32,
+                                 POINTER(Heads), POINTER(Heads), POINTER(Rotary), POINTER(Heads), c_void_p,
+                                 c_void_p]),
+    "oi2_kv4_fetch": (c_int32, [POINTER(Paged), c_int32, c_void_p, c_void_p, c_int32, c_int32, POINTER(Heads),
+                                POINTER(Heads), c_void_p, c_void_p]),
+    "oi2_kv4_attend": (c_int32, [POINTER(Paged), POINTER(PagePlan), c_int32, c_int32, c_int32,
+                                 POINTER(Heads), c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "oi2_kv4_attn_forward": (c_int32, [c_void_p, c_int32, POINTER(Attn), c_float, POINTER(Rotary),
+                                       POINTER(Paged), POINTER(PagePlan), c_int32, c_void_p, c_void_p,
+                                       c_void_p, c_size_t, c_void_p]),
     "oi2_attn_paged_workspace_bytes": (c_size_t, [POINTER(Paged), c_int32, c_int32, c_int32]),
     "oi2_attn_forward_paged": (c_int32, [c_void_p, c_int32, POINTER(Attn), c_float, POINTER(Rotary),
                                          POINTER(Paged), POINTER(PagePlan), c_int32, c_void_p, c_void_p,

@@ -185,8 +185,8 @@ class GroupedQueryAttention(torch.nn.Module):
         """The same for the packed tokens of a step over a paged cache of
         requests of different lengths: x (tokens, H) fp16 in the order of
         ``plan``, which ``cache.extend`` has laid out; ``layer`` of the cache,
-        this layer's index by default.  k and v go to the cache in 8 bits, and
-        every token attends, causally, to what its row's cache then holds.
+        this layer's index by default.  k and v go to the cache in its 8 or 4
+        bits, and every token attends, causally, to what its row's cache then holds.
         Returns out (tokens, H); with ``residual_out`` like x, x + out goes
         there.  Tokens without a position (of rejected rows, or past the step's
         last one) give 0, and x in residual_out."""
@@ -213,7 +213,8 @@ class GroupedQueryAttention(torch.nn.Module):
             nbytes = L.oi2_attn_paged_workspace_bytes(cache._ref, plan.max_tokens, plan.max_new,
                                                       max(n, 1))
             ws = x.new_empty((nbytes,), dtype=torch.uint8)
-            _lib.check(L.oi2_attn_forward_paged(
+            forward = L.oi2_kv4_attn_forward if cache.bits == 4 else L.oi2_attn_forward_paged
+            _lib.check(forward(
                 xc.data_ptr(), n, ctypes.byref(self._struct), self.eps, rotary._ref,
                 cache._ref, plan._ref, layer, out.data_ptr(),
                 _lib.ptr(residual_out), ws.data_ptr(), nbytes, stream))

@@ -1,9 +1,11 @@
 """A KV cache for requests of different lengths, in pages of 64 positions held
-in fp8 e4m3fn with a power-of-two scale per page and kv head.
+in fp8 e4m3fn with a power-of-two scale per page and kv head, or (``bits=4``) in
+whole numbers of 4 bits with a scale per position and 32 dims.
 
 ``PagedKVCache`` stands beside ``GroupedQueryAttention``'s own cache (one fp16
 buffer per layer, one length for the whole batch, engine.py:105-109): row i is
-one sequence, rows share a pool of pages, and a position takes half the bytes.
+one sequence, rows share a pool of pages, and a position takes half the bytes,
+or 28 % of them.
 A serving step is
 
     cache.extend(new_lens, plan)                    # once per step, for all layers
@@ -13,12 +15,13 @@ A serving step is
 with the step's tokens packed row after row (``plan.cu``).  Lengths, tables and
 work lists live on the GPU and nothing waits on the host, so a step can be
 captured into a graph.  ``rewind`` cuts rows back: rejected drafts, or the end
-of a sequence.
+of a sequence.  ``fetch`` takes positions of a 4-bit cache out again as dense k
+and v: a request that moves, a prefix that another cache takes over.
 
 ``extend``, ``rewind`` and ``append`` on one cache write its tables and pages:
 they, and what reads the cache, have to be ordered, on one stream or by events.
-``attend`` only reads: of one step, for several layers or queries, it may run on
-several streams at once.
+``attend`` and ``fetch`` only read: of one step, for several layers or queries,
+they may run on several streams at once.
 """
 from __future__ import annotations
 
@@ -31,6 +34,8 @@ from .rotary import Rotary
 
 PAGE = 64
 HEAD_DIM = 128
+GROUP4 = 32                 # dims of a scale of the 4-bit cache
+BLOCK4 = 9216               # bytes of its pages, per kv head
 MAX_SEQS = 2048
 
 
@@ -76,7 +81,12 @@ class PagedKVCache:
     """Pages of ``n_layers`` layers for ``n_seqs`` rows of at most ``max_len``
     positions: ``n_pages`` pages of 64 positions, ``n_kv`` kv heads of 128 for
     ``n_q`` query heads (groups of 1, 2, 4 or 8).  A page takes 16.4 KB per
-    layer and kv head.
+    layer and kv head with ``bits`` 8, 9.2 KB with 4.
+
+    With 4 bits a head's values are groups of 32 dims: whole numbers from -7 to 7
+    times the group's largest magnitude over 7, rounded to 8 significant bits.
+    Magnitudes past 65408 are held as that, a group with a NaN or an infinity as
+    NaN.
 
     block_table (n_seqs, ceil(max_len / 64)), lens (n_seqs), free (n_pages, a
     stack) and n_free (1) are the tables, int32 on the device.  A row is
@@ -85,7 +95,11 @@ class PagedKVCache:
     are the tables alone, and plan.slots say where a caller's own pages of 64
     positions hold the step's tokens."""
 
-    def __init__(self, n_layers: int, n_q: int, n_kv: int, n_seqs: int, max_len: int, n_pages: int, device="cuda"):
+    def __init__(self, n_layers: int, n_q: int, n_kv: int, n_seqs: int, max_len: int, n_pages: int, device="cuda",
+                 bits: int = 8):
+        if bits not in (4, 8):
+            raise ValueError(f"{bits} bits: 4 or 8")
+        self.bits = int(bits)
         self.n_layers, self.n_q, self.n_kv = int(n_layers), int(n_q), int(n_kv)
         self.n_seqs, self.max_len, self.n_pages = int(n_seqs), int(max_len), int(n_pages)
         if self.n_layers < 0:
@@ -108,16 +122,20 @@ class PagedKVCache:
         self.lens = ints((self.n_seqs,), 0)
         self.free = torch.arange(self.n_pages - 1, -1, -1, dtype=torch.int32, device=dev)
         self.n_free = ints((1,), self.n_pages)
-        # a page and kv head's k codes and then its v codes
-        self.pages = torch.zeros((self.n_layers, self.n_pages, self.n_kv, 2, PAGE * HEAD_DIM), dtype=torch.uint8,
-                                 device=dev)
-        self._scales = torch.full((self.n_layers, self.n_pages, self.n_kv, 2), 2.0 ** -40, dtype=torch.float32,
-                                  device=dev)
+        pool = (self.n_layers, self.n_pages, self.n_kv)
+        if self.bits == 8:
+            # a page and kv head's k codes and then its v codes
+            self.pages = torch.zeros((*pool, 2, PAGE * HEAD_DIM), dtype=torch.uint8, device=dev)
+            self._scales = torch.full((*pool, 2), 2.0 ** -40, dtype=torch.float32, device=dev)
+        else:
+            # k codes, v codes, k scales, v scales
+            self.pages = torch.zeros((*pool, BLOCK4), dtype=torch.uint8, device=dev)
+            self._scales = None
         self._views = {}
         self._struct = _lib.Paged(self.n_q, self.n_kv, self.n_seqs, self.max_len, self.n_pages, self.n_layers,
                                   self.block_table.data_ptr(), self.lens.data_ptr(), self.free.data_ptr(),
                                   self.n_free.data_ptr(), self.pages.data_ptr() or None,
-                                  self._scales.data_ptr() or None)
+                                  None if self._scales is None else self._scales.data_ptr() or None)
         self._ref = ctypes.byref(self._struct)
 
     # -- tables ---------------------------------------------------------------
@@ -195,7 +213,7 @@ class PagedKVCache:
         if given; returns the rotated q, else None.  Tokens of rejected rows and
         past the step's last one are left out: their rows of q_out are not
         written, those of a new q are 0.  Each layer takes a step once: what a page
-        holds is coded again when its scale grows."""
+        of 8 bits holds is coded again when its scale grows."""
         plan, layer = self._plan(plan), self._layer(layer)
         k, hk = self._rows(k, self.n_kv, "k")
         v, hv = self._rows(v, self.n_kv, "v", k)
@@ -215,7 +233,8 @@ class PagedKVCache:
             raise ValueError("q_out without q")
         L = _lib.load_library()
         with _lib.on_device(self.device) as stream:
-            _lib.check(L.oi2_kv_append(
+            append = L.oi2_kv4_append if self.bits == 4 else L.oi2_kv_append
+            _lib.check(append(
                 self._ref, plan._ref, layer, _lib.dtype_code(k.dtype) | (_lib.ZERO_LEFT_OUT if q is not None and new else 0), n,
                 ctypes.byref(hk), ctypes.byref(hv),
                 None if rotary is None else rotary._ref,
@@ -243,11 +262,56 @@ class PagedKVCache:
         nbytes = plan._attend_bytes
         with _lib.on_device(self.device) as stream:
             ws = q.new_empty((nbytes,), dtype=torch.uint8)
-            _lib.check(L.oi2_kv_attend(
+            attend = L.oi2_kv4_attend if self.bits == 4 else L.oi2_kv_attend
+            _lib.check(attend(
                 self._ref, plan._ref, layer, dtype, n,
                 ctypes.byref(hq), HEAD_DIM ** -0.5 if scale is None else float(scale), out.data_ptr(),
                 ws.data_ptr(), nbytes, stream))
         return out
+
+    def _given(self, x: torch.Tensor, what: str, n: int, dtype) -> torch.Tensor:
+        if x.shape != (n, self.n_kv, HEAD_DIM) or x.dtype != dtype or x.device != self.device or x.stride(2) != 1:
+            raise ValueError(f"{what}: ({n}, {self.n_kv}, {HEAD_DIM}) {dtype} on {self.device} with a dense last dimension, "
+                             f"got {tuple(x.shape)} {x.dtype} on {x.device}")
+        return x
+
+    def fetch(self, layer: int, counts, max_tokens: int, first=None, dtype=torch.float16,
+              k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
+        """Positions [first[i], first[i] + counts[i]) of row i, cut to what it
+        holds (first: 0 by default), of all rows one behind the other, as what
+        they stand for: ``(k, v, cu)``, k and v (max_tokens, n_kv, 128) of
+        ``dtype`` (fp16, exactly; bf16, fp32), cu (n_seqs + 1) int32 the first
+        token of each row and the total.  counts and first: (n_seqs) int32 on the
+        device, or anything that converts to that (a list waits for its copy).
+        Tokens from max_tokens on are left out.  Rows past the last token are 0 in
+        new tensors and not written in k_out and v_out, which may have any strides
+        that keep their values apart.  A cache of 4 bits; nothing waits on the
+        host."""
+        layer = self._layer(layer)
+        if self.bits != 4:
+            raise ValueError("fetch takes a cache of 4 bits; read() a row of either")
+        n = int(max_tokens)
+        if n < 0 or n > 2 ** 31 - 1:
+            raise ValueError(f"{max_tokens} tokens")
+        if dtype not in (torch.float16, torch.bfloat16, torch.float32):
+            raise TypeError(f"{dtype}: float16, bfloat16 or float32")
+        if (k_out is None) != (v_out is None):
+            raise ValueError("k_out and v_out together")
+        new = k_out is None
+        counts, first = self._lens(counts), None if first is None else self._lens(first)
+        L = _lib.load_library()
+        with _lib.on_device(self.device) as stream:
+            if new:
+                kv = torch.empty((2, n, self.n_kv, HEAD_DIM), dtype=dtype, device=self.device)
+                k_out, v_out = kv[0], kv[1]
+            else:
+                k_out, v_out = self._given(k_out, "k_out", n, dtype), self._given(v_out, "v_out", n, dtype)
+            cu = torch.empty(self.n_seqs + 1, dtype=torch.int32, device=self.device)
+            hk, hv = _lib.heads(k_out, self.n_kv)[1], _lib.heads(v_out, self.n_kv)[1]
+            _lib.check(L.oi2_kv4_fetch(
+                self._ref, layer, _lib.ptr(first), counts.data_ptr(), _lib.dtype_code(dtype) | (_lib.ZERO_LEFT_OUT if new else 0), n,
+                ctypes.byref(hk), ctypes.byref(hv), cu.data_ptr(), stream))
+        return k_out, v_out, cu
 
     # -- views ----------------------------------------------------------------
     def codes(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -255,13 +319,38 @@ class PagedKVCache:
         4, 4, 4, 8, 16) and v (n_pages, n_kv, 4, 16, 8, 16), whose last two
         dimensions are the 128 dims and the ones before them the 64 positions of
         a page, in order; the memory holds them in the order of the attention's
-        loads."""
+        loads.  Of 4 bits, as copies: int8 (n_pages, n_kv, 64, 128)."""
+        if self.bits == 4:
+            return self._codes4(self._layer(layer))
         return self._layer_views(layer)[0]
 
     def scales(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The scales (n_pages, n_kv) of k and of v, as views: powers of two;
-        v's is negative where the page holds a NaN in v."""
+        v's is negative where the page holds a NaN in v.  Of 4 bits, fp16: k's
+        (n_pages, n_kv, 4, 4, 4, 4) and v's (n_pages, n_kv, 64, 4), positions of a
+        page and then groups of 32 dims."""
+        if self.bits == 4:
+            x = self.pages[self._layer(layer)].view(torch.float16)
+            k, v = x[..., BLOCK4 // 2 - 512:BLOCK4 // 2 - 256], x[..., BLOCK4 // 2 - 256:]
+            # k's memory: groups, places / 16, places % 4, places / 4 % 4
+            return (k.unflatten(-1, (4, 4, 4, 4)).permute(0, 1, 3, 5, 4, 2), v.unflatten(-1, (4, PAGE)).transpose(2, 3))
         return self._layer_views(layer)[1]
+
+    def _codes4(self, layer: int):
+        x = self.pages[layer][..., :PAGE * HEAD_DIM].view(torch.int32)
+        # k's memory: places / 4 % 4, groups, places / 16, places % 4, dwords of a
+        # group; v's: places / 4 % 4, places / 16, dwords, places % 4
+        k = x[..., :1024].unflatten(-1, (4, 4, 4, 4, 4)).permute(0, 1, 4, 2, 5, 3, 6)
+        v = x[..., 1024:].unflatten(-1, (4, 4, 16, 4)).permute(0, 1, 3, 2, 5, 4)
+        e = torch.arange(4, device=self.device, dtype=torch.int32)
+        at = torch.cat([8 * e, 8 * e + 4])               # magnitudes
+        sign = torch.cat([8 * e + 7, (8 * e + 11) % 32])
+
+        def values(d):
+            d = d.reshape(self.n_pages, self.n_kv, PAGE, 16, 1)
+            n = (d >> at) & 7
+            return torch.where(((d >> sign) & 1) != 0, -n, n).to(torch.int8).flatten(3)
+        return values(k), values(v)
 
     def _layer_views(self, layer: int):
         layer = self._layer(layer)
@@ -277,6 +366,11 @@ class PagedKVCache:
         """What a row's cache stands for: k and v (n_kv, length, 128), as the
         reference lays a cache out.  Waits for the row's length."""
         n = int(self.lens[row])
+        if self.bits == 4:
+            counts = torch.zeros(self.n_seqs, dtype=torch.int32, device=self.device)
+            counts[row] = n
+            k, v, _ = self.fetch(layer, counts, n, dtype=torch.float32)
+            return k.transpose(0, 1).to(dtype).contiguous(), v.transpose(0, 1).to(dtype).contiguous()
         ids = self.block_table[row, :-(-n // PAGE)].long()
         out = []
         for c, s in zip(self.codes(layer), self.scales(layer)):

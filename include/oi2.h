@@ -587,6 +587,59 @@ int oi2_attn_forward_paged(const uint16_t* x, int32_t n_tokens, const oi2_attn* 
                            uint16_t* out, uint16_t* x_out, void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/* ---- paged 4-bit KV cache ------------------------------------------------ */
+/* The same rows, tables and plans (oi2_page_extend, oi2_page_rewind) over pages
+ * that hold 4 bits a value.  A head's 128 values are four groups of 32 dims; a
+ * group x stands for n s, whole n in [-7, 7]:
+ *   s = max |x| / 7 rounded to nearest (even) with 8 significant bits, at least
+ *       2^-24, in multiples of it, and at most 9344; 0 where all of x is 0
+ *   n = x / s rounded to nearest (even), at most 7 in magnitude
+ * so that n s is exact in fp16; magnitudes past 65408 (of bf16) are held as that.
+ * A group that holds a NaN or an infinity is NaN, which a row's attention returns
+ * where it sees it.  A position is coded by itself: nothing that a page holds
+ * changes when it grows.
+ *
+ * oi2_paged.pages: (layer, page, kv head) blocks of 9216 bytes, 16-byte aligned;
+ * oi2_paged.scales is not used.  A block holds the codes of k, those of v at 4096,
+ * k's scales (fp16) at 8192, v's at 8704, in the order in which the attention
+ * loads them, a dword u for dims 8 u .. 8 u + 7:
+ *   k, position p: 1024 (p / 4 % 4) + 256 (u / 4) + 16 (4 (p / 16) + p % 4) + 4 (u % 4)
+ *   v, position p: 1024 (p / 4 % 4) + 256 (p / 16) + 16 u + 4 (p % 4)
+ *   scale of group c, k: 8 (16 c + 4 (p / 16) + p % 4) + 2 (p / 4 % 4); v: 128 c + 2 p
+ * Codes are sign and magnitude.  Value e < 4 of a dword: magnitude at its bit
+ * 8 e, sign at 8 e + 7; value 4 + e: magnitude at 8 e + 4, sign at
+ * (8 e + 11) % 32. */
+enum { OI2_KV4_BLOCK = 9216 };
+
+/* oi2_kv_append into such pages.  A token whose slot is not one of the pool's is
+ * left out.  A step may be appended again: it writes the same. */
+int oi2_kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
+                   const oi2_heads* k, const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q, void* q_out,
+                   void* stream);
+
+/* Positions [first[i], first[i] + count[i]) of row i, cut to what it holds
+ * (negative values count as 0; first NULL: from 0), of all rows one behind the
+ * other, as values: k and v (max_tokens, n_kv, 128) of `dtype` (OI2_DTYPE_F16,
+ * _BF16 or _F32), with strides, non-negative, that keep all values apart.  first
+ * and count (n_seqs) are device memory; cu (n_seqs + 1) gets the first token of
+ * each row and the total.  Tokens from max_tokens on are left out; rows of k and v
+ * past the last token are left as they were, or 0 with OI2_ZERO_LEFT_OUT. */
+int oi2_kv4_fetch(const oi2_paged* c, int32_t layer, const int32_t* first, const int32_t* count, int32_t dtype,
+                  int32_t max_tokens, const oi2_heads* k, const oi2_heads* v, int32_t* cu, void* stream);
+
+/* oi2_kv_attend over such pages, with the workspace of
+ * oi2_kv_attend_workspace_bytes. */
+int oi2_kv4_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
+                   const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* oi2_attn_forward_paged over such pages, with the workspace of
+ * oi2_attn_paged_workspace_bytes. */
+int oi2_kv4_attn_forward(const uint16_t* x, int32_t n_tokens, const oi2_attn* w, float eps,
+                         const oi2_rotary* rotary, const oi2_paged* c, const oi2_page_plan* p, int32_t layer,
+                         uint16_t* out, uint16_t* x_out, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 /* oi2_predict_select for the n_tokens packed tokens of the plan's step, x
  * (n_tokens, H) fp16: the query is the mean over the last token of every row
  * that is taken and has tokens among them, as the batch of those tokens gives
