@@ -3,8 +3,9 @@
 //
 // One launch.  Every workgroup makes the rows' prefix sums for itself, in LDS (a
 // launch of its own for them would cost more than they do), and then takes
-// every so-many-th set of 16 tokens; a wave has four tokens, 16 lanes and 8 dims a
-// lane each, and goes over kv heads, which is how the append writes them.
+// pages of one kv head, every so-many-th of what is read: what lies in a line of
+// memory, or in a page's scales, is read by one workgroup, and its position in
+// the table by scalar loads.
 #include "capi_util.h"
 #include "kv4.h"
 #include "rotary.h"
@@ -12,13 +13,12 @@
 namespace oi2 {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kThreads = 256, kWaves = kThreads / 64, kMostGroups = 2048;
 
 struct FetchArgs {
   const int32_t *table, *lens, *first, *count;
   int32_t* cu;
   int n_seqs, width, max_len, n_pages, n_kv, max_tokens;
-  int heads_each, chunks;     // kv heads of a wave's turn, and how many turns a token's heads take
   int zero, wide;             // wide: 16-byte stores
   const uint8_t* pages;       // of the layer
   void* dst[2];               // k, v
@@ -45,8 +45,8 @@ __device__ __forceinline__ void store8(void* base, int64_t at, const f16x2 (&y)[
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] = (float)y[e / 2][e % 2];
     if (wide) {
-      *reinterpret_cast<f32x4*>(p) = f32x4{z[0], z[1], z[2], z[3]};
-      *reinterpret_cast<f32x4*>(p + 4) = f32x4{z[4], z[5], z[6], z[7]};
+      __builtin_nontemporal_store(f32x4{z[0], z[1], z[2], z[3]}, reinterpret_cast<f32x4*>(p));
+      __builtin_nontemporal_store(f32x4{z[4], z[5], z[6], z[7]}, reinterpret_cast<f32x4*>(p + 4));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] = z[e];
@@ -59,7 +59,7 @@ __device__ __forceinline__ void store8(void* base, int64_t at, const f16x2 (&y)[
       z[e] = DTYPE == OI2_DTYPE_F16 ? __builtin_bit_cast(uint32_t, y[e])
                                     : narrow<true>((float)y[e][0]) | (uint32_t)narrow<true>((float)y[e][1]) << 16;
     if (wide) {
-      *reinterpret_cast<u32x4*>(p) = u32x4{z[0], z[1], z[2], z[3]};
+      __builtin_nontemporal_store(u32x4{z[0], z[1], z[2], z[3]}, reinterpret_cast<u32x4*>(p));
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -74,76 +74,92 @@ constexpr uint32_t kMost = 0x7FFFFFFF;
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return min(a + b, kMost); }
 
 template <int DTYPE>
-__global__ __launch_bounds__(kThreads) void k_kv4_fetch(FetchArgs a) {
+__global__ __launch_bounds__(kThreads, 8) void k_kv4_fetch(FetchArgs a) {
   extern __shared__ int32_t lds[];
-  __shared__ uint32_t s_wave[kWaves];
-  const int n = a.n_seqs, tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
-  int32_t* s_end = lds;              // inclusive sums of the rows' tokens
-  int32_t* s_first = s_end + n;      // first position that is read
+  __shared__ uint2 s_wave[kWaves];
+  const int n = a.n_seqs, tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // inclusive sums of the rows' tokens and of the pages that they lie in; the
+  // first position of each row
+  int32_t *s_tokens = lds, *s_pages = lds + n, *s_first = lds + 2 * n;
   const int per = (n + kThreads - 1) / kThreads, r0 = min(tid * per, n), r1 = min(r0 + per, n);
-  uint32_t mine = 0;
+  uint2 mine = {0, 0};
   for (int r = r0; r < r1; ++r) {
     const int len = min(max(a.lens[r], 0), a.max_len), f = a.first ? min(max(a.first[r], 0), len) : 0;
     const int count = min(max(a.count[r], 0), len - f);
+    mine.x = add_sat(mine.x, (uint32_t)count);
+    mine.y = add_sat(mine.y, count ? (uint32_t)((f + count - 1) / kPage - f / kPage + 1) : 0);
     s_first[r] = f;
-    mine = add_sat(mine, (uint32_t)count);
-    s_end[r] = (int)mine;
+    s_tokens[r] = (int)mine.x;
+    s_pages[r] = (int)mine.y;
   }
-  uint32_t before = mine;            // of the wave's lanes up to this one
+  uint2 upto = mine;                 // of the wave's lanes up to this one
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const uint32_t x = (uint32_t)__shfl_up((int)before, d);
-    if (lane >= d) before = add_sat(before, x);
+    const uint32_t x = (uint32_t)__shfl_up((int)upto.x, d), y = (uint32_t)__shfl_up((int)upto.y, d);
+    if (lane >= d) upto = uint2{add_sat(upto.x, x), add_sat(upto.y, y)};
   }
-  if (lane == 63) s_wave[wave] = before;
-  uint32_t base = (uint32_t)__shfl_up((int)before, 1);
-  if (lane == 0) base = 0;
+  if (lane == 63) s_wave[wave] = upto;
+  uint2 base = {(uint32_t)__shfl_up((int)upto.x, 1), (uint32_t)__shfl_up((int)upto.y, 1)};
+  if (lane == 0) base = uint2{0, 0};
   __syncthreads();
-  for (int w = 0; w < wave; ++w) base = add_sat(base, s_wave[w]);
-  for (int r = r0; r < r1; ++r) s_end[r] = (int)add_sat((uint32_t)s_end[r], base);
+  for (int w = 0; w < wave; ++w) base = uint2{add_sat(base.x, s_wave[w].x), add_sat(base.y, s_wave[w].y)};
+  for (int r = r0; r < r1; ++r) {
+    s_tokens[r] = (int)add_sat((uint32_t)s_tokens[r], base.x);
+    s_pages[r] = (int)add_sat((uint32_t)s_pages[r], base.y);
+  }
   __syncthreads();
   if (blockIdx.x == 0)
-    for (int r = tid; r <= n; r += kThreads) a.cu[r] = r ? s_end[r - 1] : 0;
-  const int total = min(s_end[n - 1], a.max_tokens), tokens = a.zero ? a.max_tokens : total;
+    for (int r = tid; r <= n; r += kThreads) a.cu[r] = r ? s_tokens[r - 1] : 0;
+  const int total = min(s_tokens[n - 1], a.max_tokens);
 
-  const int u = lane & 15;
-  const int64_t tasks = ((int64_t)tokens + 3) / 4 * a.chunks;
-  for (int64_t task = (int64_t)blockIdx.x * kWaves + wave; task < tasks; task += (int64_t)gridDim.x * kWaves) {
-    const int64_t quad = task / a.chunks;
-    const int g0 = (int)(task - quad * a.chunks) * a.heads_each, g1 = min(g0 + a.heads_each, a.n_kv);
-    const int64_t t = 4 * quad + (lane >> 4);
-    if (t >= tokens) continue;
-    int64_t at[2];
-#pragma unroll
-    for (int w = 0; w < 2; ++w) at[w] = t * a.token_stride[w] + 8 * u;
-    if (t >= total) {
-      const f16x2 none[4] = {};
-      for (int g = g0; g < g1; ++g)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) store8<DTYPE>(a.dst[w], at[w] + g * a.head_stride[w], none, a.wide);
-      continue;
-    }
-    int lo = 0, hi = n - 1;          // the first row that ends past t
+  // A wave has the places 4 wave + 16 k + i of a page, four at a time, whose
+  // codes are 1 KB of k's and 1 KB of v's.
+  const int u = lane & 15, i = lane >> 4, p0 = 4 * wave + i;
+  const int k_at = k4_at(p0, u), v_at = v4_at(p0, u), ks_at = k4_scale_at(p0, u / 4), vs_at = v4_scale_at(p0, u / 4);
+  const int64_t units = (int64_t)s_pages[n - 1] * a.n_kv;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int page = (int)(unit / a.n_kv), g = (int)(unit - (int64_t)page * a.n_kv);
+    int lo = 0, hi = n - 1;          // the first row whose pages end past this one
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (s_end[mid] > t) hi = mid;
+      if (s_pages[mid] > page) hi = mid;
       else lo = mid + 1;
     }
-    const int pos = s_first[lo] + (int)t - (lo ? s_end[lo - 1] : 0), p = pos % kPage;
-    int id = a.table[(int64_t)lo * a.width + pos / kPage];
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int t0 = lo ? s_tokens[lo - 1] : 0, t1 = min(s_tokens[lo], total);   // the row's tokens
+    const int f = s_first[lo], j = f / kPage + page - (lo ? s_pages[lo - 1] : 0);
+    int id = a.table[(int64_t)lo * a.width + j];
     id = (unsigned)id < (unsigned)a.n_pages ? id : 0;       // a damaged table reads page 0
-    const uint8_t* block = a.pages + (int64_t)id * a.n_kv * k4Block;
-#pragma unroll 4
-    for (int g = g0; g < g1; ++g) {
-      const uint8_t* b = block + (int64_t)g * k4Block;
-      const uint32_t kd = *reinterpret_cast<const uint32_t*>(b + k4_at(p, u)), vd = *reinterpret_cast<const uint32_t*>(b + v4_at(p, u));
-      const uint16_t ks = *reinterpret_cast<const uint16_t*>(b + k4_scale_at(p, u / 4));
-      const uint16_t vs = *reinterpret_cast<const uint16_t*>(b + v4_scale_at(p, u / 4));
+    const rsrc_t b = rsrc(a.pages + ((int64_t)id * a.n_kv + g) * k4Block, k4Block);
+    uint32_t kd[4], vd[4];
+    uint16_t ks[4], vs[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {    // places 4 wave + 16 k + i
+      kd[k] = bld4(b, k_at + 64 * k);
+      vd[k] = bld4(b, v_at + 256 * k);
+      ks[k] = bld2(b, ks_at + 32 * k);
+      vs[k] = bld2(b, vs_at + 32 * k);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t t = (int64_t)t0 + j * kPage + p0 + 16 * k - f;
+      if (t < t0 || t >= t1) continue;
       f16x2 y[4];
-      values8(y, kd, ks);
-      store8<DTYPE>(a.dst[0], at[0] + g * a.head_stride[0], y, a.wide);
-      values8(y, vd, vs);
-      store8<DTYPE>(a.dst[1], at[1] + g * a.head_stride[1], y, a.wide);
+      values8(y, kd[k], ks[k]);
+      store8<DTYPE>(a.dst[0], t * a.token_stride[0] + g * a.head_stride[0] + 8 * u, y, a.wide);
+      values8(y, vd[k], vs[k]);
+      store8<DTYPE>(a.dst[1], t * a.token_stride[1] + g * a.head_stride[1] + 8 * u, y, a.wide);
+    }
+  }
+
+  if (a.zero) {
+    const f16x2 none[4] = {};
+    const int64_t rest = (int64_t)(a.max_tokens - total) * a.n_kv * 16;
+    for (int64_t x = (int64_t)blockIdx.x * kThreads + tid; x < rest; x += (int64_t)gridDim.x * kThreads) {
+      const int64_t t = total + x / (a.n_kv * 16);
+      const int g = (int)(x / 16 % a.n_kv), w = (int)(x % 16);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) store8<DTYPE>(a.dst[e], t * a.token_stride[e] + g * a.head_stride[e] + 8 * w, none, a.wide);
     }
   }
 }
@@ -211,11 +227,10 @@ extern "C" int oi2_kv4_fetch(const oi2_paged* c, int32_t layer, const int32_t* f
   a.max_tokens = max_tokens;
   a.zero = zero;
   a.pages = c->pages + (size_t)layer * c->n_pages * c->n_kv * k4Block;
-  a.heads_each = c->n_kv < 4 ? c->n_kv : 4;
-  a.chunks = (c->n_kv + a.heads_each - 1) / a.heads_each;
-  const int64_t want = (((int64_t)max_tokens + 3) / 4 * a.chunks + kWaves - 1) / kWaves;
-  const uint32_t groups = (uint32_t)(want < 1 ? 1 : want < 2048 ? want : 2048);
-  const size_t lds = (size_t)c->n_seqs * 8;
+  // a page of one kv head is a workgroup's turn
+  const int64_t rows = c->n_seqs < max_tokens ? c->n_seqs : max_tokens, want = ((int64_t)max_tokens / kPage + 2 * rows) * c->n_kv;
+  const uint32_t groups = (uint32_t)(want < 1 ? 1 : want < kMostGroups ? want : kMostGroups);
+  const size_t lds = (size_t)c->n_seqs * 12;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid(groups), block(kThreads);
   if (dtype == OI2_DTYPE_F16) hipLaunchKernelGGL(k_kv4_fetch<OI2_DTYPE_F16>, grid, block, lds, st, a);
