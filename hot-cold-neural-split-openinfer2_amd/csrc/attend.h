@@ -104,8 +104,11 @@ __device__ __forceinline__ Probs to_probs(const float (&e)[8]) {
   for (int k = 0; k < 4; ++k) {
     const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(e[2 * k], e[2 * k + 1]));
     uh[k] = hi;
-    ul[k] = __builtin_bit_cast(
-        uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(half_lo(hi), -1.0f, e[2 * k]), fmaf(half_hi(hi), -1.0f, e[2 * k + 1])));
+    // e - hi, exact; as mixed multiply-adds, which the compiler makes two instructions of
+    float l0, l1;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l0) : "v"(hi), "v"(e[2 * k]));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(l1) : "v"(hi), "v"(e[2 * k + 1]));
+    ul[k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(l0, l1));
   }
   return {__builtin_bit_cast(h8, uh), __builtin_bit_cast(h8, ul)};
 }
@@ -118,9 +121,13 @@ __device__ __forceinline__ float score_scale(float sc, float k_scale) {
   return __builtin_amdgcn_fmed3f(fabsf(sc) * k_scale, 7.52316385e-37f, 3.40282347e38f);
 }
 
+__device__ __forceinline__ float half_max(float v) {   // over the lanes l, l ^ 32
+  const u32x2v x = __builtin_bit_cast(u32x2v, __builtin_amdgcn_permlane32_swap(as_u32(v), as_u32(v), false, false));
+  return fmaxf(as_f32(x.x), as_f32(x.y));
+}
 __device__ __forceinline__ float quad_max(float v) {   // over the lanes l, l ^ 16, l ^ 32, l ^ 48
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  const u32x2v x = __builtin_bit_cast(u32x2v, __builtin_amdgcn_permlane16_swap(as_u32(v), as_u32(v), false, false));
+  return half_max(fmaxf(as_f32(x.x), as_f32(x.y)));
 }
 
 constexpr int kThreads = 256;
@@ -548,7 +555,7 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
     for (int T = 0; T < 2; ++T)
 #pragma unroll
       for (int j = 0; j < 16; ++j) cm = fmaxf(cm, s[T][j]);
-    cm = fmaf(fmaxf(cm, __shfl_xor(cm, 32)), ksc, ev);
+    cm = fmaf(half_max(cm), ksc, ev);
     const bool up = cm > m + kSlack;
     if (__any(up)) {
       const float mn = up ? cm : m;
