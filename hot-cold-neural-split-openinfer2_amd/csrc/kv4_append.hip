@@ -2,11 +2,11 @@
 // way.
 //
 // A group of 32 values has a scale of its own, so every token is coded by
-// itself: a wave takes four tokens of the packed order, 16 lanes and 8 dims a
-// lane each, for one kv head or several; the largest magnitude goes over four
-// lanes.  Four tokens because a page keeps the dwords of four positions side by
-// side: their stores of v fill 256 bytes, those of k four times 64.  q has
-// workgroups of its own behind them in the same launch.
+// itself: 16 lanes take a token of the packed order and kv head, 8 dims a lane;
+// the largest magnitude goes over four lanes.  A workgroup takes 16 tokens, the
+// next one another head's: those of 64 tokens and one head, which share lines of
+// a page, are 8 apart or a multiple, on one XCD.  q has workgroups of its own
+// behind them in the same launch.
 #include "capi_util.h"
 #include "kv4.h"
 #include "rotary.h"
@@ -17,7 +17,7 @@ namespace {
 struct Append4Args {
   const int32_t* slots;       // the plan's
   int n_kv, n_pages, n_tokens, groups;    // groups: workgroups for k and v, before q's
-  int heads_each, chunks;     // kv heads of a wave, and how many waves take a token's
+  int heads_each, chunks;     // kv heads of a workgroup, and how many take a token's
   const uint16_t* src[2];     // k, v
   int64_t token_stride[2], head_stride[2];
   int q_wide;
@@ -74,41 +74,57 @@ __device__ __forceinline__ void load8(uint32_t (&x)[4], const uint16_t* p) {
   }
 }
 
-template <bool BF16, bool WIDE, Turns TURNS>
-__device__ __forceinline__ void append4(const Append4Args& a, int task) {
-  const int quad = task / a.chunks, g0 = (task - quad * a.chunks) * a.heads_each, g1 = min(g0 + a.heads_each, a.n_kv);
-  const int lane = lane_id(), u = lane & 15;
-  const int64_t t = 4 * (int64_t)quad + (lane >> 4);
-  const int slot = t < a.n_tokens ? a.slots[t] : -1;
-  if (slot < 0 || slot / kPage >= a.n_pages) return;     // a token's lanes together
-  const int p = slot % kPage;
-  const RotaryArgs& r = a.rope;
-  const uint16_t* pk = a.src[0] + t * a.token_stride[0] + 8 * u;
-  const uint16_t* pv = a.src[1] + t * a.token_stride[1] + 8 * u;
+// A workgroup has 16 tokens of one kv head or several, whose cosines and sines its
+// threads share.
+constexpr int kTokens = 16, kPairs = kHeadD / 2;
 
-  // cosines and sines of this lane's pairs, for every head; the first dim of a
-  // pair is turned as c a - s b, the second as s a + c b
+template <bool BF16, bool WIDE, Turns TURNS>
+__device__ __forceinline__ void append4(const Append4Args& a, int b) {
+  const int set = b / a.chunks, g0 = (b - set * a.chunks) * a.heads_each, g1 = min(g0 + a.heads_each, a.n_kv);
+  const int tid = threadIdx.x, u = tid & 15, in = tid >> 4;
+  const int64_t t = kTokens * (int64_t)set + in;
+  const bool have = t < a.n_tokens;
+  const RotaryArgs& r = a.rope;
+  const int64_t row = have ? t : a.n_tokens - 1;
+  const uint16_t* pk = a.src[0] + row * a.token_stride[0] + 8 * u;
+  const uint16_t* pv = a.src[1] + row * a.token_stride[1] + 8 * u;
+  uint32_t nk[4], nv[4];
+  load8<BF16, WIDE>(nk, pk + g0 * a.head_stride[0]);
+  load8<BF16, WIDE>(nv, pv + g0 * a.head_stride[1]);
+  const int slot = have ? a.slots[t] : -1;
+
+  // Cosines and sines of this lane's pairs, for every head; the first dim of a
+  // pair is turned as c a - s b, the second as s a + c b.
   constexpr int N = TURNS == kNone ? 1 : TURNS == kNeighbours ? 4 : 8;
   CosSin cs[N];
   const int pairs = r.rot / 2;
   if constexpr (TURNS != kNone) {
-    const int pos = r.positions[t];
+    __shared__ __align__(16) CosSin s_turn[kTokens * kPairs];
+    // thread: pairs u, u + 16 .. of its token
+    const int pos = r.positions[row];
+#pragma unroll
+    for (int e = 0; e < kPairs / 16; ++e) {
+      const int j = u + 16 * e;
+      if (j >= pairs) continue;
+      CosSin x = turn(r.freq[j], pos);
+      x.c *= r.magnitude;
+      x.s *= r.magnitude;
+      s_turn[in * kPairs + j] = x;
+    }
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const int d = 8 * u + (TURNS == kNeighbours ? 2 * e : e);
       if (d >= r.rot) continue;
       const int j = TURNS == kNeighbours ? d / 2 : d < pairs ? d : d - pairs;
-      cs[e] = turn(r.freq[j], pos);
-      cs[e].c *= r.magnitude;
-      cs[e].s *= r.magnitude;
+      cs[e] = s_turn[in * kPairs + j];
       if (TURNS != kNeighbours && d >= pairs) cs[e] = CosSin{cs[e].s, cs[e].c};
     }
   }
+  if (slot < 0 || slot / kPage >= a.n_pages) return;     // a token's lanes together
+  const int p = slot % kPage, lane = lane_id();
   const int other = TURNS != kAligned || 8 * u >= r.rot ? lane : 8 * u < pairs ? lane + pairs / 8 : lane - pairs / 8;
 
-  uint32_t nk[4], nv[4];
-  load8<BF16, WIDE>(nk, pk + g0 * a.head_stride[0]);
-  load8<BF16, WIDE>(nv, pv + g0 * a.head_stride[1]);
   for (int g = g0; g < g1; ++g) {
     uint32_t k[4], v[4];
 #pragma unroll
@@ -177,7 +193,7 @@ __device__ __forceinline__ void append4(const Append4Args& a, int task) {
 template <bool BF16, bool WIDE, Turns TURNS>
 __global__ __launch_bounds__(256) void k_kv4_append(Append4Args a) {
   const int b = blockIdx.x;
-  if (b < a.groups) append4<BF16, WIDE, TURNS>(a, 4 * b + (int)(threadIdx.x >> 6));
+  if (b < a.groups) append4<BF16, WIDE, TURNS>(a, b);
   else if constexpr (TURNS != kNone) {
     if (a.q_wide) rotate_tokens<BF16, true, 256>(a.rope, b - a.groups);
     else rotate_tokens<BF16, false, 256>(a.rope, b - a.groups);
@@ -231,9 +247,12 @@ extern "C" int oi2_kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_
     if ((uintptr_t)in[w]->data % 16 || in[w]->token_stride % 8 || in[w]->head_stride % 8) wide = false;
   }
   a.pages = c->pages + (size_t)layer * c->n_pages * c->n_kv * k4Block;
+  // heads share their turns while 1024 workgroups are left
+  const int64_t sets = ((int64_t)n_tokens + kTokens - 1) / kTokens;
   a.heads_each = 1;
+  while (r && a.heads_each < c->n_kv && sets * c->n_kv / (2 * a.heads_each) >= 1024) a.heads_each *= 2;
   a.chunks = (c->n_kv + a.heads_each - 1) / a.heads_each;
-  const int64_t waves = ((int64_t)n_tokens + 3) / 4 * a.chunks, pages = (waves + 3) / 4;
+  const int64_t pages = sets * a.chunks;
   int64_t rows = 0;
   Turns turns = kNone;
   if (r) {
