@@ -67,7 +67,7 @@ __device__ __forceinline__ uint32_t code8(const uint32_t (&x)[4], uint16_t& scal
 template <bool BF16, bool WIDE>
 __device__ __forceinline__ void load8(uint32_t (&x)[4], const uint16_t* p) {
   if constexpr (WIDE) {
-    *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(p);
+    *reinterpret_cast<u32x4*>(x) = load16_nt(reinterpret_cast<const uint8_t*>(p));
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
@@ -195,8 +195,8 @@ __global__ __launch_bounds__(256) void k_kv4_append(Append4Args a) {
   const int b = blockIdx.x;
   if (b < a.groups) append4<BF16, WIDE, TURNS>(a, b);
   else if constexpr (TURNS != kNone) {
-    if (a.q_wide) rotate_tokens<BF16, true, 256>(a.rope, b - a.groups);
-    else rotate_tokens<BF16, false, 256>(a.rope, b - a.groups);
+    if (a.q_wide) rotate_tokens<BF16, true, 256, true>(a.rope, b - a.groups);
+    else rotate_tokens<BF16, false, 256, true>(a.rope, b - a.groups);
   }
 }
 

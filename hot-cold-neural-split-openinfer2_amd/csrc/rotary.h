@@ -105,24 +105,27 @@ struct RotaryArgs {
 // Cosines and sines of a workgroup's tokens: kTurns at most.
 constexpr int kTurns = 256;
 
-// The heads of tokens_each tokens by a workgroup of NT threads.  Their cosines
+// The heads of tokens_each tokens by a workgroup of THREADS threads.  Their cosines
 // and sines are made once, in LDS, while the first heads are on their way; a
 // thread takes eight pairs of a head in WIDE (16-byte loads and stores: pairs
 // 8 u .. of the rotated part, or 16 dims behind it; needs a rotary_dim and
 // head_dim that 16 divides and rows at 16-byte addresses), otherwise one pair,
-// and then the same of the head NT / per_head further on, whose loads are under
-// way while this one is turned.  12001 tokens of 32 + 8 heads out of cache 47 us
+// and then the same of the head THREADS / per_head further on, whose loads are under
+// way while this one is turned.  NT: non-temporal loads, as of inputs that nothing
+// reads again: behind 600 MB of writes 5875 tokens of 32 heads take 20.6 us instead
+// of 30.4; calls one by one on what is in the caches 68 instead of 62 (12001 tokens
+// of 40 heads).  12001 tokens of 32 + 8 heads out of cache 47 us
 // (5.2 TB/s); with the turns made by each thread for up to 8 heads of its own
 // 51.5, for 2 of them 56.
-template <bool BF16, bool WIDE, int NT>
+template <bool BF16, bool WIDE, int THREADS, bool NT = false>
 __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int b) {
   constexpr int P = WIDE ? 8 : 1;
-  static_assert(NT >= kTurns);
+  static_assert(THREADS >= kTurns);
   __shared__ __align__(16) CosSin s_turn[kTurns];
   __shared__ int s_pos[kTurns];
   const int tid = threadIdx.x, t0 = b * a.tokens_each, nt = min(a.tokens_each, a.n_tokens - t0);
   const int pairs = a.rot / 2, lanes = pairs / P, all = a.heads[0] + a.heads[1];
-  const int slot = tid / a.per_head, slots = NT / a.per_head, u = tid - slot * a.per_head;
+  const int slot = tid / a.per_head, slots = THREADS / a.per_head, u = tid - slot * a.per_head;
   const bool rotate = u < lanes, halves = rotate && !a.interleaved;
   const int d0 = halves ? P * u : 2 * P * u, d1 = halves ? P * u + pairs : 2 * P * u + P;
   uint16_t v[2 * P], ahead[2 * P];
@@ -131,8 +134,9 @@ __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int b) {
     const uint16_t* p = (w ? a.src[1] : a.src[0]) + (int64_t)(t0 + t) * (w ? a.token_stride[1] : a.token_stride[0]) +
                         (w ? h - a.heads[0] : h) * (w ? a.head_stride[1] : a.head_stride[0]);
     if constexpr (WIDE) {
-      *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(p + d0);
-      *reinterpret_cast<u32x4*>(x + 8) = *reinterpret_cast<const u32x4*>(p + d1);
+      const uint8_t *p0 = reinterpret_cast<const uint8_t*>(p + d0), *p1 = reinterpret_cast<const uint8_t*>(p + d1);
+      *reinterpret_cast<u32x4*>(x) = NT ? load16_nt(p0) : load16(p0);
+      *reinterpret_cast<u32x4*>(x + 8) = NT ? load16_nt(p1) : load16(p1);
     } else {
       x[0] = p[d0];
       x[1] = p[d1];

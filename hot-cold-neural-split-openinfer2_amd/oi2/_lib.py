@@ -282,6 +282,19 @@ class on_device:
             torch.cuda.set_device(self.before)
 
 
+def launch(device: torch.device, fn, *args) -> None:
+    """fn(*args, stream) with ``device`` current, on its current stream, its
+    status checked: on_device's, at half the cost where the device is current."""
+    index = device.index
+    if torch.cuda.is_initialized() and torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index) or None)
+    else:
+        with on_device(device) as stream:
+            rc = fn(*args, stream)
+    if rc != OI2_OK:
+        check(rc)
+
+
 def heads(x: torch.Tensor, n: int) -> tuple[torch.Tensor, Heads]:
     """(tokens, n heads, dim) as the C ABI takes it, and the tensor that it
     points into: x, or a copy where its last dimension is not dense."""

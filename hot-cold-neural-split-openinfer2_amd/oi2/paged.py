@@ -149,6 +149,8 @@ class PagedKVCache:
     def _lens(self, lens) -> torch.Tensor:
         if not isinstance(lens, torch.Tensor):
             lens = torch.tensor(lens, dtype=torch.int32)
+        if lens.dtype is torch.int32 and lens.shape == self.lens.shape and lens.device == self.device and lens.is_contiguous():
+            return lens
         if lens.shape != (self.n_seqs,) or lens.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"lengths: ({self.n_seqs},) int32, got {tuple(lens.shape)} {lens.dtype}")
         if lens.dtype == torch.int64:
@@ -232,13 +234,10 @@ class PagedKVCache:
         elif q_out is not None:
             raise ValueError("q_out without q")
         L = _lib.load_library()
-        with _lib.on_device(self.device) as stream:
-            append = L.oi2_kv4_append if self.bits == 4 else L.oi2_kv_append
-            _lib.check(append(
-                self._ref, plan._ref, layer, _lib.dtype_code(k.dtype) | (_lib.ZERO_LEFT_OUT if q is not None and new else 0), n,
-                ctypes.byref(hk), ctypes.byref(hv),
-                None if rotary is None else rotary._ref,
-                None if q is None else ctypes.byref(hq), _lib.ptr(q_out), stream))
+        _lib.launch(self.device, L.oi2_kv4_append if self.bits == 4 else L.oi2_kv_append,
+                    self._ref, plan._ref, layer, _lib.dtype_code(k.dtype) | (_lib.ZERO_LEFT_OUT if q is not None and new else 0), n,
+                    ctypes.byref(hk), ctypes.byref(hv), None if rotary is None else rotary._ref,
+                    None if q is None else ctypes.byref(hq), _lib.ptr(q_out))
         return q_out
 
     def attend(self, layer: int, q: torch.Tensor, plan: PagePlan, scale: float | None = None,
@@ -260,13 +259,10 @@ class PagedKVCache:
             raise ValueError("out must be a contiguous tensor like q")
         L = _lib.load_library()
         nbytes = plan._attend_bytes
-        with _lib.on_device(self.device) as stream:
-            ws = q.new_empty((nbytes,), dtype=torch.uint8)
-            attend = L.oi2_kv4_attend if self.bits == 4 else L.oi2_kv_attend
-            _lib.check(attend(
-                self._ref, plan._ref, layer, dtype, n,
-                ctypes.byref(hq), HEAD_DIM ** -0.5 if scale is None else float(scale), out.data_ptr(),
-                ws.data_ptr(), nbytes, stream))
+        ws = q.new_empty((nbytes,), dtype=torch.uint8)
+        _lib.launch(self.device, L.oi2_kv4_attend if self.bits == 4 else L.oi2_kv_attend,
+                    self._ref, plan._ref, layer, dtype, n, ctypes.byref(hq),
+                    HEAD_DIM ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), nbytes)
         return out
 
     def _given(self, x: torch.Tensor, what: str, n: int, dtype) -> torch.Tensor:
@@ -297,20 +293,19 @@ class PagedKVCache:
             raise TypeError(f"{dtype}: float16, bfloat16 or float32")
         if (k_out is None) != (v_out is None):
             raise ValueError("k_out and v_out together")
-        new = k_out is None
         counts, first = self._lens(counts), None if first is None else self._lens(first)
-        L = _lib.load_library()
-        with _lib.on_device(self.device) as stream:
-            if new:
-                kv = torch.empty((2, n, self.n_kv, HEAD_DIM), dtype=dtype, device=self.device)
-                k_out, v_out = kv[0], kv[1]
-            else:
-                k_out, v_out = self._given(k_out, "k_out", n, dtype), self._given(v_out, "v_out", n, dtype)
-            cu = torch.empty(self.n_seqs + 1, dtype=torch.int32, device=self.device)
-            hk, hv = _lib.heads(k_out, self.n_kv)[1], _lib.heads(v_out, self.n_kv)[1]
-            _lib.check(L.oi2_kv4_fetch(
-                self._ref, layer, _lib.ptr(first), counts.data_ptr(), _lib.dtype_code(dtype) | (_lib.ZERO_LEFT_OUT if new else 0), n,
-                ctypes.byref(hk), ctypes.byref(hv), cu.data_ptr(), stream))
+        code = _lib.dtype_code(dtype)
+        if k_out is None:
+            code |= _lib.ZERO_LEFT_OUT
+            k_out = torch.empty((n, self.n_kv, HEAD_DIM), dtype=dtype, device=self.device)
+            v_out = torch.empty_like(k_out)
+            st = self.n_kv * HEAD_DIM
+            hk, hv = _lib.Heads(k_out.data_ptr(), self.n_kv, st, HEAD_DIM), _lib.Heads(v_out.data_ptr(), self.n_kv, st, HEAD_DIM)
+        else:
+            hk, hv = (_lib.heads(self._given(x, what, n, dtype), self.n_kv)[1] for x, what in ((k_out, "k_out"), (v_out, "v_out")))
+        cu = counts.new_empty(self.n_seqs + 1)
+        _lib.launch(self.device, _lib.load_library().oi2_kv4_fetch, self._ref, layer, _lib.ptr(first), counts.data_ptr(), code, n,
+                    ctypes.byref(hk), ctypes.byref(hv), cu.data_ptr())
         return k_out, v_out, cu
 
     # -- views ----------------------------------------------------------------
