@@ -66,7 +66,6 @@ __device__ __forceinline__ T scalar_load(const T* p) {
   return v;
 }
 
-// Bytes [0, n) of a dword's four kept, the rest zero.
 // A NaN among v must not reach rows that do not see its position (their p is 0,
 // and 0 times it NaN).  Where some row may not, NaN goes into the products as 0,
 // and the first position of a NaN is noted for each dim: a row that sees it has

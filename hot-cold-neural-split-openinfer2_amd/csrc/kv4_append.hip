@@ -217,6 +217,7 @@ int check_paged4(const oi2_paged* c, int32_t layer) {
   if (int rc = check_paged(c, layer, false)) return rc;
   OI2_CHECK_ARG(layer >= 0 && layer < c->n_layers, "layer %d of a cache of %d", layer, c->n_layers);
   OI2_CHECK_ARG(c->pages && (uintptr_t)c->pages % 16 == 0, "pages must be non-null and 16-byte aligned");
+  OI2_CHECK_ARG(!c->scales, "a cache of 4 bits has its scales in its pages");
   return OI2_OK;
 }
 

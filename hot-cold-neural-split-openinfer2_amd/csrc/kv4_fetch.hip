@@ -116,16 +116,25 @@ __global__ __launch_bounds__(kThreads, 8) void k_kv4_fetch(FetchArgs a) {
   // codes are 1 KB of k's and 1 KB of v's.
   const int u = lane & 15, i = lane >> 4, p0 = 4 * wave + i;
   const int k_at = k4_at(p0, u), v_at = v4_at(p0, u), ks_at = k4_scale_at(p0, u / 4), vs_at = v4_scale_at(p0, u / 4);
-  const int64_t units = (int64_t)s_pages[n - 1] * a.n_kv;
-  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const int page = (int)(unit / a.n_kv), g = (int)(unit - (int64_t)page * a.n_kv);
-    int lo = 0, hi = n - 1;          // the first row whose pages end past this one
+  auto row_where = [&](auto holds) {         // the first row that holds it
+    int lo = 0, hi = n - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (s_pages[mid] > page) hi = mid;
+      if (holds(mid)) hi = mid;
       else lo = mid + 1;
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
+    return __builtin_amdgcn_readfirstlane(lo);
+  };
+  int pages = s_pages[n - 1];
+  if (s_tokens[n - 1] > total) {             // those up to the last token that fits
+    const int r = row_where([&](int x) { return s_tokens[x] >= total; });
+    const int left = total - (r ? s_tokens[r - 1] : 0), f = s_first[r];
+    pages = (r ? s_pages[r - 1] : 0) + (left ? (f + left - 1) / kPage - f / kPage + 1 : 0);
+  }
+  const int64_t units = (int64_t)pages * a.n_kv;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int page = (int)(unit / a.n_kv), g = (int)(unit - (int64_t)page * a.n_kv);
+    const int lo = row_where([&](int x) { return s_pages[x] > page; });
     const int t0 = lo ? s_tokens[lo - 1] : 0, t1 = min(s_tokens[lo], total);   // the row's tokens
     const int f = s_first[lo], j = f / kPage + page - (lo ? s_pages[lo - 1] : 0);
     int id = a.table[(int64_t)lo * a.width + j];
@@ -214,6 +223,8 @@ extern "C" int oi2_kv4_fetch(const oi2_paged* c, int32_t layer, const int32_t* f
     }
     OI2_CHECK_ARG(!meet(k, v, max_tokens, size), "k and v share memory");
   }
+  auto in_cu = [&](const int32_t* x) { return x && x < cu + c->n_seqs + 1 && cu < x + c->n_seqs; };
+  OI2_CHECK_ARG(!in_cu(first) && !in_cu(count) && !in_cu(c->lens), "cu shares memory with what is read");
   a.table = c->block_table;
   a.lens = c->lens;
   a.first = first;

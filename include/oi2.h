@@ -600,8 +600,8 @@ int oi2_attn_forward_paged(const uint16_t* x, int32_t n_tokens, const oi2_attn* 
  * changes when it grows.
  *
  * oi2_paged.pages: (layer, page, kv head) blocks of 9216 bytes, 16-byte aligned;
- * oi2_paged.scales is not used.  A block holds the codes of k, those of v at 4096,
- * k's scales (fp16) at 8192, v's at 8704, in the order in which the attention
+ * oi2_paged.scales is NULL.  A block holds the codes of k, those of v at 4096, k's
+ * scales (fp16) at 8192, v's at 8704, in the order in which the attention
  * loads them, a dword u for dims 8 u .. 8 u + 7:
  *   k, position p: 1024 (p / 4 % 4) + 256 (u / 4) + 16 (4 (p / 16) + p % 4) + 4 (u % 4)
  *   v, position p: 1024 (p / 4 % 4) + 256 (p / 16) + 16 u + 4 (p % 4)

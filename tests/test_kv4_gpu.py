@@ -239,6 +239,21 @@ def test_fetch(dev, n_kv, lens, first, count):
     assert torch.equal(c.fetch(0, count, n)[2].cpu(), torch.tensor(np.cumsum([0] + [min(max(a, 0), b) for a, b in zip(count, lens)])).int())
 
 
+@pytest.mark.parametrize("room", [0, 1, 36, 37, 38, 64, 100, 101, 137, 138, 400])
+def test_fetch_of_more_than_there_is_room_for(dev, room):
+    """Rooms that end in a row, at its end, on a page's edge and inside a page,
+    where rows start inside one."""
+    print(f"[fetch4] room {room}", flush=True)
+    c, o = _held(dev, 3, [101, 64, 0, 200], torch.float16)
+    first, count = [27, 0, 0, 63], [37, 64, 9, 2 ** 31 - 1]
+    k, v, cu = o.fetch(first, count)
+    gk, gv, gcu = c.fetch(0, count, room, first=first)
+    assert gcu.tolist() == cu
+    m = min(cu[-1], room)
+    for got, want in ((gk, k), (gv, v)):
+        assert torch.equal(got[:m].cpu(), torch.from_numpy(want[:m]).half()) and not got[m:].any()
+
+
 def test_fetch_is_what_read_gives(dev):
     c, o = _held(dev, 8, [130, 7, 0], torch.bfloat16)
     for row in (0, 1, 2, -2):

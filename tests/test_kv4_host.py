@@ -39,6 +39,11 @@ REFUSED = [
     ("fetch", dict(dtype=7), b"dtype"), ("fetch", dict(n=-1), b"tokens"), ("fetch", dict(count=None), b"null"), ("fetch", dict(cu_out=None), b"null"),
     ("fetch", dict(layer=-1), b"layer"), ("fetch", dict(pages=None), b"pages"), ("fetch", dict(k=_lib.Heads(None, 8, 1024, 128)), b"non-null"),
     ("fetch", dict(k=_lib.Heads(AT, 4, 1024, 128)), b"heads"), ("fetch", dict(v=_lib.Heads(AT + 1, 8, 1024, 128)), b"aligned"),
+    # a cache of 8 bits
+    ("append", dict(scales=64), b"scales"), ("attend", dict(scales=64), b"scales"), ("fetch", dict(scales=64), b"scales"),
+    # cu where the counts are, or where they end
+    ("fetch", dict(count=AT, cu_out=AT), b"shares memory"), ("fetch", dict(count=AT, cu_out=AT + 12), b"shares memory"),
+    ("fetch", dict(count=AT, cu_out=AT - 16), b"shares memory"), ("fetch", dict(lens=AT, cu_out=AT + 4), b"shares memory"),
     # an output's values in one place, or backwards
     ("fetch", dict(k=_lib.Heads(AT, 8, 0, 128)), b"share memory"), ("fetch", dict(k=_lib.Heads(AT, 8, 1024, 64)), b"share memory"),
     ("fetch", dict(k=_lib.Heads(AT, 8, 1023, 128)), b"share memory"), ("fetch", dict(v=_lib.Heads(AT, 8, -1024, 128)), b"share memory"),
