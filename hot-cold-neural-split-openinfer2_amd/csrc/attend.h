@@ -138,6 +138,36 @@ constexpr int kSc1 = 16;                   // cache-policy operand: agent-cohere
 __device__ __forceinline__ void st_agent(float* p, float v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// An item of a list, of `groups` workgroups, and the kv head.  False where the
+// launch leaves it out: the list has fewer, the call has not its tokens, or
+// (with fewer tokens than the plan's) not its last part, so that its arrivals
+// would not be complete.
+struct Found {
+  const AttendItem* full;
+  ItemHead it;
+  int g, n_tok;               // n_tok: the call's tokens of it
+};
+__device__ __forceinline__ bool few_find(const AttendArgs& a, int b, Found& f) {
+  const int item = b / a.n_kv;
+  f.g = b - item * a.n_kv;
+  f.full = a.few.items + item;
+  f.it = scalar_load(static_cast<const ItemHead*>(f.full));
+  if (item >= scalar_load(a.work + kNFew)) return false;
+  f.n_tok = min(f.it.n_tokens, a.n_tokens - f.it.token0);
+  return f.n_tok > 0 && item - f.it.part + f.it.n_parts <= a.few.groups / a.n_kv;
+}
+__device__ __forceinline__ bool many_find(const AttendArgs& a, int b, Found& f) {
+  // the last tiles, which see most, first
+  const int back = b / a.n_kv;
+  f.g = b - back * a.n_kv;
+  const int item = min(scalar_load(a.work + kNMany), a.many.groups / a.n_kv) - 1 - back;
+  if (item < 0) return false;
+  f.full = a.many.items + item;
+  f.it = scalar_load(static_cast<const ItemHead*>(f.full));
+  f.n_tok = min(f.it.n_tokens, a.n_tokens - f.it.token0);
+  return f.n_tok > 0 && item - f.it.part + f.it.n_parts <= a.many.groups / a.n_kv;
+}
+
 // A part's sums, row by row of n_rows, are stored (agent-coherent, by every
 // thread).  True in the workgroup that completes the set, which then joins it.
 __device__ __forceinline__ bool arrive(const PartArgs& pa, const ItemHead& it, int n_kv, int g) {
@@ -160,8 +190,10 @@ __device__ __forceinline__ bool arrive(const PartArgs& pa, const ItemHead& it, i
 // together, and are taken in with a running maximum.  smem: 16.1 bytes
 // a thread.
 template <bool BF16, int ROWS>
-__device__ __forceinline__ void join_parts(const AttendArgs& a, const PartArgs& pa, const ItemHead& it, int g, int n_rows,
-                                           float* smem) {
+__device__ __forceinline__ void join_parts(const AttendArgs& a, const PartArgs& pa, const Found& f, uint8_t* smem8) {
+  float* smem = reinterpret_cast<float*>(smem8);
+  const ItemHead& it = f.it;
+  const int g = f.g, n_rows = f.n_tok << a.group_log;
   constexpr int kGroups = kThreads / 32, RB = ROWS == kFewRows ? 1 : 4, U = ROWS == kFewRows ? 8 : 4;
   f32x4* s_y = reinterpret_cast<f32x4*>(smem);       // (kGroups, 32)
   float* s_M = smem + 4 * kThreads;
@@ -262,57 +294,56 @@ __device__ __forceinline__ void join_parts(const AttendArgs& a, const PartArgs& 
 
 // ── few rows ─────────────────────────────────────────────────────────────────
 
+// SETS sets of kFewRows rows.
 constexpr int kORow = kHeadD + 4;          // floats of an output row in LDS, padded
-constexpr int kFewLds = (kFewWaves * kFewRows * (kORow + 2) + kHeadD) * 4;
+template <int SETS>
+constexpr int kFewLds = (kFewWaves * SETS * kFewRows * (kORow + 2) + kHeadD) * 4;
 
 // Each wave's sums, maxima and exponential sums; the first NaN of each dim.
+template <int SETS>
 struct FewLds {
-  float (*o)[kFewRows][kORow];
-  float (*m)[kFewRows];
-  float (*l)[kFewRows];
+  static constexpr int kRows = SETS * kFewRows;
+  float (*o)[kRows][kORow];
+  float (*m)[kRows];
+  float (*l)[kRows];
   int* nan;
   __device__ __forceinline__ explicit FewLds(uint8_t* smem) {
-    typedef float Rows[kFewRows];
-    o = reinterpret_cast<float (*)[kFewRows][kORow]>(smem);
-    m = reinterpret_cast<Rows*>(smem + kFewWaves * kFewRows * kORow * 4);
+    typedef float Rows[kRows];
+    o = reinterpret_cast<float (*)[kRows][kORow]>(smem);
+    m = reinterpret_cast<Rows*>(smem + kFewWaves * kRows * kORow * 4);
     l = m + kFewWaves;
     nan = reinterpret_cast<int*>(l + kFewWaves);
   }
 };
 
 // A workgroup's tile, as lane (r = lane % 16, grp = lane / 16) of wave w has it.
+template <int SETS>
 struct FewTile {
   ItemHead it;
   const AttendItem* full;
   int g, w, lane, r, grp, n_rows;
-  int lim;                    // positions that query row r sees
+  int lim[SETS];              // positions that query row 16 set + r sees
   int all_see;                // ... and every row does
-  float sc;                   // of the scores of q
-  h8 q[4];                    // query row r: B operand of step i, dims dim_of(grp, i) ..
+  float sc[SETS];             // of the scores of q
+  h8 q[SETS][4];              // that row: B operand of step i, dims dim_of(grp, i) ..
 };
 
-// False where the launch leaves the tile out.
-template <bool BF16, class DimOf>
-__device__ __forceinline__ bool few_open(const AttendArgs& a, int b, const FewLds& lds, FewTile& t, DimOf dim_of) {
-  const int item = b / a.n_kv, g = b - item * a.n_kv;
-  const AttendItem& full = a.few.items[item];
-  const ItemHead it = scalar_load(static_cast<const ItemHead*>(&full));
-  if (item >= scalar_load(a.work + kNFew)) return false;
-  const int n_tok = min(it.n_tokens, a.n_tokens - it.token0);
-  // a tile whose last part is not in the launch (fewer tokens than the plan's)
-  // is left out whole: its arrivals would not be complete
-  if (n_tok <= 0 || item - it.part + it.n_parts > a.few.groups / a.n_kv) return false;
+template <bool BF16, int SETS, class DimOf>
+__device__ __forceinline__ void few_open(const AttendArgs& a, const Found& f, const FewLds<SETS>& lds, FewTile<SETS>& t, DimOf dim_of) {
+  const ItemHead& it = f.it;
+  const int g = f.g, n_tok = f.n_tok;
   const int tid = threadIdx.x, lane = lane_id(), r = lane & 15, grp = lane >> 4;
   t.w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lg = a.group_log, n_rows = n_tok << lg;
   if (tid < kHeadD) lds.nan[tid] = kNoNan;
   __syncthreads();
 
-  uint16_t qv[4][8];
-  const int tok = r >> lg;
-  {
+#pragma unroll
+  for (int set = 0; set < SETS; ++set) {
+    const int row = kFewRows * set + r, tok = row >> lg;
+    uint16_t qv[4][8];
     const uint16_t* pq = a.q + (int64_t)(it.token0 + min(tok, n_tok - 1)) * a.token_stride +
-                         (int64_t)((g << lg) + (r & ((1 << lg) - 1))) * a.head_stride;
+                         (int64_t)((g << lg) + (row & ((1 << lg) - 1))) * a.head_stride;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint16_t* p = pq + dim_of(grp, i);
@@ -323,42 +354,41 @@ __device__ __forceinline__ bool few_open(const AttendArgs& a, int b, const FewLd
         for (int e = 0; e < 8; ++e) qv[i][e] = p[e];
       }
     }
+    int qe = 0;
+    if (BF16) {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(bf16_bits_to_float(qv[i][e])));
+      top = quad_max(top);
+      qe = min(max((int)(as_u32(top) >> 23) - 127 - kTopExp, -126), 126);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.q[set][i] = q_frag<BF16>(qv[i], qe, a.scale < 0.0f);
+    t.sc[set] = BF16 ? ldexp2(a.scale, qe) : a.scale;
+    t.lim[set] = row < n_rows ? min(it.pos0 + tok + 1, it.kv_len) : 0;
   }
-  int qe = 0;
-  if (BF16) {
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(bf16_bits_to_float(qv[i][e])));
-    top = quad_max(top);
-    qe = min(max((int)(as_u32(top) >> 23) - 127 - kTopExp, -126), 126);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) t.q[i] = q_frag<BF16>(qv[i], qe, a.scale < 0.0f);
-  t.sc = BF16 ? ldexp2(a.scale, qe) : a.scale;
-  t.lim = r < n_rows ? min(it.pos0 + tok + 1, it.kv_len) : 0;
   t.all_see = min(it.pos0 + 1, it.kv_len);
   t.it = it;
-  t.full = &full;
+  t.full = f.full;
   t.g = g;
   t.lane = lane;
   t.r = r;
   t.grp = grp;
   t.n_rows = n_rows;
-  return true;
 }
 
 // The four waves' sums, which are in LDS, are joined, and leave as the tile's
-// output or as a part's sums.
-template <bool BF16>
-__device__ __forceinline__ void few_close(const AttendArgs& a, const FewTile& t, const FewLds& lds, uint8_t* smem) {
+// output or as a part's sums; true where the parts are then to be joined.
+template <bool BF16, int SETS>
+__device__ __forceinline__ bool few_close(const AttendArgs& a, const FewTile<SETS>& t, const FewLds<SETS>& lds) {
   const ItemHead& it = t.it;
   const int tid = threadIdx.x, g = t.g, n_rows = t.n_rows, lg = a.group_log;
   const float ninf = -__builtin_inff();
   __syncthreads();
   // thread: E dims from d0 of a query row
-  constexpr int E = kFewRows * kHeadD / kThreads;
+  constexpr int E = SETS * kFewRows * kHeadD / kThreads;
   const int row = tid * E / kHeadD, d0 = tid * E % kHeadD;
   float M = ninf, L = 0.0f, y[E];
 #pragma unroll
@@ -378,21 +408,23 @@ __device__ __forceinline__ void few_close(const AttendArgs& a, const FewTile& t,
 #pragma unroll
   for (int e = 0; e < E; ++e) y[e] = lds.nan[d0 + e] < sees ? __builtin_nanf("") : y[e];
   if (it.n_parts > 1) {
-    const int64_t base = ((int64_t)(it.slot0 + it.part) * a.n_kv + g) * kFewRows;
+    // one set's are in the list of few rows, more in that of many
+    constexpr int kRows = SETS == 1 ? kFewRows : kManyRows;
+    const PartArgs& pa = SETS == 1 ? a.few : a.many;
+    const int64_t base = ((int64_t)(it.slot0 + it.part) * a.n_kv + g) * kRows;
     if (row < n_rows) {
-      const rsrc_t ro = rsrc(a.few.o + base * kHeadD, kFewRows * kHeadD * 4);
+      const rsrc_t ro = rsrc(pa.o + base * kHeadD, kRows * kHeadD * 4);
 #pragma unroll
       for (int e = 0; e < E; e += 2)
         __builtin_amdgcn_raw_buffer_store_b64(u32x2v{as_u32(y[e]), as_u32(y[e + 1])}, ro, (row * kHeadD + d0 + e) * 4, 0, kSc1);
       if (d0 == 0) {
-        st_agent(a.few.ml + 2 * (base + row), M);
-        st_agent(a.few.ml + 2 * (base + row) + 1, L);
+        st_agent(pa.ml + 2 * (base + row), M);
+        st_agent(pa.ml + 2 * (base + row) + 1, L);
       }
     }
-    if (arrive(a.few, it, a.n_kv, g)) join_parts<BF16, kFewRows>(a, a.few, it, g, n_rows, reinterpret_cast<float*>(smem));
-    return;
+    return arrive(pa, it, a.n_kv, g);
   }
-  if (row >= n_rows) return;
+  if (row >= n_rows) return false;
   const float inv = it.kv_len > 0 ? 1.0f / L : 0.0f;     // a rejected row: zeros
   uint16_t z[E];
 #pragma unroll
@@ -400,6 +432,7 @@ __device__ __forceinline__ void few_close(const AttendArgs& a, const FewTile& t,
   uint16_t* to = a.out + ((int64_t)(it.token0 + tk) * a.n_q + head) * kHeadD + d0;
 #pragma unroll
   for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(to + e) = z[e] | (uint32_t)z[e + 1] << 16;
+  return false;
 }
 
 // ── many rows ────────────────────────────────────────────────────────────────
@@ -444,16 +477,10 @@ __device__ __forceinline__ int v_lds(int row, int c) { return kVLds + row * 128 
 constexpr int kManyLds = 4 * kHalfLds + kHeadD * 4;
 
 template <bool BF16, class Pages>
-__device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t* s_page) {
+__device__ __forceinline__ bool attend_many(const AttendArgs& a, const Found& f, uint8_t* s_page) {
   int* s_nan = reinterpret_cast<int*>(s_page + 4 * kHalfLds);
-  // the last tiles, which see most, first
-  const int back = b / a.n_kv, g = b - back * a.n_kv;
-  const int item = min(scalar_load(a.work + kNMany), a.many.groups / a.n_kv) - 1 - back;
-  if (item < 0) return;
-  const AttendItem& full = a.many.items[item];
-  const ItemHead it = scalar_load(static_cast<const ItemHead*>(&full));
-  const int n_tok = min(it.n_tokens, a.n_tokens - it.token0);
-  if (n_tok <= 0 || item - it.part + it.n_parts > a.many.groups / a.n_kv) return;
+  const ItemHead& it = f.it;
+  const int g = f.g, n_tok = f.n_tok;
   const int tid = threadIdx.x, lane = lane_id(), r = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lg = a.group_log, n_rows = n_tok << lg;
@@ -594,8 +621,8 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
   };
 
   if (it.page0 < it.page1) {
-    const int64_t b0 = (int64_t)scalar_load(full.ids) * a.n_kv + g;
-    const int64_t b1 = (int64_t)scalar_load(full.ids + 1) * a.n_kv + g;
+    const int64_t b0 = (int64_t)scalar_load(f.full->ids) * a.n_kv + g;
+    const int64_t b1 = (int64_t)scalar_load(f.full->ids + 1) * a.n_kv + g;
     int64_t b2 = block_of(it.page0 + 2);
     pages.load(b0);
     float2 sc0 = pages.scale_of(b0), sc1 = pages.scale_of(b1);
@@ -640,10 +667,9 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
       st_agent(a.many.ml + 2 * (base + row), m);
       st_agent(a.many.ml + 2 * (base + row) + 1, l);
     }
-    if (arrive(a.many, it, a.n_kv, g)) join_parts<BF16, kManyRows>(a, a.many, it, g, n_rows, reinterpret_cast<float*>(s_page));
-    return;
+    return arrive(a.many, it, a.n_kv, g);
   }
-  if (row >= n_rows) return;
+  if (row >= n_rows) return false;
   const float inv = it.kv_len > 0 ? 1.0f / l : 0.0f;   // a rejected row: zeros
   uint16_t* po = a.out + ((int64_t)(it.token0 + tok) * a.n_q + (g << lg) + (row & ((1 << lg) - 1))) * kHeadD;
   Pages::each_four(o, h, [&](int chunk, f32x4 x) {
@@ -652,6 +678,7 @@ __device__ __forceinline__ void attend_many(const AttendArgs& a, int b, uint8_t*
     for (int e = 0; e < 4; ++e) z[e] = narrow<BF16>(x[e] * inv);
     *reinterpret_cast<u32x2v*>(po + 4 * chunk) = *reinterpret_cast<u32x2v*>(z);
   });
+  return false;
 }
 
 // Zeros for the rows past the step's last token.

@@ -56,20 +56,25 @@ __device__ __forceinline__ void fix_scales(uint32_t (&s)[N], int pos, int kv_len
 // A wave takes every fourth page, loads the next one (9 KB) while it works on
 // this one, and its page number by a scalar load two ahead; the four meet in
 // LDS at the end.
-template <bool BF16>
-__device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* smem) {
-  const FewLds lds(smem);
-  FewTile t;
-  if (!few_open<BF16>(a, b, lds, t, [](int grp, int i) { return 32 * grp + 8 * i; })) return;
+template <bool BF16, int SETS>
+__device__ __forceinline__ bool attend_few(const AttendArgs& a, const Found& found, uint8_t* smem) {
+  const FewLds<SETS> lds(smem);
+  FewTile<SETS> t;
+  few_open<BF16>(a, found, lds, t, [](int grp, int i) { return 32 * grp + 8 * i; });
   const ItemHead& it = t.it;
-  const int g = t.g, w = t.w, lane = t.lane, r = t.r, grp = t.grp, lim = t.lim, all_see = t.all_see;
+  const int g = t.g, w = t.w, lane = t.lane, r = t.r, grp = t.grp, all_see = t.all_see;
 
   const float ninf = -__builtin_inff();
-  f32x4 o[8];
+  f32x4 o[SETS][8];
+  float m[SETS], l[SETS], ksc[SETS];
 #pragma unroll
-  for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = ninf, l = 0.0f;
-  const float ksc = score_scale(t.sc, 1.0f);
+  for (int z = 0; z < SETS; ++z) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[z][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[z] = ninf;
+    l[z] = 0.0f;
+    ksc[z] = score_scale(t.sc[z], 1.0f);
+  }
 
   const int32_t* table = a.table + (int64_t)it.row * a.width;
   auto block_of = [&](int page) {
@@ -116,15 +121,21 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
     const rsrc_t rn = page_rsrc(next, page + kFewWaves);
     next = block_of(page + 2 * kFewWaves);
 
-    float s[16];
+    float s[SETS][16];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      f32x4 acc[SETS] = {};
       const f16x2 sk = twice(k < 2 ? ks.x : ks.y, k & 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc = mfma16(k_values(kr[k][i], sk), t.q[i], acc);
+      for (int i = 0; i < 4; ++i) {
+        const h8 kv = k_values(kr[k][i], sk);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * k + i] = acc[i];
+        for (int z = 0; z < SETS; ++z) acc[z] = mfma16(kv, t.q[z][i], acc[z]);
+      }
+#pragma unroll
+      for (int z = 0; z < SETS; ++z)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[z][4 * k + i] = acc[z][i];
     }
     __builtin_amdgcn_sched_barrier(0);
     load_k(rn);
@@ -132,36 +143,41 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
     const bool whole = page * kPage + kPage <= all_see;
     if (!whole) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = p0 + j < lim ? s[j] : ninf;
+      for (int z = 0; z < SETS; ++z)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[z][j] = p0 + j < t.lim[z] ? s[z][j] : ninf;
       fix_scales(vs, p0, it.kv_len, 8 * r, lds.nan);
     }
-    float cm = s[0];
+    Probs p[SETS][2];
 #pragma unroll
-    for (int j = 1; j < 16; ++j) cm = fmaxf(cm, s[j]);
-    cm = quad_max(cm) * ksc;
-    const bool up = cm > m + kSlack;
-    if (__any(up)) {
-      const float mn = up ? cm : m;
-      const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-      l *= alpha;
+    for (int z = 0; z < SETS; ++z) {
+      float cm = s[z][0];
 #pragma unroll
-      for (int d = 0; d < 8; ++d) o[d] *= alpha;
-      m = mn;
-    }
-    const float rel = kLift - (m == ninf ? 0.0f : m);
-    float sum[2] = {0.0f, 0.0f};
-    Probs p[2];
+      for (int j = 1; j < 16; ++j) cm = fmaxf(cm, s[z][j]);
+      cm = quad_max(cm) * ksc[z];
+      const bool up = cm > m[z] + kSlack;
+      if (__any(up)) {
+        const float mn = up ? cm : m[z];
+        const float alpha = m[z] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[z] - mn);
+        l[z] *= alpha;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        e[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + j], ksc, rel));
-        sum[h] += e[j];
+        for (int d = 0; d < 8; ++d) o[z][d] *= alpha;
+        m[z] = mn;
       }
-      p[h] = to_probs(e);
+      const float rel = kLift - (m[z] == ninf ? 0.0f : m[z]);
+      float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          e[j] = __builtin_amdgcn_exp2f(fmaf(s[z][8 * h + j], ksc[z], rel));
+          sum[h] += e[j];
+        }
+        p[z][h] = to_probs(e);
+      }
+      l[z] += sum[0] + sum[1];
     }
-    l += sum[0] + sum[1];
     // positions 16 grp + 8 h + 2 k, + 1 are dwords 2 (k % 2), + 1 of vector 2 h + k / 2
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -178,27 +194,44 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
         }
         const h8 f0 = {v0[0][0], v0[0][1], v0[1][0], v0[1][1], v0[2][0], v0[2][1], v0[3][0], v0[3][1]};
         const h8 f1 = {v1[0][0], v1[0][1], v1[1][0], v1[1][1], v1[2][0], v1[2][1], v1[3][0], v1[3][1]};
-        o[2 * q] = mfma16(f0, p[h].hi, o[2 * q]);
-        o[2 * q] = mfma16(f0, p[h].lo, o[2 * q]);
-        o[2 * q + 1] = mfma16(f1, p[h].hi, o[2 * q + 1]);
-        o[2 * q + 1] = mfma16(f1, p[h].lo, o[2 * q + 1]);
+#pragma unroll
+        for (int z = 0; z < SETS; ++z) {
+          o[z][2 * q] = mfma16(f0, p[z][h].hi, o[z][2 * q]);
+          o[z][2 * q] = mfma16(f0, p[z][h].lo, o[z][2 * q]);
+          o[z][2 * q + 1] = mfma16(f1, p[z][h].hi, o[z][2 * q + 1]);
+          o[z][2 * q + 1] = mfma16(f1, p[z][h].lo, o[z][2 * q + 1]);
+        }
       }
     __builtin_amdgcn_sched_barrier(0);
     load_v(rn);
   }
 
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)              // dims 8 (4 grp + i) ..
+  for (int z = 0; z < SETS; ++z) {
+    const int row = kFewRows * z + r;
+    l[z] += __shfl_xor(l[z], 16);
+    l[z] += __shfl_xor(l[z], 32);
 #pragma unroll
-    for (int d = 0; d < 8; d += 4)
-      *reinterpret_cast<f32x4*>(&lds.o[w][r][8 * (4 * grp + i) + d]) = f32x4{o[d][i], o[d + 1][i], o[d + 2][i], o[d + 3][i]};
-  if (grp == 0) {
-    lds.m[w][r] = m;
-    lds.l[w][r] = l;
+    for (int i = 0; i < 4; ++i)            // dims 8 (4 grp + i) ..
+#pragma unroll
+      for (int d = 0; d < 8; d += 4)
+        *reinterpret_cast<f32x4*>(&lds.o[w][row][8 * (4 * grp + i) + d]) =
+            f32x4{o[z][d][i], o[z][d + 1][i], o[z][d + 2][i], o[z][d + 3][i]};
+    if (grp == 0) {
+      lds.m[w][row] = m[z];
+      lds.l[w][row] = l[z];
+    }
   }
-  few_close<BF16>(a, t, lds, smem);
+  return few_close<BF16>(a, t, lds);
+}
+
+// Zeros for the tokens of a rejected row.
+__device__ __forceinline__ void zero_tile(const AttendArgs& a, const Found& f) {
+  const int lg = a.group_log;
+  for (int i = threadIdx.x; i < f.n_tok << lg << 4; i += kThreads) {   // 16 vectors of 8 dims a row
+    const int row = i >> 4, head = (f.g << lg) + (row & ((1 << lg) - 1));
+    *reinterpret_cast<u32x4*>(a.out + ((int64_t)(f.it.token0 + (row >> lg)) * a.n_q + head) * kHeadD + 8 * (i & 15)) = u32x4{0, 0, 0, 0};
+  }
 }
 
 // ── many rows ────────────────────────────────────────────────────────────────
@@ -271,20 +304,45 @@ struct Pages4 {
 
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void k_kv4_attend_few(AttendArgs a) {
-  __shared__ __align__(16) uint8_t smem[kFewLds];
+  __shared__ __align__(16) uint8_t smem[kFewLds<1>];
   const int b = blockIdx.x;
-  if (b < a.few.groups) attend_few<BF16>(a, b, smem);
-  else zero_rest(a, b - a.few.groups);
+  Found f;
+  if (b >= a.few.groups) zero_rest(a, b - a.few.groups);
+  else if (few_find(a, b, f) && attend_few<BF16, 1>(a, f, smem)) join_parts<BF16, kFewRows>(a, a.few, f, smem);
+}
+
+// Steps whose rows all have kSetsRows query rows at most: drafts.
+constexpr int kSets = 2, kSetsRows = kSets * kFewRows;
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void k_kv4_attend_sets(AttendArgs a) {
+  __shared__ __align__(16) uint8_t smem[kFewLds<kSets>];
+  const int b = blockIdx.x;
+  Found f;
+  if (b < a.many.groups) {
+    if (!many_find(a, b, f)) return;
+    if (f.it.n_tokens << a.group_log > kSetsRows) zero_tile(a, f);     // only a rejected row has more
+    else if (attend_few<BF16, kSets>(a, f, smem)) join_parts<BF16, kManyRows>(a, a.many, f, smem);
+  } else if (b - a.many.groups >= a.few.groups) {
+    zero_rest(a, b - a.many.groups - a.few.groups);
+  } else if (few_find(a, b - a.many.groups, f) && attend_few<BF16, 1>(a, f, smem)) {
+    join_parts<BF16, kFewRows>(a, a.few, f, smem);
+  }
 }
 
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void k_kv4_attend(AttendArgs a) {
-  static_assert(kManyLds >= kFewLds && kThreads == 64 * kFewWaves, "one workgroup for either");
+  static_assert(kManyLds >= kFewLds<1> && kThreads == 64 * kFewWaves, "one workgroup for either");
   __shared__ __align__(1024) uint8_t smem[kManyLds];
   const int b = blockIdx.x;
-  if (b < a.many.groups) attend_many<BF16, Pages4>(a, b, smem);
-  else if (b - a.many.groups < a.few.groups) attend_few<BF16>(a, b - a.many.groups, smem);
-  else zero_rest(a, b - a.many.groups - a.few.groups);
+  Found f;
+  if (b < a.many.groups) {
+    if (many_find(a, b, f) && attend_many<BF16, Pages4>(a, f, smem)) join_parts<BF16, kManyRows>(a, a.many, f, smem);
+  } else if (b - a.many.groups >= a.few.groups) {
+    zero_rest(a, b - a.many.groups - a.few.groups);
+  } else if (few_find(a, b - a.many.groups, f) && attend_few<BF16, 1>(a, f, smem)) {
+    join_parts<BF16, kFewRows>(a, a.few, f, smem);
+  }
 }
 
 }  // namespace
@@ -304,7 +362,10 @@ extern "C" int oi2_kv4_attend(const oi2_paged* c, const oi2_page_plan* p, int32_
   AttendArgs& a = call.a;
   a.pages = c->pages + (size_t)layer * c->n_pages * c->n_kv * k4Block;
   const dim3 grid(call.groups), block(kThreads);
-  if (a.many.groups && call.bf16) hipLaunchKernelGGL(k_kv4_attend<true>, grid, block, 0, st, a);
+  const bool sets = a.many.groups && (int64_t)p->max_new << a.group_log <= kSetsRows;
+  if (sets && call.bf16) hipLaunchKernelGGL(k_kv4_attend_sets<true>, grid, block, 0, st, a);
+  else if (sets) hipLaunchKernelGGL(k_kv4_attend_sets<false>, grid, block, 0, st, a);
+  else if (a.many.groups && call.bf16) hipLaunchKernelGGL(k_kv4_attend<true>, grid, block, 0, st, a);
   else if (a.many.groups) hipLaunchKernelGGL(k_kv4_attend<false>, grid, block, 0, st, a);
   else if (call.bf16) hipLaunchKernelGGL(k_kv4_attend_few<true>, grid, block, 0, st, a);
   else hipLaunchKernelGGL(k_kv4_attend_few<false>, grid, block, 0, st, a);

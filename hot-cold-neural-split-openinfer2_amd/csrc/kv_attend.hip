@@ -66,14 +66,14 @@ __device__ __forceinline__ void take_nans(u32x4& x, int pos, int* first) {   // 
 // of 700 positions 8.1, three rounds and the merge.  Tried without gain: 8 and
 // 16 waves, pages dealt out in equal shares whatever row they belong to.
 template <bool BF16>
-__device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* smem) {
-  const FewLds lds(smem);
-  FewTile t;
-  if (!few_open<BF16>(a, b, lds, t, [](int grp, int i) { return 16 * (4 * (i >> 1) + grp) + 8 * (i & 1); })) return;
+__device__ __forceinline__ bool attend_few(const AttendArgs& a, const Found& found, uint8_t* smem) {
+  const FewLds<1> lds(smem);
+  FewTile<1> t;
+  few_open<BF16>(a, found, lds, t, [](int grp, int i) { return 16 * (4 * (i >> 1) + grp) + 8 * (i & 1); });
   const ItemHead& it = t.it;
-  const int g = t.g, w = t.w, lane = t.lane, r = t.r, grp = t.grp, lim = t.lim, all_see = t.all_see;
-  const h8 (&qf)[4] = t.q;
-  const float sc = t.sc;
+  const int g = t.g, w = t.w, lane = t.lane, r = t.r, grp = t.grp, lim = t.lim[0], all_see = t.all_see;
+  const h8 (&qf)[4] = t.q[0];
+  const float sc = t.sc[0];
 
   const float ninf = -__builtin_inff();
   f32x4 o[8];
@@ -194,7 +194,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs& a, int b, uint8_t* 
     lds.m[w][r] = m;
     lds.l[w][r] = l;
   }
-  few_close<BF16>(a, t, lds, smem);
+  return few_close<BF16>(a, t, lds);
 }
 
 // ── many rows ────────────────────────────────────────────────────────────────
@@ -275,20 +275,26 @@ struct Pages8 {
 // the long tiles first, the others fill the chip behind and beside them.
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void k_attend_few(AttendArgs a) {
-  __shared__ __align__(16) uint8_t smem[kFewLds];
+  __shared__ __align__(16) uint8_t smem[kFewLds<1>];
   const int b = blockIdx.x;
-  if (b < a.few.groups) attend_few<BF16>(a, b, smem);
-  else zero_rest(a, b - a.few.groups);
+  Found f;
+  if (b >= a.few.groups) zero_rest(a, b - a.few.groups);
+  else if (few_find(a, b, f) && attend_few<BF16>(a, f, smem)) join_parts<BF16, kFewRows>(a, a.few, f, smem);
 }
 
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendArgs a) {
-  static_assert(kManyLds >= kFewLds && kThreads == 64 * kFewWaves, "one workgroup for either");
+  static_assert(kManyLds >= kFewLds<1> && kThreads == 64 * kFewWaves, "one workgroup for either");
   __shared__ __align__(1024) uint8_t smem[kManyLds];
   const int b = blockIdx.x;
-  if (b < a.many.groups) attend_many<BF16, Pages8>(a, b, smem);
-  else if (b - a.many.groups < a.few.groups) attend_few<BF16>(a, b - a.many.groups, smem);
-  else zero_rest(a, b - a.many.groups - a.few.groups);
+  Found f;
+  if (b < a.many.groups) {
+    if (many_find(a, b, f) && attend_many<BF16, Pages8>(a, f, smem)) join_parts<BF16, kManyRows>(a, a.many, f, smem);
+  } else if (b - a.many.groups >= a.few.groups) {
+    zero_rest(a, b - a.many.groups - a.few.groups);
+  } else if (few_find(a, b - a.many.groups, f) && attend_few<BF16>(a, f, smem)) {
+    join_parts<BF16, kFewRows>(a, a.few, f, smem);
+  }
 }
 
 }  // namespace

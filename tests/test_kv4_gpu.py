@@ -363,7 +363,7 @@ def test_attend_head_layouts(dev, n_q, n_kv):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("new", [[1, 1, 1], [2, 40, 300]])
+@pytest.mark.parametrize("new", [[1, 1, 1], [2, 40, 300], [8, 5, 7]])
 def test_attend_values_of_many_sizes(dev, dtype, new):
     """Groups whose k and v differ by many powers of two, all-zero ones among
     them, and other scales of the scores: 0, negative, large."""
@@ -389,7 +389,7 @@ def test_attend_values_of_many_sizes(dev, dtype, new):
         _check_attend(c.attend(0, q, plan, scale=scale), want, bound, dtype)
 
 
-@pytest.mark.parametrize("new", [[1, 1], [3, 2], [90, 150]])
+@pytest.mark.parametrize("new", [[1, 1], [3, 2], [90, 150], [7, 8]])
 def test_attend_nan_where_it_is_seen(dev, new):
     """A group of v that is not finite reaches the rows that see its position, in
     its dims alone; one of k the rows that see it, in every dim; none what lies
@@ -426,7 +426,8 @@ def test_attend_nan_where_it_is_seen(dev, new):
 
 
 @pytest.mark.parametrize("n_kv,past,new", [(8, [20000], [1]), (8, [9000, 300, 5000], [1, 1, 1]), (8, [6000], [300]),
-                                           (4, [7000, 20, 4000], [2, 250, 1])])
+                                           (4, [7000, 20, 4000], [2, 250, 1]), (8, [9000, 300, 5000], [8, 5, 7]),
+                                           (4, [6000, 900], [4, 3])])
 def test_attend_rows_cut_into_parts(dev, n_kv, past, new):
     print(f"[attend4 parts] kv {n_kv} {past} + {new}", flush=True)
     c, o, plan, ref, q = _filled(dev, 32, n_kv, past, new, torch.float16, 11)
@@ -435,6 +436,24 @@ def test_attend_rows_cut_into_parts(dev, n_kv, past, new):
     _check_attend(y, want, bound, torch.float16)
     for _ in range(3):
         assert torch.equal(c.attend(0, q, plan), y)
+
+
+@pytest.mark.parametrize("n_q,n_kv,new", [(32, 8, [8, 5, 6, 7]), (32, 8, [9, 8, 33, 40]), (32, 4, [3, 4, 5, 2]), (8, 8, [17, 31, 32, 33]),
+                                          (4, 2, [16, 9, 17, 8])])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attend_tiles_around_17_to_32_rows(dev, dtype, n_q, n_kv, new):
+    """Drafts, and ends of chunks: more rows than one set, up to two of them, one
+    beyond; cut into parts and not; calls with fewer tokens than the plan's."""
+    for past in ([0, 63, 64, 200], [1500, 10, 2000, 1100]):
+        print(f"[attend4 sets] {dtype} q {n_q} kv {n_kv} {past} + {new}", flush=True)
+        c, o, plan, ref, q = _filled(dev, n_q, n_kv, past, new, dtype, 17)
+        want, bound = o.attend(_np(q), ref, D ** -0.5)
+        y = c.attend(0, q, plan)
+        _check_attend(y, want, bound, dtype)
+        assert torch.equal(c.attend(0, q, plan), y)
+        for n in (1, new[0] - 1, new[0], new[0] + 1, sum(new) - 1):
+            got = c.attend(0, q[:n], plan)
+            _check_attend(got, want[:n], bound[:n], dtype)
 
 
 def test_attend_every_position_counts_once(dev):
@@ -497,6 +516,28 @@ def test_attend_rejected_rows_and_padding(dev):
     c2.append(0, k[:2], v[:2], p3)
     z = c2.attend(0, q, p3)
     assert z[0].any() and not z[1:].any()
+
+
+@pytest.mark.parametrize("max_new", [4, 8, 40])
+def test_attend_rejected_rows_with_many_tokens(dev, max_new):
+    """Rows with more tokens than the plan's rows may have keep them in the packed
+    order, and get zeros there whichever tiles they are in."""
+    print(f"[attend4 rejected] {max_new}", flush=True)
+    new = [max_new, 200, 3, max_new + 1, 1]
+    c = oi2.PagedKVCache(1, 32, 8, 5, 400, 30, device=dev, bits=4)
+    plan = c.extend(new, c.new_plan(sum(new) + 5, max_new=max_new))
+    assert plan.rejected.tolist() == [0, 1, 0, 1, 0]
+    n = sum(new)
+    k, v = (torch.randn((n, 8, D), device=dev).half() for _ in range(2))
+    c.append(0, k, v, plan)
+    q = torch.randn((n + 5, 32, D), device=dev).half()
+    y = torch.full_like(q, 9.0)
+    c.attend(0, q, plan, out=y)
+    at = np.cumsum([0] + new)
+    for i, rejected in enumerate([0, 1, 0, 1, 0]):
+        x = y[at[i]:at[i + 1]]
+        assert not x.any() if rejected else bool((x != 9).any(2).all()) and bool(x.any(2).all())
+    assert bool((y[n:] == 9).all())
 
 
 # ── together ─────────────────────────────────────────────────────────────────
