@@ -56,6 +56,22 @@ __device__ __forceinline__ void fix_scales(uint32_t (&s)[N], int pos, int kv_len
 // A wave takes every fourth page, loads the next one (9 KB) while it works on
 // this one, and its page number by a scalar load two ahead; the four meet in
 // LDS at the end.
+//
+// Bound by loads and instructions alike: 48 tokens over 500 to 20000 positions
+// 57.7 us (258 MB, 4.5 TB/s); their loads alone 50, the products alone 52; two
+// over 60 and 150 thousand 37.3 (34 and 34), 20 rows of 4 tokens 19.7 (18 and 18).
+// Besides: 4 us to the first scores, parts of unequal length, 4 for arrivals and
+// joins.  158 registers, three workgroups a CU: with two 48 tokens take 65, with
+// four (128 registers) 92.  Measured slower: pages two ahead (66.5), parts half as
+// long (64), equal shares of all pages (61.5, and 54 instead of 20 for the drafts),
+// a second launch that joins (the two long ones 41.4), the query loaded behind
+// the first page (59.2).
+//
+// SETS: of 16 query rows.  Two where all rows have 17 to 32: a page is decoded
+// once for both, and 244 registers leave two workgroups a CU.  Drafts of 8 tokens
+// over 300 to 14000 positions 44 us instead of 91 the way of many rows, of 5 over
+// 200 to 4000 34 instead of 68.  33 to 64 rows stay there: 56 of them took 72.8
+// with four sets (414 registers) and 63.2 with two workgroups a tile, and there 65.
 template <bool BF16, int SETS>
 __device__ __forceinline__ bool attend_few(const AttendArgs& a, const Found& found, uint8_t* smem) {
   const FewLds<SETS> lds(smem);
@@ -239,6 +255,14 @@ __device__ __forceinline__ void zero_tile(const AttendArgs& a, const Found& f) {
 // Thread (n = tid / 64, lane): the 16 bytes of k of one position and group, and
 // those of v of positions 16 grp + 4 n .. + 3, dims 8 r ...  Row 16 e + r of V^T
 // in LDS is dim 8 r + e, so that a wave's stores are to 16 rows side by side.
+//
+// A prompt of 4100 tokens 206 us (667 TFLOP/s of the formula's operations, half as
+// much again with the low parts'), 10 chunks of 1 to 800 tokens over 400 to 9000
+// positions 104 (472).  The CUs are busy 83 and 70 % of the time (the rest is
+// start, unequal parts, joins), in it the matrix cores 56 and 45 %, vector
+// instructions 62 %, LDS 33 %; two waves a SIMD overlap them by chance.  A page's
+// staging is 97 of its 340 vector instructions; low parts to nearest, which are 16
+// fewer, took 1 % off the prompt alone.
 struct Pages4 {
   const AttendArgs& a;
   const ItemHead& it;
@@ -311,7 +335,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_kv4_attend_few(AttendArgs a) {
   else if (few_find(a, b, f) && attend_few<BF16, 1>(a, f, smem)) join_parts<BF16, kFewRows>(a, a.few, f, smem);
 }
 
-// Steps whose rows all have kSetsRows query rows at most: drafts.
+// Steps whose rows all have kSetsRows query rows at most (max_new says so), and
+// some more than one set.  A kernel of its own: beside attend_many and chosen by
+// the tile it made every step with chunks 2 us longer, by its 20 KB of code and
+// the registers that its arguments hold.
 constexpr int kSets = 2, kSetsRows = kSets * kFewRows;
 
 template <bool BF16>

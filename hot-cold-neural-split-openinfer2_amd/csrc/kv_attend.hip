@@ -199,13 +199,12 @@ __device__ __forceinline__ bool attend_few(const AttendArgs& a, const Found& fou
 
 // ── many rows ────────────────────────────────────────────────────────────────
 
-// The next page's staging stands between the products of the scores, and a
-// fragment's exponentials between the products of the fragment before.  What
-// bounds it: the products, a third of them for the probabilities' low parts;
-// the matrix cores are busy 60 % of the time, and two waves a SIMD fill the rest
-// by chance.  A call of 5000 tokens 288 to 306 us, boxes differ, in fp16 and 285 to
-// 302 in bf16 (670 to 720 TFLOP/s of the formula's operations, a third more with
-// the low parts'), 6 chunks beside 3 short rows 98 to 102.  With one fp16 part of a
+// What bounds many rows: the products, a third of them for the probabilities' low
+// parts; the matrix cores are busy 60 % of the time, and two waves a SIMD fill the
+// rest by chance.  A call of 5000 tokens 287 us in fp16 (714 TFLOP/s of the
+// formula's operations, half as much again with the low parts'), 6 chunks beside 3
+// short rows 97, where a low part by a subtraction and a conversion took 291 and
+// 98 (boxes differ: 288 to 306, in bf16 285 to 302).  With one fp16 part of a
 // probability, of 249 us before k's conflicts went, the exponentials alone made
 // 38, staging 35, the fragments' reads 55, the products 68, and there was tried
 // without gain: fragments read three steps ahead; raised priority around

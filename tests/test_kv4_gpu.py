@@ -363,7 +363,7 @@ def test_attend_head_layouts(dev, n_q, n_kv):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("new", [[1, 1, 1], [2, 40, 300], [8, 5, 7]])
+@pytest.mark.parametrize("new", [[1, 1, 1], [2, 40, 300], [8, 5, 7], [16, 9, 7]])
 def test_attend_values_of_many_sizes(dev, dtype, new):
     """Groups whose k and v differ by many powers of two, all-zero ones among
     them, and other scales of the scores: 0, negative, large."""
@@ -389,7 +389,7 @@ def test_attend_values_of_many_sizes(dev, dtype, new):
         _check_attend(c.attend(0, q, plan, scale=scale), want, bound, dtype)
 
 
-@pytest.mark.parametrize("new", [[1, 1], [3, 2], [90, 150], [7, 8]])
+@pytest.mark.parametrize("new", [[1, 1], [3, 2], [90, 150], [7, 8], [16, 11]])
 def test_attend_nan_where_it_is_seen(dev, new):
     """A group of v that is not finite reaches the rows that see its position, in
     its dims alone; one of k the rows that see it, in every dim; none what lies
@@ -427,7 +427,7 @@ def test_attend_nan_where_it_is_seen(dev, new):
 
 @pytest.mark.parametrize("n_kv,past,new", [(8, [20000], [1]), (8, [9000, 300, 5000], [1, 1, 1]), (8, [6000], [300]),
                                            (4, [7000, 20, 4000], [2, 250, 1]), (8, [9000, 300, 5000], [8, 5, 7]),
-                                           (4, [6000, 900], [4, 3])])
+                                           (4, [6000, 900], [4, 3]), (4, [6000, 900], [7, 8])])
 def test_attend_rows_cut_into_parts(dev, n_kv, past, new):
     print(f"[attend4 parts] kv {n_kv} {past} + {new}", flush=True)
     c, o, plan, ref, q = _filled(dev, 32, n_kv, past, new, torch.float16, 11)
@@ -439,11 +439,12 @@ def test_attend_rows_cut_into_parts(dev, n_kv, past, new):
 
 
 @pytest.mark.parametrize("n_q,n_kv,new", [(32, 8, [8, 5, 6, 7]), (32, 8, [9, 8, 33, 40]), (32, 4, [3, 4, 5, 2]), (8, 8, [17, 31, 32, 33]),
-                                          (4, 2, [16, 9, 17, 8])])
+                                          (4, 2, [16, 9, 17, 8]), (4, 2, [16, 9, 13, 8]), (32, 8, [16, 9, 12, 3]), (32, 4, [8, 5, 7, 6]),
+                                          (8, 8, [33, 64, 1, 49]), (8, 8, [65, 64, 1, 49])])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_attend_tiles_around_17_to_32_rows(dev, dtype, n_q, n_kv, new):
-    """Drafts, and ends of chunks: more rows than one set, up to two of them, one
-    beyond; cut into parts and not; calls with fewer tokens than the plan's."""
+def test_attend_tiles_around_17_to_64_rows(dev, dtype, n_q, n_kv, new):
+    """Drafts, and ends of chunks: more rows than one set, up to two and four of
+    them, one beyond; cut into parts and not; calls with fewer tokens than the plan's."""
     for past in ([0, 63, 64, 200], [1500, 10, 2000, 1100]):
         print(f"[attend4 sets] {dtype} q {n_q} kv {n_kv} {past} + {new}", flush=True)
         c, o, plan, ref, q = _filled(dev, n_q, n_kv, past, new, dtype, 17)
@@ -518,7 +519,7 @@ def test_attend_rejected_rows_and_padding(dev):
     assert z[0].any() and not z[1:].any()
 
 
-@pytest.mark.parametrize("max_new", [4, 8, 40])
+@pytest.mark.parametrize("max_new", [4, 8, 16, 40])
 def test_attend_rejected_rows_with_many_tokens(dev, max_new):
     """Rows with more tokens than the plan's rows may have keep them in the packed
     order, and get zeros there whichever tiles they are in."""
