@@ -440,7 +440,8 @@ def test_attend_rows_cut_into_parts(dev, n_kv, past, new):
 
 @pytest.mark.parametrize("n_q,n_kv,new", [(32, 8, [8, 5, 6, 7]), (32, 8, [9, 8, 33, 40]), (32, 4, [3, 4, 5, 2]), (8, 8, [17, 31, 32, 33]),
                                           (4, 2, [16, 9, 17, 8]), (4, 2, [16, 9, 13, 8]), (32, 8, [16, 9, 12, 3]), (32, 4, [8, 5, 7, 6]),
-                                          (8, 8, [33, 64, 1, 49]), (8, 8, [65, 64, 1, 49])])
+                                          (8, 8, [33, 64, 1, 49]), (8, 8, [65, 64, 1, 49]), (8, 8, [17, 31, 32, 5]), (32, 8, [8, 1, 6, 3]),
+                                          (32, 4, [3, 4, 1, 2])])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_attend_tiles_around_17_to_64_rows(dev, dtype, n_q, n_kv, new):
     """Drafts, and ends of chunks: more rows than one set, up to two and four of
@@ -628,7 +629,7 @@ def test_serving_loop_captured(dev):
     assert torch.equal(caches[0].pages, caches[1].pages)
 
 
-@pytest.mark.parametrize("past,new", [([9000, 300, 5000], [1, 1, 1]), ([7000, 20, 4000], [2, 250, 1])])
+@pytest.mark.parametrize("past,new", [([9000, 300, 5000], [1, 1, 1]), ([7000, 20, 4000], [2, 250, 1]), ([9000, 300, 5000], [8, 1, 5])])
 def test_layers_of_a_step_on_two_streams(dev, past, new):
     """attend and fetch of two layers at the same time."""
     print(f"[kv4 streams] {past} + {new}", flush=True)
