@@ -713,8 +713,12 @@ struct AttendCall {
   uint32_t groups;
   bool bf16;
 };
+inline int32_t* counters_at(const PlanLayout& l, int n_kv, void* workspace) {
+  return reinterpret_cast<int32_t*>((float*)workspace + few_floats(l, n_kv) + many_floats(l, n_kv));
+}
 inline int attend_call(AttendCall& call, const oi2_paged* c, const oi2_page_plan* p, int32_t dtype, int32_t n_tokens,
-                       const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes, hipStream_t st) {
+                       const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes, hipStream_t st,
+                       bool cleared = false) {
   call = AttendCall{};
   if (int rc = check_plan(c, p)) return rc;
   const bool zero = dtype & OI2_ZERO_LEFT_OUT;
@@ -757,9 +761,9 @@ inline int attend_call(AttendCall& call, const oi2_paged* c, const oi2_page_plan
   a.many.groups = (int)many;
   a.many.o = a.few.o + few_floats(l, c->n_kv);
   a.many.ml = a.many.o + (size_t)l.cap_parts_many * c->n_kv * kManyRows * kHeadD;
-  a.few.count = (int32_t*)(a.few.o + few_floats(l, c->n_kv) + many_floats(l, c->n_kv));
+  a.few.count = counters_at(l, c->n_kv, workspace);
   a.many.count = a.few.count + (size_t)l.cap_parts_few * c->n_kv;
-  if (need) {
+  if (need && !cleared) {
     const int n = (int)counters(l, c->n_kv);
     hipLaunchKernelGGL(k_clear, dim3((n + 1023) / 1024), dim3(1024), 0, st, a.few.count, n);
     OI2_CHECK_LAUNCH();

@@ -1053,11 +1053,10 @@ size_t oi2_attn_paged_workspace_bytes(const oi2_paged* c, int32_t max_tokens, in
   return paged_layout(n_tokens, c->n_q, c->n_kv, attend).total;
 }
 
-// append, attend: the cache's own.
+// four: a cache of 4 bits.
 static int attn_forward_paged(const uint16_t* x, int32_t n_tokens, const oi2_attn* w, float eps, const oi2_rotary* rotary,
                               const oi2_paged* c, const oi2_page_plan* p, int32_t layer, uint16_t* out, uint16_t* x_out,
-                              void* workspace, size_t workspace_bytes, void* stream, decltype(&oi2_kv_append) append,
-                              decltype(&oi2_kv_attend) attend_call) {
+                              void* workspace, size_t workspace_bytes, void* stream, bool four) {
   if (int rc = check_plan(c, p)) return rc;
   if (int rc = check_rotary(rotary)) return rc;
   OI2_CHECK_ARG(rotary->head_dim == kHd, "rotary head_dim %d, expected %d", rotary->head_dim, kHd);
@@ -1127,10 +1126,18 @@ static int attn_forward_paged(const uint16_t* x, int32_t n_tokens, const oi2_att
     launch_gemv(a, n_tokens, w->n_q + 2 * w->n_kv, st);
   }
   OI2_CHECK_LAUNCH();
-  if (int rc = append(c, p, layer, OI2_DTYPE_F16, n_tokens, &k, &v, rotary, &q, qb, stream)) return rc;
-  if (int rc = attend_call(c, p, layer, OI2_DTYPE_F16, n_tokens, &q, 1.0f / sqrtf((float)kHd), attn, ws + L.attend, attend,
-                           stream))
-    return rc;
+  const float scale = 1.0f / sqrtf((float)kHd);
+  int rc;
+  if (four) {
+    int32_t* count;
+    const int n = kv4_counters(c, p, ws + L.attend, &count);
+    rc = kv4_append(c, p, layer, OI2_DTYPE_F16, n_tokens, &k, &v, rotary, &q, qb, count, n, stream);
+    if (!rc) rc = kv4_attend(c, p, layer, OI2_DTYPE_F16, n_tokens, &q, scale, attn, ws + L.attend, attend, true, stream);
+  } else {
+    rc = oi2_kv_append(c, p, layer, OI2_DTYPE_F16, n_tokens, &k, &v, rotary, &q, qb, stream);
+    if (!rc) rc = oi2_kv_attend(c, p, layer, OI2_DTYPE_F16, n_tokens, &q, scale, attn, ws + L.attend, attend, stream);
+  }
+  if (rc) return rc;
   if (prompt) {
     ProjArgs a{};
     a.w0 = w->wo;
@@ -1164,8 +1171,7 @@ int oi2_attn_forward_paged(const uint16_t* x, int32_t n_tokens, const oi2_attn* 
   clear_error();
   OI2_CHECK_ARG(w && rotary, "null attention weights or rotary frequencies");
   if (int rc = check_paged(c, layer, true)) return rc;
-  return attn_forward_paged(x, n_tokens, w, eps, rotary, c, p, layer, out, x_out, workspace, workspace_bytes, stream,
-                            oi2_kv_append, oi2_kv_attend);
+  return attn_forward_paged(x, n_tokens, w, eps, rotary, c, p, layer, out, x_out, workspace, workspace_bytes, stream, false);
 }
 
 int oi2_kv4_attn_forward(const uint16_t* x, int32_t n_tokens, const oi2_attn* w, float eps, const oi2_rotary* rotary,
@@ -1174,8 +1180,7 @@ int oi2_kv4_attn_forward(const uint16_t* x, int32_t n_tokens, const oi2_attn* w,
   clear_error();
   OI2_CHECK_ARG(w && rotary, "null attention weights or rotary frequencies");
   if (int rc = check_paged4(c, layer)) return rc;
-  return attn_forward_paged(x, n_tokens, w, eps, rotary, c, p, layer, out, x_out, workspace, workspace_bytes, stream,
-                            oi2_kv4_append, oi2_kv4_attend);
+  return attn_forward_paged(x, n_tokens, w, eps, rotary, c, p, layer, out, x_out, workspace, workspace_bytes, stream, true);
 }
 
 }  // extern "C"

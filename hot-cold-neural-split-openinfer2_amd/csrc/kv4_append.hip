@@ -28,6 +28,8 @@ struct Append4Args {
   int64_t token_stride[2], head_stride[2];
   int q_wide;
   uint8_t* pages;             // of the layer
+  int32_t* clear;             // n_clear ints
+  int n_clear;
   RotaryArgs rope;            // q's tensors; its frequencies serve k too
 };
 
@@ -199,6 +201,7 @@ __device__ __forceinline__ void append4(const Append4Args& a, int b) {
 template <bool BF16, bool WIDE, Turns TURNS>
 __global__ __launch_bounds__(256) void k_kv4_append(Append4Args a) {
   const int b = blockIdx.x;
+  for (int i = 256 * b + threadIdx.x; i < a.n_clear; i += 256 * gridDim.x) a.clear[i] = 0;
   if (b < a.groups) append4<BF16, WIDE, TURNS>(a, b);
   else if constexpr (TURNS != kNone) {
     if (a.q_wide) rotate_tokens<BF16, true, 256, true>(a.rope, b - a.groups);
@@ -227,14 +230,8 @@ int check_paged4(const oi2_paged* c, int32_t layer) {
   return OI2_OK;
 }
 
-}  // namespace oi2
-
-using namespace oi2;
-
-extern "C" int oi2_kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
-                              const oi2_heads* k, const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q,
-                              void* q_out, void* stream) {
-  clear_error();
+int kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens, const oi2_heads* k,
+               const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q, void* q_out, int32_t* clear, int n_clear, void* stream) {
   if (int rc = check_paged4(c, layer)) return rc;
   if (int rc = check_plan(c, p)) return rc;
   bool zero;
@@ -245,6 +242,8 @@ extern "C" int oi2_kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_
   a.n_kv = c->n_kv;
   a.n_pages = c->n_pages;
   a.n_tokens = n_tokens;
+  a.clear = clear;
+  a.n_clear = n_clear;
   bool wide = true;
   const oi2_heads* in[2] = {k, v};
   for (int w = 0; w < 2; ++w) {
@@ -280,4 +279,13 @@ extern "C" int oi2_kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_
   else launch_append4<false, false>(a, turns, groups, st);
   OI2_CHECK_LAUNCH();
   return OI2_OK;
+}
+
+}  // namespace oi2
+
+extern "C" int oi2_kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
+                              const oi2_heads* k, const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q,
+                              void* q_out, void* stream) {
+  oi2::clear_error();
+  return oi2::kv4_append(c, p, layer, dtype, n_tokens, k, v, r, q, q_out, nullptr, 0, stream);
 }

@@ -373,18 +373,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_kv4_attend(AttendArgs a) {
 }
 
 }  // namespace
-}  // namespace oi2
 
-using namespace oi2;
+int kv4_counters(const oi2_paged* c, const oi2_page_plan* p, void* workspace, int32_t** at) {
+  const PlanLayout l = plan_layout(*c, p->max_tokens, p->max_new);
+  *at = counters_at(l, c->n_kv, workspace);
+  return (int)counters(l, c->n_kv);
+}
 
-extern "C" int oi2_kv4_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
-                              const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes,
-                              void* stream) {
-  clear_error();
+int kv4_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens, const oi2_heads* q, float scale,
+               void* out, void* workspace, size_t workspace_bytes, bool cleared, void* stream) {
   if (int rc = check_paged4(c, layer)) return rc;
   hipStream_t st = (hipStream_t)stream;
   AttendCall call;
-  if (int rc = attend_call(call, c, p, dtype, n_tokens, q, scale, out, workspace, workspace_bytes, st)) return rc;
+  if (int rc = attend_call(call, c, p, dtype, n_tokens, q, scale, out, workspace, workspace_bytes, st, cleared)) return rc;
   if (!call.groups) return OI2_OK;
   AttendArgs& a = call.a;
   a.pages = c->pages + (size_t)layer * c->n_pages * c->n_kv * k4Block;
@@ -398,4 +399,13 @@ extern "C" int oi2_kv4_attend(const oi2_paged* c, const oi2_page_plan* p, int32_
   else hipLaunchKernelGGL(k_kv4_attend_few<false>, grid, block, 0, st, a);
   OI2_CHECK_LAUNCH();
   return OI2_OK;
+}
+
+}  // namespace oi2
+
+extern "C" int oi2_kv4_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens,
+                              const oi2_heads* q, float scale, void* out, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  oi2::clear_error();
+  return oi2::kv4_attend(c, p, layer, dtype, n_tokens, q, scale, out, workspace, workspace_bytes, false, stream);
 }

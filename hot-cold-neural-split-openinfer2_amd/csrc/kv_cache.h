@@ -88,6 +88,16 @@ inline PlanLayout plan_layout(const oi2_paged& c, int32_t n_tokens, int32_t max_
 int check_paged(const oi2_paged* c, int32_t layer, bool pool);
 int check_plan(const oi2_paged* c, const oi2_page_plan* p);
 int check_paged4(const oi2_paged* c, int32_t layer);     // of the 4-bit cache, which has no scales besides its pages
+
+// The 4-bit cache's append and attention as one call's: the append clears the
+// attention's counters, n_clear ints at `clear`, which then launches once
+// (`cleared`).  kv4_counters: how many a workspace has, and where.
+int kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens, const oi2_heads* k,
+               const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q, void* q_out, int32_t* clear, int n_clear, void* stream);
+int kv4_attend(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, int32_t dtype, int32_t n_tokens, const oi2_heads* q, float scale,
+               void* out, void* workspace, size_t workspace_bytes, bool cleared, void* stream);
+int kv4_counters(const oi2_paged* c, const oi2_page_plan* p, void* workspace, int32_t** at);
+
 int check_append(const oi2_paged* c, const oi2_page_plan* p, int32_t& dtype, bool& zero, int32_t n_tokens, const oi2_heads* k,
                  const oi2_heads* v, const oi2_rotary* r, const oi2_heads* q, const void* q_out);
 

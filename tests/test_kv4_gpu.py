@@ -545,7 +545,7 @@ def test_attend_rejected_rows_with_many_tokens(dev, max_new):
 # ── together ─────────────────────────────────────────────────────────────────
 
 @pytest.mark.parametrize("n_kv", [8, 32])
-@pytest.mark.parametrize("past,new", [([5], [1]), ([200, 64, 7], [1, 1, 1]), ([0, 130, 63, 9, 1], [1, 2, 0, 1, 1]),
+@pytest.mark.parametrize("past,new", [([5], [1]), ([200, 64, 7], [1, 1, 1]), ([3000, 70], [1, 1]), ([2500, 1300], [7, 130]), ([1800], [8]), ([0, 130, 63, 9, 1], [1, 2, 0, 1, 1]),
                                       ([0, 300], [70, 1]), ([40, 0, 100], [3, 190, 1])])
 def test_layer_over_pages(dev, n_kv, past, new):
     """GroupedQueryAttention.forward_paged: the pages are append's of the same
@@ -556,10 +556,11 @@ def test_layer_over_pages(dev, n_kv, past, new):
     rows, n_pages = len(past), sum(P8.pages_of(a + b) for a, b in zip(past, new))
     attn = oi2.GroupedQueryAttention(0, w, _cfg(n_kv))
     rot = oi2.Rotary(D, 1e4, device=dev)
-    c, c2 = (oi2.PagedKVCache(2, N_Q, n_kv, rows, 400, n_pages, device=dev, bits=4) for _ in range(2))
-    o = P.Cache4(rows, 400, n_pages, n_kv)
+    most = max(400, *(a + b for a, b in zip(past, new)))
+    c, c2 = (oi2.PagedKVCache(2, N_Q, n_kv, rows, most, n_pages, device=dev, bits=4) for _ in range(2))
+    o = P.Cache4(rows, most, n_pages, n_kv)
     wq, _, _, wo, nw = _dense(w)
-    one, zero = torch.ones((1000, D // 2), device=dev), torch.zeros((1000, D // 2), device=dev)
+    one, zero = torch.ones((4000, D // 2), device=dev), torch.zeros((4000, D // 2), device=dev)
     for step in (past, new):
         n = sum(step)
         plan, p2 = (x.extend(step, x.new_plan(n + 3, max_new=max(step))) for x in (c, c2))
@@ -569,6 +570,10 @@ def test_layer_over_pages(dev, n_kv, past, new):
         out = attn.forward_paged(x, c, plan, rot, layer=1, residual_out=resid)
         assert torch.equal(resid, (x.float() + out.float()).half())
         assert not out[n:].any()
+        # counters of parts are cleared whatever the workspace's memory held; the step is coded again, to the same
+        dirty = torch.full((64 << 20,), 255, dtype=torch.uint8, device=dev)
+        del dirty
+        assert torch.equal(attn.forward_paged(x, c, plan, rot, layer=1), out)
         _, (k, v) = oi2.GroupedQueryAttention(0, w, _cfg(n_kv))(x[None], one, zero)
         c2.append(1, k[0].transpose(0, 1), v[0].transpose(0, 1), p2, rotary=rot)
         assert torch.equal(c.pages, c2.pages)
