@@ -28,7 +28,7 @@ struct Append4Args {
   int64_t token_stride[2], head_stride[2];
   int q_wide;
   uint8_t* pages;             // of the layer
-  int32_t* clear;             // n_clear ints
+  int32_t* clear;             // n_clear ints for the attention behind it
   int n_clear;
   RotaryArgs rope;            // q's tensors; its frequencies serve k too
 };
