@@ -179,24 +179,41 @@ __global__ __launch_bounds__(kThreads, 8) void k_kv4_fetch(FetchArgs a) {
   }
 }
 
-// Whether no two of the (tokens, heads, 128) values at h share memory.
-bool apart(const oi2_heads* h, int64_t tokens) {
-  const int64_t st = h->token_stride, sh = h->head_stride, nh = h->heads;
-  if (st < 0 || sh < 0) return false;
-  if (tokens <= 1) return nh <= 1 || sh >= kHeadD;
-  if (nh <= 1) return st >= kHeadD;
-  return (sh >= kHeadD && st >= (nh - 1) * sh + kHeadD) || (st >= kHeadD && sh >= (tokens - 1) * st + kHeadD);
+// Whether two different ones of (tokens, heads, 128) values share memory, or, with
+// from != 0, one of them and one of the same values `from` elements further on:
+// those dt tokens and dh heads apart are from + dt st + dh sh elements apart.
+bool touch(int64_t tokens, int64_t heads, int64_t st, int64_t sh, int64_t from) {
+  constexpr int64_t near = kHeadD - 1;
+  for (int64_t dh = 1 - heads; dh < heads; ++dh) {
+    const int64_t d = from + dh * sh;
+    if (d >= -near && d <= near && (dh || from || (tokens > 1 && !st))) return true;
+    if (tokens < 2 || !st) continue;
+    // dt = 0 is done; the others nearest to -d / st
+    int64_t dt = -d / st;
+    dt = dt < 1 - tokens ? 1 - tokens : dt > tokens - 1 ? tokens - 1 : dt;
+    for (int64_t x = dt - 1; x <= dt + 1; ++x)
+      if (x && x > -tokens && x < tokens && d + x * st >= -near && d + x * st <= near) return true;
+  }
+  return false;
 }
 
-// Whether those at k and at v do: where their spans meet, only values that lie
-// alike, one behind the other within a token, are taken for apart.
+// Whether no two of the (tokens, heads, 128) values at h share memory.
+bool apart(const oi2_heads* h, int64_t tokens) {
+  const int64_t st = tokens > 1 ? h->token_stride : 0, sh = h->heads > 1 ? h->head_stride : 0, nh = h->heads;
+  if (st < 0 || sh < 0) return false;
+  if (tokens > 1 && nh > 1 && sh >= kHeadD && st >= (nh - 1) * sh + kHeadD) return true;
+  return !touch(tokens, nh, st, sh, 0);
+}
+
+// Whether those at k and at v do, or, with strides of their own, lie within one
+// another's span.
 bool meet(const oi2_heads* k, const oi2_heads* v, int64_t tokens, int size) {
-  auto span = [&](const oi2_heads* h) { return ((tokens - 1) * h->token_stride + (h->heads - 1) * h->head_stride + kHeadD) * size; };
+  const int64_t t = tokens - 1, h = k->heads - 1;
+  auto span = [&](const oi2_heads* x) { return (t * x->token_stride + h * x->head_stride + kHeadD) * size; };
   const uintptr_t a = (uintptr_t)k->data, b = (uintptr_t)v->data;
-  if (a + span(k) <= b || b + span(v) <= a) return false;
-  if (k->token_stride != v->token_stride || k->head_stride != v->head_stride || a == b) return true;
-  const int64_t apart = (int64_t)(a < b ? b - a : a - b), one = ((k->heads - 1) * k->head_stride + kHeadD) * size;
-  return apart < one || (tokens > 1 && apart + one > k->token_stride * size);
+  if (a + span(k) <= b || b + span(v) <= a || a == b) return a == b;
+  if ((t && k->token_stride != v->token_stride) || (h && k->head_stride != v->head_stride)) return true;
+  return touch(tokens, k->heads, t ? k->token_stride : 0, h ? k->head_stride : 0, (int64_t)(b - a) / size);
 }
 
 }  // namespace

@@ -281,8 +281,9 @@ class PagedKVCache:
         device, or anything that converts to that (a list waits for its copy).
         Tokens from max_tokens on are left out.  Rows past the last token are 0 in
         new tensors and not written in k_out and v_out, which may have any strides
-        that keep their values apart.  A cache of 4 bits; nothing waits on the
-        host."""
+        that keep their values apart, the same ones where they lie in one another's
+        span: slices of one buffer, whichever dimension comes first.  A cache of 4
+        bits; nothing waits on the host."""
         layer = self._layer(layer)
         if self.bits != 4:
             raise ValueError("fetch takes a cache of 4 bits; read() a row of either")

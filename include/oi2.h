@@ -620,10 +620,12 @@ int oi2_kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, in
 /* Positions [first[i], first[i] + count[i]) of row i, cut to what it holds
  * (negative values count as 0; first NULL: from 0), of all rows one behind the
  * other, as values: k and v (max_tokens, n_kv, 128) of `dtype` (OI2_DTYPE_F16,
- * _BF16 or _F32), with strides, non-negative, that keep all values apart.  first
- * and count (n_seqs) are device memory; cu (n_seqs + 1) gets the first token of
- * each row and the total.  Tokens from max_tokens on are left out; rows of k and v
- * past the last token are left as they were, or 0 with OI2_ZERO_LEFT_OUT. */
+ * _BF16 or _F32), with strides, non-negative, that keep all values apart, and the
+ * same ones for both where k and v lie in one another's span (as slices of one
+ * buffer in any order of its dimensions do).  first and count (n_seqs) are device
+ * memory; cu (n_seqs + 1) gets the first token of each row and the total.  Tokens
+ * from max_tokens on are left out; rows of k and v past the last token are left as
+ * they were, or 0 with OI2_ZERO_LEFT_OUT. */
 int oi2_kv4_fetch(const oi2_paged* c, int32_t layer, const int32_t* first, const int32_t* count, int32_t dtype,
                   int32_t max_tokens, const oi2_heads* k, const oi2_heads* v, int32_t* cu, void* stream);
 
