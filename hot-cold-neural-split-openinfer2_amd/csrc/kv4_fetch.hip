@@ -205,13 +205,17 @@ bool apart(const oi2_heads* h, int64_t tokens) {
   return !touch(tokens, nh, st, sh, 0);
 }
 
+// Bytes from the first of them to the last one's end.
+int64_t span(const oi2_heads* x, int64_t tokens, int size) {
+  return ((tokens - 1) * x->token_stride + (x->heads - 1) * x->head_stride + kHeadD) * size;
+}
+
 // Whether those at k and at v do, or, with strides of their own, lie within one
 // another's span.
 bool meet(const oi2_heads* k, const oi2_heads* v, int64_t tokens, int size) {
   const int64_t t = tokens - 1, h = k->heads - 1;
-  auto span = [&](const oi2_heads* x) { return (t * x->token_stride + h * x->head_stride + kHeadD) * size; };
   const uintptr_t a = (uintptr_t)k->data, b = (uintptr_t)v->data;
-  if (a + span(k) <= b || b + span(v) <= a || a == b) return a == b;
+  if (a + span(k, tokens, size) <= b || b + span(v, tokens, size) <= a || a == b) return a == b;
   if ((t && k->token_stride != v->token_stride) || (h && k->head_stride != v->head_stride)) return true;
   return touch(tokens, k->heads, t ? k->token_stride : 0, h ? k->head_stride : 0, (int64_t)(b - a) / size);
 }
@@ -246,8 +250,26 @@ extern "C" int oi2_kv4_fetch(const oi2_paged* c, int32_t layer, const int32_t* f
     }
     OI2_CHECK_ARG(!meet(k, v, max_tokens, size), "k and v share memory");
   }
-  auto in_cu = [&](const int32_t* x) { return x && x < cu + c->n_seqs + 1 && cu < x + c->n_seqs; };
-  OI2_CHECK_ARG(!in_cu(first) && !in_cu(count) && !in_cu(c->lens), "cu shares memory with what is read");
+  struct Range {
+    const void* at;
+    int64_t bytes;
+  };
+  auto cross = [](const Range& x, const Range& y) {
+    const uintptr_t a = (uintptr_t)x.at, b = (uintptr_t)y.at;
+    return a && b && a < b + y.bytes && b < a + x.bytes;
+  };
+  const int64_t rows = 4 * (int64_t)c->n_seqs, width = (c->max_len + kPage - 1) / kPage;
+  const Range sums = {cu, rows + 4};
+  const Range read[] = {{first, rows}, {count, rows}, {c->lens, rows}, {c->block_table, rows * width},
+                        {c->pages, (int64_t)c->n_layers * c->n_pages * c->n_kv * k4Block}};
+  for (const Range& r : read) OI2_CHECK_ARG(!cross(sums, r), "cu shares memory with what is read");
+  for (const oi2_heads* x : {k, v}) {
+    if (!max_tokens) break;
+    const Range out = {x->data, span(x, max_tokens, dtype == OI2_DTYPE_F32 ? 4 : 2)};
+    bool over = cross(out, sums);
+    for (const Range& r : read) over = over || cross(out, r);
+    OI2_CHECK_ARG(!over, "k or v shares memory with what is read, or with cu");
+  }
   a.table = c->block_table;
   a.lens = c->lens;
   a.first = first;
@@ -255,14 +277,14 @@ extern "C" int oi2_kv4_fetch(const oi2_paged* c, int32_t layer, const int32_t* f
   a.cu = cu;
   a.n_seqs = c->n_seqs;
   a.max_len = c->max_len;
-  a.width = (c->max_len + kPage - 1) / kPage;
+  a.width = (int)width;
   a.n_pages = c->n_pages;
   a.n_kv = c->n_kv;
   a.max_tokens = max_tokens;
   a.zero = zero;
   a.pages = c->pages + (size_t)layer * c->n_pages * c->n_kv * k4Block;
   // a page of one kv head is a workgroup's turn
-  const int64_t rows = c->n_seqs < max_tokens ? c->n_seqs : max_tokens, want = ((int64_t)max_tokens / kPage + 2 * rows) * c->n_kv;
+  const int64_t some = c->n_seqs < max_tokens ? c->n_seqs : max_tokens, want = ((int64_t)max_tokens / kPage + 2 * some) * c->n_kv;
   const uint32_t groups = (uint32_t)(want < 1 ? 1 : want < kMostGroups ? want : kMostGroups);
   const size_t lds = (size_t)c->n_seqs * 12;
   hipStream_t st = (hipStream_t)stream;

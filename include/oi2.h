@@ -625,7 +625,8 @@ int oi2_kv4_append(const oi2_paged* c, const oi2_page_plan* p, int32_t layer, in
  * buffer in any order of its dimensions do).  first and count (n_seqs) are device
  * memory; cu (n_seqs + 1) gets the first token of each row and the total.  Tokens
  * from max_tokens on are left out; rows of k and v past the last token are left as
- * they were, or 0 with OI2_ZERO_LEFT_OUT. */
+ * they were, or 0 with OI2_ZERO_LEFT_OUT.  Outputs may not share memory with each
+ * other or with what is read. */
 int oi2_kv4_fetch(const oi2_paged* c, int32_t layer, const int32_t* first, const int32_t* count, int32_t dtype,
                   int32_t max_tokens, const oi2_heads* k, const oi2_heads* v, int32_t* cu, void* stream);
 

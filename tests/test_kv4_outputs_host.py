@@ -81,3 +81,41 @@ def test_strides_of_their_own():
     assert _fetch((AT, 256, 5), (AT + 256, 256, 9), 8, 1) is None
     assert "share memory" in _fetch((AT, 5, 256), (AT + 254, 9, 256), 1, 8)
     assert "share memory" in _fetch((AT, 256, 128), (AT, 256, 128), 1, 1)
+
+
+READ = [("first", 4), ("count", 4), ("lens", 4), ("block_table", 4 * 16), ("cu", 5)]
+
+
+@pytest.mark.parametrize("what,ints", READ)
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_outputs_over_what_is_read(which, what, ints):
+    """k and v are refused where they share memory with counts, lengths, table or
+    sums, at either end; so are sums where the table lies.  4 rows of 16 pages."""
+    lib, ref = oi2.load_library(), ctypes.byref
+    tokens, heads, size = 8, 2, 8 * 2 * 128 * 2
+    for at in (AT, AT + size - 4, AT - 4 * ints + 4, AT + 512):
+        where = dict(first=1024, count=2048, lens=3072, block_table=4096, cu=8192)
+        where[what] = at
+        c = _lib.Paged(n_q=heads, n_kv=heads, n_seqs=4, max_len=1000, n_pages=1, n_layers=1, block_table=where["block_table"],
+                       lens=where["lens"], free_pages=64, n_free=64, pages=1 << 20, scales=None)
+        other = _lib.Heads(AT << 1, heads, 256, 128)
+        mine = _lib.Heads(AT, heads, 256, 128)
+        k, v = (mine, other) if which == "k" else (other, mine)
+        rc = lib.oi2_kv4_fetch(ref(c), 0, where["first"], where["count"], _lib.DTYPE_F16, tokens, ref(k), ref(v), where["cu"], None)
+        assert rc == 1 and b"shares memory with what is read" in lib.oi2_last_error(), (at, lib.oi2_last_error())
+
+
+def test_outputs_over_the_pages():
+    lib, ref = oi2.load_library(), ctypes.byref
+    c = _lib.Paged(n_q=2, n_kv=2, n_seqs=4, max_len=1000, n_pages=3, n_layers=2, block_table=4096, lens=3072, free_pages=64, n_free=64,
+                   pages=1 << 20, scales=None)
+    end = (1 << 20) + 2 * 3 * 2 * 9216
+    k, v = _lib.Heads(AT, 2, 256, 128), _lib.Heads(AT << 1, 2, 256, 128)
+    for bad in ((1 << 20) - 4096 + 16, end - 16):
+        x = _lib.Heads(bad, 2, 256, 128)
+        for a, b in ((x, v), (k, x)):
+            assert lib.oi2_kv4_fetch(ref(c), 0, None, 2048, _lib.DTYPE_F16, 8, ref(a), ref(b), 8192, None) == 1
+            assert b"shares memory with what is read" in lib.oi2_last_error()
+    for cu in (end - 4, 4096 - 4, 4096 + 4 * 4 * 16 - 4):
+        assert lib.oi2_kv4_fetch(ref(c), 0, None, 2048, _lib.DTYPE_F16, 8, ref(k), ref(v), cu, None) == 1
+        assert b"cu shares memory with what is read" in lib.oi2_last_error()
