@@ -144,3 +144,61 @@ def test_chunks_beside_tokens_repeat_themselves(dev, dtype):
         junk = torch.full(((1 + i) << 24,), 255 if i % 2 else 1, dtype=torch.uint8, device=dev)
         del junk
         assert torch.equal(c.attend(0, q, plan), y), i
+
+
+def test_two_captured_steps_over_layers(dev):
+    """Two layers over rows cut into parts, captured as a step of single tokens and
+    as one of drafts and a chunk, replayed in turn with eager work between:
+    every replay equals the same calls made eagerly on a cache of its own."""
+    print("[kv4 layer graphs]", flush=True)
+    g = torch.Generator(device=dev).manual_seed(23)
+    attn = [oi2.GroupedQueryAttention(0, _weights(dev, 8, seed=30 + li), _cfg(8)) for li in range(2)]
+    rot = oi2.Rotary(D, 1e4, device=dev)
+    past, news = [2500, 63, 1400], [[1, 1, 1], [8, 0, 50]]
+    caches = [oi2.PagedKVCache(2, N_Q, 8, 3, 3000, 110, device=dev, bits=4) for _ in range(2)]
+    kv = [torch.randn((2, sum(past), 8, D), generator=g, device=dev).half() for _ in range(2)]
+    for c in caches:
+        p = c.extend(past, c.new_plan(sum(past)))
+        for li in range(2):
+            c.append(li, kv[li][0], kv[li][1], p, rotary=rot)
+    plans = [[c.new_plan(sum(n), max_new=max(n)) for n in news] for c in caches]
+    lens = [torch.tensor(n, dtype=torch.int32, device=dev) for n in news]
+    xs = [torch.zeros((sum(n), H), dtype=torch.float16, device=dev) for n in news]
+    back = torch.tensor(past, dtype=torch.int32, device=dev)
+
+    def step(c, plan, new, x):
+        c.extend(new, plan)
+        for li in range(2):
+            r = torch.empty_like(x)
+            attn[li].forward_paged(x, c, plan, rot, layer=li, residual_out=r)
+            x = r
+        return x
+
+    for i in range(2):                                 # eagerly once: nothing is loaded or set up while capturing
+        step(caches[1], plans[1][i], lens[i], xs[i])
+    caches[1].rewind(back)
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(caches[0], plans[0][i], lens[i], xs[i]))
+        graphs.append(graph)
+    for k in range(12):
+        for i in (k % 2, 1 - k % 2):
+            xs[i].copy_(torch.randn(xs[i].shape, generator=g, device=dev))
+            graphs[i].replay()
+            got = outs[i].clone()
+            want = step(caches[1], plans[1][i], lens[i], xs[i])
+            torch.cuda.synchronize()
+            assert torch.equal(got, want) and bool(torch.isfinite(got).all()), (k, i)
+            outs[i].zero_()
+        if k % 4 == 3:
+            for c in caches:
+                c.rewind(back)
+    # rows of the pool that the eager steps filled before are coded alike
+    n = [int(x) for x in caches[0].lens]
+    assert n == caches[1].lens.tolist()
+    for li in range(2):
+        for a, b in zip(*(c.fetch(li, n, sum(n))[:2] for c in caches)):
+            assert torch.equal(a, b)
