@@ -4,15 +4,23 @@
 // A group of 32 values has a scale of its own, so every token is coded by
 // itself: 16 lanes take a token of the packed order and kv head, 8 dims a lane;
 // the largest magnitude goes over four lanes.  A workgroup takes 16 tokens, the
-// next one another head's: those of 64 tokens and one head, which share lines of
-// a page, are 8 apart or a multiple, on one XCD.  q has workgroups of its own
-// behind them in the same launch.
+// next one other heads of them: those of 64 tokens and one head, which share lines
+// of a page, are as far apart as a set of tokens has workgroups (`chunks`).  Where
+// that is a multiple of 8 (8, 16 or 32 heads, one a workgroup) they are on one XCD;
+// elsewhere (4 heads; long rotated steps, whose workgroups take several heads)
+// lines are written in parts from several.  q has workgroups of its own behind
+// them in the same launch.
 //
 // Bound by the chain of slot, loads, reduction and stores for a step (24 tokens 6
-// us), by bytes for prompts, whose inputs are read past the caches: 5875 tokens of 8
-// heads 9.8 us (31 MB, behind 600 MB of writes; 14.0 without that).  Rotated, by the
-// fp64 turns: the same with q's 32 heads 34 us, with turns made by every thread
-// for its own dims instead of once a token 53.
+// us), by bytes for prompts: 5875 tokens of 8 heads 9.8 us (31 MB, behind 600 MB of
+// writes).  Rotated, by the fp64 turns: the same with q's 32 heads 34 us, with
+// turns made by every thread for its own dims instead of once a token 53.
+//
+// k, v and q are read by non-temporal loads, for calls whose inputs are no longer
+// in the caches: with cached ones the 9.8 us are 14.0, the rotated step's 34 are
+// 45.  In a captured layer, where the projection has just written them, cached
+// ones are as fast or little faster: a token 23.0 us a layer instead of 23.4, a
+// prompt of 512 75.6 instead of 76.0, of 2000 and of 5000 the same (236.5, 835).
 #include "capi_util.h"
 #include "kv4.h"
 #include "rotary.h"

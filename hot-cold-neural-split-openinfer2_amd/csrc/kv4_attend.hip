@@ -62,15 +62,19 @@ __device__ __forceinline__ void fix_scales(uint32_t (&s)[N], int pos, int kv_len
 // over 60 and 150 thousand 37.3 (34 and 34), 20 rows of 4 tokens 19.7 (18 and 18).
 // Besides: 4 us to the first scores, parts of unequal length, 4 for arrivals and
 // joins.  158 registers, three workgroups a CU: with two 48 tokens take 65, with
-// four (128 registers) 92.  Measured slower: pages two ahead (66.5), parts half as
-// long (64), equal shares of all pages (61.5, and 54 instead of 20 for the drafts),
-// a second launch that joins (the two long ones 41.4), the query loaded behind
-// the first page (59.2).
+// four (128 registers) 92.  Measured slower: pages two ahead (66.5), equal shares of
+// all pages (61.5, and 54 instead of 20 for the drafts), a second launch that joins
+// (the two long ones 41.4), the query loaded behind the first page (59.2).  Shorter
+// parts: every part halved 64 instead of 61 (an earlier form), the two long ones 46
+// instead of 40, the drafts 27.5 instead of 21; cut three times as fine only where
+// a step has 256 tiles or more 55.3 instead of 57.4, and nothing elsewhere.  That is
+// not done: the plan, which is laid out for either cache, cuts the rows.
 //
 // SETS: of 16 query rows.  Two where all rows have 17 to 32: a page is decoded
-// once for both, and 244 registers leave two workgroups a CU.  Drafts of 8 tokens
-// over 300 to 14000 positions 44 us instead of 91 the way of many rows, of 5 over
-// 200 to 4000 34 instead of 68.  33 to 64 rows stay there: 56 of them took 72.8
+// once for both, and 244 registers leave two workgroups a CU (126 scalars are kept
+// in lanes of vector registers; none goes to memory).  24 drafts of 8 tokens over
+// 300 to 14000 positions 44 us (110 MB, 2.5 TB/s) instead of 91 the way of many
+// rows, 40 of 5 over 200 to 4000 34 instead of 68.  33 to 64 rows stay there: 56 of them took 72.8
 // with four sets (414 registers) and 63.2 with two workgroups a tile, and there 65.
 template <bool BF16, int SETS>
 __device__ __forceinline__ bool attend_few(const AttendArgs& a, const Found& found, uint8_t* smem) {

@@ -4,13 +4,18 @@
 // One launch.  Every workgroup makes the rows' prefix sums for itself, in LDS (a
 // launch of its own for them would cost more than they do), and then takes
 // pages of one kv head, every so-many-th of what is read: what lies in a line of
-// memory, or in a page's scales, is read by one workgroup, and its position in
-// the table by scalar loads.
+// memory, or in a page's scales, is read by one workgroup.  A turn is a chain of a
+// search of the sums in LDS, the table's entry, the page and the stores.
 //
 // Bound by its bytes: 48 rows of up to 6000 positions, 82 MB of pages to 291 MB of
-// values, 62 us (6.0 TB/s; a copy reaches 5.1); with stores through the caches 91,
-// a page's heads by one workgroup 110.  A prompt or a few rows: the sums and one
-// turn, 7 us.
+// values, 62 us called again and again (6.0 TB/s; a copy reaches 5.1), 87 with the
+// pages out of the caches (4.3); a page's heads by one workgroup 110 instead of
+// 62.  A few rows: the sums and one turn, 7 us; 5875 tokens 10.
+//
+// Non-temporal stores: with cached ones those 48 rows take 91 us instead of 62.
+// With a kernel that reads the values behind it, 900 positions 8.9 us and 8.7 with
+// cached stores, 6000 22.0 and 21.6, 24000 48.3 and 45.8, 96000 213 and 224,
+// 288000 637 and 653 (8 heads, fp16, both kernels).
 #include "capi_util.h"
 #include "kv4.h"
 #include "rotary.h"
@@ -18,7 +23,8 @@
 namespace oi2 {
 namespace {
 
-// kMostGroups: as many workgroups as are resident at a time.
+// kMostGroups: as many workgroups as are resident at a time, eight a CU, while
+// their sums (12 bytes a row) leave room in LDS: up to 1700 rows or so.
 constexpr int kThreads = 256, kWaves = kThreads / 64, kMostGroups = 2048;
 
 struct FetchArgs {
