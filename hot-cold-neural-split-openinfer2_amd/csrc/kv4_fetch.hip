@@ -207,7 +207,9 @@ bool touch(int64_t tokens, int64_t heads, int64_t st, int64_t sh, int64_t from) 
 bool apart(const oi2_heads* h, int64_t tokens) {
   const int64_t st = tokens > 1 ? h->token_stride : 0, sh = h->heads > 1 ? h->head_stride : 0, nh = h->heads;
   if (st < 0 || sh < 0) return false;
-  if (tokens > 1 && nh > 1 && sh >= kHeadD && st >= (nh - 1) * sh + kHeadD) return true;
+  // dense in either order: nothing to count
+  if (sh >= kHeadD && st >= (nh - 1) * sh + kHeadD) return true;
+  if (st >= kHeadD && sh >= (tokens - 1) * st + kHeadD) return true;
   return !touch(tokens, nh, st, sh, 0);
 }
 
